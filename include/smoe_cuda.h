@@ -476,6 +476,144 @@ int smoe_cuda_decode_advance_batch(SmoeCudaCtx* ctx, SmoeSamplerRow* rows, uint3
                                    uint32_t hcap, const uint32_t* tokens, uint32_t batch,
                                    uint32_t* pos, const float* u_seq, uint32_t u_len);
 
+/* ---- Long-context serving: prompts of many sequences in one pass, a paged
+ * 4-bit KV cache, single-token attention over it and eviction from it. No
+ * counterpart in the reference, which keeps one fp32 ring per sequence
+ * (decode.hpp:34) and prefills one sequence at a time (prefill.cpp:82-465).
+ * All pointers are device pointers; calls are asynchronous on the context
+ * stream and allocate nothing, so they can be captured in a CUDA graph. Row
+ * ranges, lengths and page numbers are read on the device: one outside its
+ * buffer is skipped and raises SMOE_ERR_DEVICE at the next synchronize. */
+
+/* Attention of packed prompts. Sequence s has the q / out rows
+ * [cu_q[s], cu_q[s+1]) and the k / v rows [cu_k[s], cu_k[s+1]); query head h
+ * reads KV head h / (num_heads / num_kv_heads). With off = len_k - len_q
+ * (the keys that precede the first new token), row i of a sequence attends
+ * to keys j <= i + off when causal, and of those to j > i + off - window
+ * when window != 0 (window needs causal); to all keys otherwise:
+ *   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j]
+ * A row with no key (len_k < len_q, len_k 0) gives zeros and lse -inf. Keys,
+ * values and rows that a row does not attend to have no influence on it,
+ * whatever they hold (infinities and NaN included).
+ * bf16 operands and result, fp32 scores, statistics and accumulators; the
+ * probabilities are rounded to bf16 for the tensor cores.
+ * Strides in elements: row r of head h of q starts at q + r * q_row + h *
+ * q_head; strides are multiples of 8 and bases 16-byte aligned; head_dim
+ * contiguous, a multiple of 8, <= 128; <= 128 query heads per KV head. The
+ * rows of a call with equal arguments give equal bits. */
+typedef struct SmoeCudaPackedAttnArgs {
+    const uint16_t* q;            /* bf16 [total_q][num_heads][head_dim]     */
+    const uint16_t* k;            /* bf16 [total_k][num_kv_heads][head_dim]  */
+    const uint16_t* v;
+    uint16_t*       out;          /* bf16 [total_q][num_heads][head_dim]     */
+    float*          lse;          /* [total_q][num_heads] log sum exp, or NULL */
+    const uint32_t* cu_q;         /* [n_seqs + 1] first row of each sequence */
+    const uint32_t* cu_k;         /* [n_seqs + 1], NULL: cu_q                */
+    uint64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    uint32_t n_seqs, total_q, total_k;
+    uint32_t num_heads, num_kv_heads, head_dim;
+    uint32_t causal, window;
+    float    scale;
+} SmoeCudaPackedAttnArgs;
+int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* args);
+
+/* Paged 4-bit KV cache of one layer. A page holds SMOE_KV4_PAGE entries; its
+ * block of one KV head is contiguous, with head_dim / 64 groups:
+ *   K codes [group][entry][32 bytes]   2 codes per byte, LSB first
+ *   V codes [group][entry][32 bytes]
+ *   K       [group][entry] { bf16 scale, bf16 bias }
+ *   V       [group][entry] { bf16 scale, bf16 bias }
+ * (AFFINE-Q4 per 64 values: value = scale * code + bias). Entry e of sequence
+ * s is entry e % SMOE_KV4_PAGE of page table[s][e / SMOE_KV4_PAGE]; pages of
+ * different sequences are distinct. len (entries held before this step),
+ * seen (tokens ever appended) and table are shared by all layers and change
+ * once a step (smoe_cuda_kv4_advance). pos and score are per layer, paged
+ * like the blocks, and only needed for eviction. head_dim 64 or 128. */
+#define SMOE_KV4_PAGE 64
+typedef struct SmoeKv4Cache {
+    uint8_t*        blocks;       /* [n_pages][num_kv_heads][block bytes], 16-byte aligned */
+    const uint32_t* table;        /* [n_seqs][table_stride] page numbers     */
+    const uint32_t* len;          /* [n_seqs]                                */
+    const uint32_t* seen;         /* [n_seqs], or NULL: len                  */
+    uint32_t*       pos;          /* [n_pages][num_kv_heads][PAGE] token position of each entry, or NULL */
+    float*          score;        /* [n_pages][num_kv_heads][PAGE] accumulated weight, or NULL */
+    uint32_t n_pages, n_seqs, table_stride, num_kv_heads, head_dim;
+} SmoeKv4Cache;
+/* Bytes of one page of one KV head; 0 for an unsupported head_dim. */
+uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim);
+
+/* Packed K and V rows: sequence s has the rows [cu[s], cu[s+1]). Row r of KV
+ * head h of k starts at element r * k_row + h * k_head; strides multiples of
+ * 4, bases 16-byte aligned, head_dim contiguous. */
+typedef struct SmoeKv4Rows {
+    void*           k;            /* dtype [total][num_kv_heads][head_dim]   */
+    void*           v;
+    const uint32_t* cu;           /* [n_seqs + 1]                            */
+    uint64_t        k_row, k_head, v_row, v_head;
+    uint32_t        total;
+    int             dtype;        /* SMOE_DTYPE_F32 or SMOE_DTYPE_BF16       */
+} SmoeKv4Rows;
+/* Quantise the rows into the entries len[s], len[s] + 1, .. of each sequence:
+ * bias = bf16(min), scale = bf16((max - min) * (1/15)), code =
+ * clamp(round((x - bias) / scale), 0, 15) (0 when scale is not positive).
+ * pos (if given) gets seen[s], seen[s] + 1, ..; score (if given) 0. len and
+ * seen stay. */
+int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4Rows* rows);
+/* Write the values of the entries first[s], first[s] + 1, .. (first NULL: 0)
+ * into the rows of each sequence. */
+int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32_t* first,
+                       const SmoeKv4Rows* rows);
+
+/* One query token per sequence over its len[s] + extra entries (extra: those
+ * appended in this step): out[s][h] = sum_j p[h][j] v[j], p[h] =
+ * softmax_j(scale * q[s][h] . k[j]); zeros for a sequence without entries.
+ * score_out (optional, paged like cache->score, which it may be) gets
+ *   score_out[j] = decay * cache->score[j] + sum over the KV head's query
+ *   heads of p[h][j]     (decay 0 or cache->score NULL: without the first)
+ * for the attended entries; others stay. fp32 statistics and accumulators;
+ * the codes are exact tensor-core operands, probabilities and an fp32 q go
+ * in as sums of bf16 pieces, so results are good to about 2^-16. max_len: an
+ * upper limit of len[s] + extra, known to the host (it sizes the grid and
+ * the workspace; longer sequences are cut there and raise SMOE_ERR_DEVICE).
+ * workspace: smoe_cuda_kv4_attention_workspace bytes, 16-byte aligned, its
+ * contents free between calls. */
+typedef struct SmoeKv4AttnArgs {
+    const void*  q;               /* dtype [n_seqs][num_heads][head_dim]     */
+    void*        out;             /* dtype [n_seqs][num_heads][head_dim]     */
+    float*       score_out;
+    void*        workspace;
+    uint64_t     workspace_bytes;
+    uint64_t     q_row, out_row;  /* elements between sequences, multiples of 4 */
+    uint32_t     num_heads, extra, max_len;
+    int          dtype;           /* SMOE_DTYPE_F32 or SMOE_DTYPE_BF16       */
+    float        scale, decay;
+} SmoeKv4AttnArgs;
+/* 0 when no workspace is needed. Reads num_heads, max_len and score_out. */
+uint64_t smoe_cuda_kv4_attention_workspace(const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* args);
+int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* args);
+
+/* Cut every sequence with more than `keep` entries to `keep`, per KV head:
+ * the entries whose pos + recent >= seen[s] stay, and of the others the best
+ * by score (ties: the lowest entry; NaN is the lowest score; more recent ones
+ * than keep: the lowest entries of them). Kept entries below `keep` stay
+ * where they are; the j-th kept entry past it moves to the j-th free one
+ * below it, K, V, pos and score. Entries past `keep` are left as they are.
+ * pos_out / score_out NULL: pos and score are updated in place; else those of
+ * all entries below min(len, keep) are written there (distinct arrays, same
+ * layout) and cache->pos / score stay. len stays (smoe_cuda_kv4_advance cuts
+ * it). max_len: an upper limit of len, as above. Entries not yet counted in
+ * len take no part. */
+uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len);
+int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t keep, uint32_t recent,
+                        uint32_t max_len, uint32_t* pos_out, float* score_out, void* workspace,
+                        uint64_t workspace_bytes);
+
+/* End of a step, once for all layers: len[s] = min(len[s] + n, keep) (keep 0:
+ * no limit) and seen[s] += n (seen optional), n = cu[s+1] - cu[s], or
+ * n_each when cu is NULL. */
+int smoe_cuda_kv4_advance(SmoeCudaCtx* ctx, uint32_t* len, uint32_t* seen, uint32_t n_seqs,
+                          const uint32_t* cu, uint32_t n_each, uint32_t keep);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

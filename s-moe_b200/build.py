@@ -18,7 +18,7 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libsmoe_cuda.so")
 LIB_TRACE = os.path.join(HERE, "libsmoe_cuda_trace.so")
 SOURCES = [os.path.join(HERE, "csrc", "smoe_cuda.cu"), os.path.join(HERE, "csrc", "smoe_noalloc.cu"),
-           os.path.join(HERE, "csrc", "smoe_vault.cpp")]
+           os.path.join(HERE, "csrc", "smoe_vault.cpp"), os.path.join(HERE, "csrc", "smoe_serve.cu")]
 DEPS = SOURCES + [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + [
     os.path.join(ROOT, "include", "smoe_cuda.h")]
 
@@ -27,6 +27,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
     "-Xptxas", "-v",
+    "--threads", "4",
     "-lcublas",
 ]
 

@@ -1,0 +1,47 @@
+// serve.cuh - what the long-context serving entries (smoe_serve.cu) share:
+// the parts of the context they use, their launches, and the look-up of a
+// packed row's sequence.
+#pragma once
+#include <atomic>
+#include <cuda_runtime.h>
+
+#include "../../include/smoe_cuda.h"
+#include "smoe_common.cuh"
+
+namespace smoe {
+
+struct CtxView {
+    int device, num_sms;
+    size_t smem_optin;
+    cudaStream_t stream;
+    uint32_t* err;                       // device error word
+    std::atomic<uint64_t>* dispatches;
+};
+CtxView ctx_view(SmoeCudaCtx* c);                        // smoe_cuda.cu
+int ctx_fail(int code, const char* msg, long v);         // sets the message of the failure, returns code
+
+// Programmatic dependent launch: the next kernel of the stream may start its
+// set-up while this one runs; it waits for this one's end before it touches
+// memory. Every kernel of these entries calls both.
+SMOE_DEVINL void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+SMOE_DEVINL void pdl_acquire() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+SMOE_DEVINL void serve_err(uint32_t* err, uint32_t code) { atomicCAS(err, 0u, code); }
+
+// The sequence s with cu[s] <= row < cu[s + 1] (cu ascending, cu[0] = 0), by
+// one warp together: each step looks at 32 bounds, so 1024 sequences take
+// two dependent loads. n when there is none.
+SMOE_DEVINL uint32_t seq_of_row(const uint32_t* cu, uint32_t n, uint32_t row, uint32_t lane) {
+    uint32_t lo = 0, span = n;           // the answer is in [lo, lo + span)
+    while (span > 1) {
+        const uint32_t step = (span + 31) / 32, at = lo + min((lane + 1) * step, span);
+        const uint32_t past = __ballot_sync(0xffffffffu, __ldg(cu + at) <= row);   // bounds at or below the row
+        const uint32_t k = __popc(past);
+        if (k * step >= span) return n;
+        lo += k * step;
+        span = min(step, span - k * step);
+    }
+    return (span == 1 && __ldg(cu + lo) <= row && row < __ldg(cu + lo + 1)) ? lo : n;
+}
+
+}  // namespace smoe

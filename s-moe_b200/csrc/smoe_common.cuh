@@ -12,6 +12,8 @@ enum : uint32_t {
     SMOE_DEVERR_MBAR_TIMEOUT = 1,   // a bulk copy never completed
     SMOE_DEVERR_SPIN_TIMEOUT = 2,   // a cross-CTA or cross-GPU wait ran out
     SMOE_DEVERR_BAD_EXPERT = 3,     // an expert id >= the layer's expert count (slot skipped)
+    SMOE_DEVERR_BAD_RANGE = 4,      // a sequence's rows or length outside their buffer (skipped or cut)
+    SMOE_DEVERR_BAD_PAGE = 5,       // a cache entry past the page table, or a page number past the cache (skipped)
 };
 
 // Waits without a caller-given limit (the bulk-copy completions of the

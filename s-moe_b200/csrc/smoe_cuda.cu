@@ -18,6 +18,7 @@
 #include "sampler.cuh"
 #include "decode.cuh"
 #include "ffn_grouped.cuh"
+#include "serve.cuh"
 
 namespace {
 
@@ -574,6 +575,12 @@ uint64_t smoe_cuda_kernel_dispatches(const SmoeCudaCtx* c) { return c ? c->dispa
 }  // extern "C"
 
 namespace smoe {
+CtxView ctx_view(SmoeCudaCtx* c) { return {c->device, c->num_sms, c->smem_optin, c->stream, c->err, &c->dispatches}; }
+int ctx_fail(int code, const char* msg, long v) {
+    std::snprintf(g_err, sizeof(g_err), "%s (%ld)", msg, v);
+    return code;
+}
+
 __global__ void k_expf_ref(const float* x, float* y, uint32_t n) {
     for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x)
         y[i] = expf_ref(x[i]);

@@ -1,0 +1,163 @@
+// smoe_serve.cu - the long-context serving entries of include/smoe_cuda.h:
+// packed prompt attention and the 4-bit KV cache. Kernels live in
+// prompt_attn.cuh and kv4.cuh.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "serve.cuh"
+#include "kv4.cuh"
+#include "prompt_attn.cuh"
+
+namespace {
+
+using smoe::ctx_fail;
+using smoe::CtxView;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <typename... KArgs, typename... Args>
+int launch(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+    cudaLaunchConfig_t lc{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.gridDim = grid;
+    lc.blockDim = block;
+    lc.dynamicSmemBytes = smem;
+    lc.stream = c.stream;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&lc, kern, KArgs(args)...);
+    if (e != cudaSuccess) return ctx_fail(SMOE_ERR_CUDA, cudaGetErrorString(e), long(e));
+    *c.dispatches += 1;
+    return SMOE_OK;
+}
+
+// The cache a call names: shape, pointers and alignment.
+int check_cache(const SmoeKv4Cache* c, const char* what) {
+    if (!c || !c->blocks || !c->table || !c->len || c->n_pages == 0 || c->n_seqs == 0 || c->table_stride == 0 ||
+        c->num_kv_heads == 0)
+        return ctx_fail(SMOE_ERR_ARG, what, 0);
+    if (!smoe_cuda_kv4_block_bytes(c->head_dim))
+        return ctx_fail(SMOE_ERR_UNSUPPORTED, "the 4-bit cache takes head_dim 64 or 128", c->head_dim);
+    if (!aligned(c->blocks, 16)) return ctx_fail(SMOE_ERR_ARG, "cache blocks must be 16-byte aligned", 0);
+    if (c->n_seqs > 65535 || c->num_kv_heads > 65535)
+        return ctx_fail(SMOE_ERR_ARG, "at most 65535 sequences and KV heads", c->n_seqs);
+    return SMOE_OK;
+}
+
+int check_rows(const SmoeKv4Rows* r, const char* what) {
+    if (!r || !r->k || !r->v || !r->cu) return ctx_fail(SMOE_ERR_ARG, what, 0);
+    if (r->dtype != SMOE_DTYPE_F32 && r->dtype != SMOE_DTYPE_BF16)
+        return ctx_fail(SMOE_ERR_ARG, "rows are fp32 or bf16", r->dtype);
+    if (!aligned(r->k, 16) || !aligned(r->v, 16) || (r->k_row | r->k_head | r->v_row | r->v_head) % 4)
+        return ctx_fail(SMOE_ERR_ARG, "rows need 16-byte aligned bases and strides that are multiples of 4", 0);
+    return SMOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a) {
+    if (!ctx || !a || !a->cu_q || a->num_heads == 0 || a->num_kv_heads == 0 || a->num_heads % a->num_kv_heads ||
+        (a->window && !a->causal))
+        return ctx_fail(SMOE_ERR_ARG, "bad packed attention arguments", 0);
+    if (a->total_q == 0 || a->n_seqs == 0) return SMOE_OK;
+    if (!a->q || !a->out || (a->total_k && (!a->k || !a->v)))
+        return ctx_fail(SMOE_ERR_ARG, "packed attention: null operand", 0);
+    if (a->head_dim == 0 || a->head_dim > 128 || a->head_dim % 8)
+        return ctx_fail(SMOE_ERR_UNSUPPORTED, "packed attention takes head_dim <= 128, a multiple of 8", a->head_dim);
+    if (a->num_heads / a->num_kv_heads > 128)
+        return ctx_fail(SMOE_ERR_UNSUPPORTED, "at most 128 query heads per KV head", a->num_heads / a->num_kv_heads);
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) ||
+        (a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head | a->out_row | a->out_head) % 8)
+        return ctx_fail(SMOE_ERR_ARG, "packed attention needs 16-byte aligned bases and strides that are multiples of 8", 0);
+    const CtxView c = smoe::ctx_view(ctx);
+    return launch(c, smoe::k_attention_packed, dim3((a->total_q + 7) / 8, a->num_heads), dim3(256), 0, *a, c.err);
+}
+
+uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim) {
+    return head_dim == 64 || head_dim == 128 ? smoe::Kv4Geom(head_dim).block : 0;
+}
+
+int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4Rows* rows) {
+    if (!ctx) return ctx_fail(SMOE_ERR_ARG, "null context", 0);
+    int rc = check_cache(cache, "kv4_append: bad cache");
+    if (rc || (rc = check_rows(rows, "kv4_append: bad rows"))) return rc;
+    if (rows->total == 0) return SMOE_OK;
+    const CtxView c = smoe::ctx_view(ctx);
+    return launch(c, smoe::k_kv4_append, dim3((rows->total + 7) / 8), dim3(256), 0, smoe::Kv4Args{*cache, c.err}, *rows);
+}
+
+int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32_t* first, const SmoeKv4Rows* rows) {
+    if (!ctx) return ctx_fail(SMOE_ERR_ARG, "null context", 0);
+    int rc = check_cache(cache, "kv4_read: bad cache");
+    if (rc || (rc = check_rows(rows, "kv4_read: bad rows"))) return rc;
+    if (rows->total == 0) return SMOE_OK;
+    const CtxView c = smoe::ctx_view(ctx);
+    return launch(c, smoe::k_kv4_read, dim3((rows->total + 7) / 8), dim3(256), 0, smoe::Kv4Args{*cache, c.err}, first, *rows);
+}
+
+uint64_t smoe_cuda_kv4_attention_workspace(const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
+    if (!cache || !t) return 0;
+    const uint64_t stride = (uint64_t(t->max_len) + 63) / 64 * 64;
+    return uint64_t(cache->n_seqs) * t->num_heads * stride * 4;
+}
+
+int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
+    if (!ctx || !t) return ctx_fail(SMOE_ERR_ARG, "kv4_attention: null argument", 0);
+    int rc = check_cache(cache, "kv4_attention: bad cache");
+    if (rc) return rc;
+    if (!t->q || !t->out || t->num_heads == 0 || t->num_heads % cache->num_kv_heads || t->max_len > 0x7fffffffu)
+        return ctx_fail(SMOE_ERR_ARG, "kv4_attention: bad arguments", t->num_heads);
+    if (t->dtype != SMOE_DTYPE_F32 && t->dtype != SMOE_DTYPE_BF16)
+        return ctx_fail(SMOE_ERR_ARG, "kv4_attention: q and out are fp32 or bf16", t->dtype);
+    if (!aligned(t->q, 16) || !aligned(t->out, 16) || (t->q_row | t->out_row) % 4)
+        return ctx_fail(SMOE_ERR_ARG, "kv4_attention needs 16-byte aligned q and out and strides that are multiples of 4", 0);
+    const uint64_t need = smoe_cuda_kv4_attention_workspace(cache, t);
+    if (need && (!t->workspace || t->workspace_bytes < need || !aligned(t->workspace, 16)))
+        return ctx_fail(SMOE_ERR_ARG, "kv4_attention: workspace missing, too small or unaligned; bytes needed", long(need));
+    const CtxView c = smoe::ctx_view(ctx);
+    smoe::Kv4Attn p{{*cache, c.err}, *t, static_cast<float*>(t->workspace), (t->max_len + 63) / 64 * 64};
+    return launch(c, smoe::k_kv4_attention, dim3(cache->num_kv_heads, cache->n_seqs), dim3(256), 0, p);
+}
+
+uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len) {
+    // a pair moves at most min(keep, len - keep) <= len / 2 entries
+    return cache ? uint64_t(cache->n_seqs) * cache->num_kv_heads * (uint64_t(max_len / 2) * 2 + 4) * 4 : 0;
+}
+
+int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t keep, uint32_t recent, uint32_t max_len,
+                        uint32_t* pos_out, float* score_out, void* workspace, uint64_t workspace_bytes) {
+    if (!ctx) return ctx_fail(SMOE_ERR_ARG, "null context", 0);
+    int rc = check_cache(cache, "kv4_evict: bad cache");
+    if (rc) return rc;
+    if (!cache->pos || !cache->score) return ctx_fail(SMOE_ERR_ARG, "kv4_evict needs the cache's pos and score", 0);
+    if (keep == 0 || max_len > 0x7fffffffu) return ctx_fail(SMOE_ERR_ARG, "kv4_evict: bad keep or max_len", keep);
+    if (!pos_out != !score_out || pos_out == cache->pos || score_out == cache->score) {
+        // one of the two alone, or the cache's own array: in place is asked for with NULL
+        return ctx_fail(SMOE_ERR_ARG, "kv4_evict: pos_out and score_out are both NULL or both separate arrays", 0);
+    }
+    const uint64_t need = smoe_cuda_kv4_evict_workspace(cache, max_len);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return ctx_fail(SMOE_ERR_ARG, "kv4_evict: workspace missing, too small or unaligned; bytes needed", long(need));
+    const CtxView c = smoe::ctx_view(ctx);
+    const uint32_t cap = max_len / 2;
+    smoe::Kv4Evict p{{*cache, c.err}, keep, recent, max_len, pos_out, score_out, static_cast<uint32_t*>(workspace), cap, cap * 2 + 4};
+    const dim3 pairs(cache->num_kv_heads, cache->n_seqs);
+    if ((rc = launch(c, smoe::k_kv4_evict_select, pairs, dim3(smoe::kEvThreads), 0, p))) return rc;
+    const uint32_t work = std::max(std::min(keep, max_len) / 256u, 1u), pairs_n = pairs.x * pairs.y;
+    const uint32_t split = std::max(1u, std::min(work, uint32_t(c.num_sms) * 8u / pairs_n));
+    return launch(c, smoe::k_kv4_evict_move, dim3(split, pairs.x, pairs.y), dim3(256), 0, p);
+}
+
+int smoe_cuda_kv4_advance(SmoeCudaCtx* ctx, uint32_t* len, uint32_t* seen, uint32_t n_seqs, const uint32_t* cu,
+                          uint32_t n_each, uint32_t keep) {
+    if (!ctx || !len || n_seqs == 0) return ctx_fail(SMOE_ERR_ARG, "bad kv4_advance arguments", n_seqs);
+    return launch(smoe::ctx_view(ctx), smoe::k_kv4_advance, dim3((n_seqs + 255) / 256), dim3(256), 0, len, seen, n_seqs, cu,
+                  n_each, keep);
+}
+
+}  // extern "C"

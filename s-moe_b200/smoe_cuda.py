@@ -25,6 +25,7 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 MAX_ACTIVE = 16
 MAX_FFN_BATCH = 64
+KV4_PAGE = 64
 
 # Every symbol include/smoe_cuda.h declares (checked by the CPU tests).
 EXPORTS = [
@@ -44,6 +45,9 @@ EXPORTS = [
     "smoe_cuda_rope_tables", "smoe_cuda_attention_prefill_async",
     "smoe_cuda_vault_parse", "smoe_cuda_vault_expert", "smoe_cuda_vault_upload_layer", "smoe_cuda_vault_last_error",
     "smoe_cuda_moe_layer_shard",
+    "smoe_cuda_attention_packed", "smoe_cuda_kv4_block_bytes", "smoe_cuda_kv4_append", "smoe_cuda_kv4_read",
+    "smoe_cuda_kv4_attention_workspace", "smoe_cuda_kv4_attention", "smoe_cuda_kv4_evict_workspace",
+    "smoe_cuda_kv4_evict", "smoe_cuda_kv4_advance",
 ]
 
 
@@ -70,6 +74,36 @@ class AttnLayerArgs(C.Structure):
               [(n, C.c_uint32) for n in ("d_model", "q_dim", "kv_dim", "head_dim", "num_heads",
                                          "num_kv_heads", "slot", "valid", "attn_ctx")] + \
               [("attn_scale", C.c_float)]
+
+
+class PackedAttnArgs(C.Structure):
+    """SmoeCudaPackedAttnArgs (packed_attn_args makes one from torch tensors)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "cu_q", "cu_k")] + \
+              [(n, C.c_uint64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
+                                         "out_head")] + \
+              [(n, C.c_uint32) for n in ("n_seqs", "total_q", "total_k", "num_heads", "num_kv_heads", "head_dim",
+                                         "causal", "window")] + [("scale", C.c_float)]
+
+
+class Kv4Cache(C.Structure):
+    """SmoeKv4Cache (kv4_cache makes one from torch tensors)."""
+    _fields_ = [(n, C.c_void_p) for n in ("blocks", "table", "len", "seen", "pos", "score")] + \
+              [(n, C.c_uint32) for n in ("n_pages", "n_seqs", "table_stride", "num_kv_heads", "head_dim")]
+
+
+class Kv4Rows(C.Structure):
+    """SmoeKv4Rows (kv4_rows makes one from torch tensors)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "cu")] + \
+              [(n, C.c_uint64) for n in ("k_row", "k_head", "v_row", "v_head")] + \
+              [("total", C.c_uint32), ("dtype", C.c_int)]
+
+
+class Kv4AttnArgs(C.Structure):
+    """SmoeKv4AttnArgs (kv4_attn_args makes one from torch tensors)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "score_out", "workspace")] + \
+              [(n, C.c_uint64) for n in ("workspace_bytes", "q_row", "out_row")] + \
+              [(n, C.c_uint32) for n in ("num_heads", "extra", "max_len")] + \
+              [("dtype", C.c_int), ("scale", C.c_float), ("decay", C.c_float)]
 
 
 class EpHandle(C.Structure):
@@ -206,6 +240,18 @@ def lib():
         L.smoe_cuda_tiled_expert_bytes.argtypes = [u32, u32, u32]
         L.smoe_cuda_tiled_expert_bytes.restype = u64
         L.smoe_cuda_prepack_layer.argtypes = [vp, C.POINTER(MoeLayer), vp, u64, C.POINTER(MoeLayer)]
+        L.smoe_cuda_attention_packed.argtypes = [vp, C.POINTER(PackedAttnArgs)]
+        L.smoe_cuda_kv4_block_bytes.argtypes = [u32]
+        L.smoe_cuda_kv4_block_bytes.restype = u64
+        L.smoe_cuda_kv4_append.argtypes = [vp, C.POINTER(Kv4Cache), C.POINTER(Kv4Rows)]
+        L.smoe_cuda_kv4_read.argtypes = [vp, C.POINTER(Kv4Cache), vp, C.POINTER(Kv4Rows)]
+        L.smoe_cuda_kv4_attention_workspace.argtypes = [C.POINTER(Kv4Cache), C.POINTER(Kv4AttnArgs)]
+        L.smoe_cuda_kv4_attention_workspace.restype = u64
+        L.smoe_cuda_kv4_attention.argtypes = [vp, C.POINTER(Kv4Cache), C.POINTER(Kv4AttnArgs)]
+        L.smoe_cuda_kv4_evict_workspace.argtypes = [C.POINTER(Kv4Cache), u32]
+        L.smoe_cuda_kv4_evict_workspace.restype = u64
+        L.smoe_cuda_kv4_evict.argtypes = [vp, C.POINTER(Kv4Cache), u32, u32, u32, vp, vp, vp, u64]
+        L.smoe_cuda_kv4_advance.argtypes = [vp, vp, vp, u32, vp, u32, u32]
         L.smoe_cuda_debug_expf.argtypes = [vp, vp, u32, vp]
         L.smoe_cuda_canonical_from_u32.argtypes = [u32]
         L.smoe_cuda_canonical_from_u32.restype = f32
@@ -412,9 +458,165 @@ class Context:
         check(self.L.smoe_cuda_decode_advance_batch(self.h, ptr(rows), ptr(history), hcap, ptr(tokens), batch,
                                                     ptr(pos), ptr(u_seq), u_len), "decode_advance_batch")
 
+    # ---- long-context serving
+    def attention_packed(self, args: PackedAttnArgs):
+        check(self.L.smoe_cuda_attention_packed(self.h, C.byref(args)), "attention_packed")
+
+    def kv4_append(self, cache: Kv4Cache, rows: Kv4Rows):
+        check(self.L.smoe_cuda_kv4_append(self.h, C.byref(cache), C.byref(rows)), "kv4_append")
+
+    def kv4_read(self, cache: Kv4Cache, first, rows: Kv4Rows):
+        check(self.L.smoe_cuda_kv4_read(self.h, C.byref(cache), ptr(first), C.byref(rows)), "kv4_read")
+
+    def kv4_attention(self, cache: Kv4Cache, args: Kv4AttnArgs):
+        check(self.L.smoe_cuda_kv4_attention(self.h, C.byref(cache), C.byref(args)), "kv4_attention")
+
+    def kv4_evict(self, cache: Kv4Cache, keep, recent, max_len, workspace, pos_out=None, score_out=None):
+        """workspace: a torch tensor of at least kv4_evict_workspace(cache, max_len) bytes."""
+        check(self.L.smoe_cuda_kv4_evict(self.h, C.byref(cache), keep, recent, max_len, ptr(pos_out), ptr(score_out),
+                                         ptr(workspace), _nbytes(workspace)), "kv4_evict")
+
+    def kv4_advance(self, lens, seen, n_seqs, cu=None, n_each=1, keep=0):
+        check(self.L.smoe_cuda_kv4_advance(self.h, ptr(lens), ptr(seen), n_seqs, ptr(cu), n_each, keep),
+              "kv4_advance")
+
     def sample(self, logits, vocab, batch, rows, history, history_stride, tokens):
         check(self.L.smoe_cuda_sample(self.h, ptr(logits), vocab, batch, ptr(rows), ptr(history),
                                       history_stride, ptr(tokens)), "sample")
+
+
+def _nbytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _dtype_of(t) -> int:
+    import torch
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    raise TypeError(f"float32 or bfloat16 tensors are taken, not {t.dtype}")
+
+
+def _rows3(t, name):
+    """(row stride, head stride) of a [rows, heads, head_dim] tensor."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name}: [rows, heads, head_dim] with contiguous head_dim is taken")
+    return t.stride(0), t.stride(1)
+
+
+def _ints(t, name, n=None):
+    import torch
+    if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or (n is not None and t.numel() < n):
+        raise ValueError(f"{name}: a contiguous 32-bit integer tensor{'' if n is None else f' of {n} values'} is taken")
+    return ptr(t)
+
+
+def packed_attn_args(q, k, v, out, cu_q, cu_k=None, scale=None, causal=True, window=0, lse=None) -> PackedAttnArgs:
+    """Arguments of Context.attention_packed from torch tensors: q, out
+    [total_q, heads, head_dim], k, v [total_k, kv_heads, head_dim] (bf16, any
+    row and head strides), cu_q / cu_k [n_seqs + 1] int32, lse [total_q,
+    heads] fp32. scale: 1 / sqrt(head_dim) by default. The tensors must stay
+    alive while the structure is used."""
+    import torch
+    a = PackedAttnArgs()
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: bfloat16 is taken, not {t.dtype}")
+        setattr(a, name, ptr(t))
+        row, head = _rows3(t, name)
+        setattr(a, name + "_row", row)
+        setattr(a, name + "_head", head)
+    if out.shape != q.shape or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise ValueError("q and out, and k and v, have the same shape, and all the same head_dim")
+    if lse is not None:
+        if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2]:
+            raise ValueError("lse: a contiguous float32 [total_q, heads] tensor is taken")
+        a.lse = ptr(lse)
+    a.n_seqs = cu_q.numel() - 1
+    a.cu_q = _ints(cu_q, "cu_q")
+    a.cu_k = None if cu_k is None else _ints(cu_k, "cu_k", a.n_seqs + 1)
+    a.total_q, a.total_k = q.shape[0], k.shape[0]
+    a.num_heads, a.num_kv_heads, a.head_dim = q.shape[1], k.shape[1], q.shape[2]
+    a.causal, a.window = int(causal), window
+    a.scale = 1.0 / q.shape[2] ** 0.5 if scale is None else scale
+    return a
+
+
+def kv4_cache(blocks, table, lens, head_dim, seen=None, pos=None, score=None) -> Kv4Cache:
+    """A 4-bit cache from torch tensors: blocks [n_pages, kv_heads,
+    kv4_block_bytes(head_dim)] uint8, table [n_seqs, pages] int32, lens / seen
+    [n_seqs] int32, pos / score [n_pages, kv_heads, 64] int32 / fp32. The
+    tensors must stay alive while the structure is used."""
+    import torch
+    c = Kv4Cache()
+    if blocks.dtype != torch.uint8 or not blocks.is_contiguous() or blocks.dim() != 3 or \
+            blocks.shape[2] != kv4_block_bytes(head_dim):
+        raise ValueError("blocks: a contiguous uint8 [n_pages, kv_heads, kv4_block_bytes(head_dim)] tensor is taken")
+    if table.dim() != 2:
+        raise ValueError("table: [n_seqs, pages] is taken")
+    c.blocks = ptr(blocks)
+    c.n_pages, c.num_kv_heads, c.head_dim = blocks.shape[0], blocks.shape[1], head_dim
+    c.n_seqs, c.table_stride = table.shape
+    c.table, c.len = _ints(table, "table"), _ints(lens, "lens", c.n_seqs)
+    c.seen = None if seen is None else _ints(seen, "seen", c.n_seqs)
+    n = c.n_pages * c.num_kv_heads * KV4_PAGE
+    c.pos = None if pos is None else _ints(pos, "pos", n)
+    if score is not None:
+        if score.dtype != torch.float32 or not score.is_contiguous() or score.numel() < n:
+            raise ValueError("score: a contiguous float32 [n_pages, kv_heads, 64] tensor is taken")
+        c.score = ptr(score)
+    return c
+
+
+def kv4_block_bytes(head_dim: int) -> int:
+    """Bytes of one page of one KV head (raises for an unsupported head_dim)."""
+    b = int(lib().smoe_cuda_kv4_block_bytes(head_dim))
+    if b == 0:
+        raise SmoeCudaError("the 4-bit cache takes head_dim 64 or 128")
+    return b
+
+
+def kv4_rows(k, v, cu) -> Kv4Rows:
+    """K / V rows for kv4_append and kv4_read: [total, kv_heads, head_dim],
+    float32 or bfloat16, cu [n_seqs + 1] int32."""
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v have the same shape and type")
+    r = Kv4Rows()
+    r.k, r.v, r.cu = ptr(k), ptr(v), _ints(cu, "cu")
+    (r.k_row, r.k_head), (r.v_row, r.v_head) = _rows3(k, "k"), _rows3(v, "v")
+    r.total, r.dtype = k.shape[0], _dtype_of(k)
+    return r
+
+
+def kv4_attn_args(q, out, max_len, extra=0, scale=None, score_out=None, decay=1.0) -> Kv4AttnArgs:
+    """Arguments of Context.kv4_attention: q, out [n_seqs, heads, head_dim]
+    (float32 or bfloat16, heads contiguous); score_out: paged like the
+    cache's score array, which it may be."""
+    for name, t in (("q", q), ("out", out)):
+        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+            raise ValueError(f"{name}: [n_seqs, heads, head_dim] with contiguous heads is taken")
+    if q.shape != out.shape or q.dtype != out.dtype:
+        raise ValueError("q and out have the same shape and type")
+    a = Kv4AttnArgs()
+    a.q, a.out, a.q_row, a.out_row = ptr(q), ptr(out), q.stride(0), out.stride(0)
+    a.num_heads, a.extra, a.max_len, a.dtype = q.shape[1], extra, max_len, _dtype_of(q)
+    a.scale = 1.0 / q.shape[2] ** 0.5 if scale is None else scale
+    a.decay, a.score_out = decay, ptr(score_out)
+    return a
+
+
+def kv4_attention_workspace(cache: Kv4Cache, args: Kv4AttnArgs) -> int:
+    return int(lib().smoe_cuda_kv4_attention_workspace(C.byref(cache), C.byref(args)))
+
+
+def kv4_attn_set_workspace(args: Kv4AttnArgs, workspace) -> Kv4AttnArgs:
+    args.workspace, args.workspace_bytes = ptr(workspace) if workspace is not None else None, _nbytes(workspace)
+    return args
+
+
+def kv4_evict_workspace(cache: Kv4Cache, max_len: int) -> int:
+    return int(lib().smoe_cuda_kv4_evict_workspace(C.byref(cache), max_len))
 
 
 def _vault_bytes(vault):
