@@ -1,9 +1,11 @@
 // smoe_serve.cu - the long-context serving entries of include/smoe_cuda.h:
 // packed prompt attention and the 4-bit KV cache. Kernels live in
 // prompt_attn.cuh and kv4.cuh.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "serve.cuh"
 #include "kv4.cuh"
@@ -32,6 +34,49 @@ int launch(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size
     if (e != cudaSuccess) return ctx_fail(SMOE_ERR_CUDA, cudaGetErrorString(e), long(e));
     *c.dispatches += 1;
     return SMOE_OK;
+}
+
+// Raise a kernel's shared-memory limit once per (kernel, device).
+template <typename K>
+int smem_limit(const CtxView& c, K kern, size_t smem) {
+    static thread_local uint64_t done = 0;                        // one per kernel type and pointer list below
+    static thread_local const void* last = nullptr;
+    if (smem > c.smem_optin) return ctx_fail(SMOE_ERR_UNSUPPORTED, "kernel needs more shared memory than the device has", long(smem));
+    if (last == reinterpret_cast<const void*>(kern) && (c.device < 64 && (done >> c.device & 1))) return SMOE_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return ctx_fail(SMOE_ERR_CUDA, cudaGetErrorString(e), long(e));
+    if (last != reinterpret_cast<const void*>(kern)) done = 0;
+    last = reinterpret_cast<const void*>(kern);
+    if (c.device < 64) done |= uint64_t(1) << c.device;
+    return SMOE_OK;
+}
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// bf16 [rows][heads][head_dim] with the given strides (elements), read in
+// boxes of 64 columns x box_heads x box_rows, 128-byte swizzle, zeros outside.
+int map_rows(CUtensorMap* m, const void* base, uint32_t head_dim, uint32_t heads, uint32_t rows, uint64_t row, uint64_t head,
+             uint32_t box_heads, uint32_t box_rows) {
+    const EncodeTiled enc = encode_tiled();
+    if (!enc) return ctx_fail(SMOE_ERR_CUDA, "cuTensorMapEncodeTiled is missing", 0);
+    const cuuint64_t dims[3] = {head_dim, heads, rows};
+    const cuuint64_t strides[2] = {std::max<uint64_t>(head, 8) * 2, std::max<uint64_t>(row, 8) * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_rows}, one[3] = {1, 1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, one,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? SMOE_OK : ctx_fail(SMOE_ERR_ARG, "tensor map refused (strides too large?)", long(r));
 }
 
 // The cache a call names: shape, pointers and alignment.
@@ -74,8 +119,30 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
     if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) ||
         (a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head | a->out_row | a->out_head) % 8)
         return ctx_fail(SMOE_ERR_ARG, "packed attention needs 16-byte aligned bases and strides that are multiples of 8", 0);
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return ctx_fail(SMOE_ERR_ARG, "packed attention needs a finite scale >= 0", 0);
     const CtxView c = smoe::ctx_view(ctx);
-    return launch(c, smoe::k_attention_packed, dim3((a->total_q + 7) / 8, a->num_heads), dim3(256), 0, *a, c.err);
+    smoe::PackedArgs p{*a, a->num_heads / a->num_kv_heads, 0, std::max(a->scale * 1.4426950408889634f, 1e-35f), c.err};
+    // (a scale of 0 must still keep the masked scores' -inf: 1e-35 times any finite score is 0 to the exponential)
+    p.tokens = smoe::kPaRows / p.group;
+    CUtensorMap mq, mk, mv;
+    int rc = map_rows(&mq, a->q, a->head_dim, a->num_heads, a->total_q, a->q_row, a->q_head, p.group, p.tokens);
+    if (rc) return rc;
+    if (a->total_k) {
+        if ((rc = map_rows(&mk, a->k, a->head_dim, a->num_kv_heads, a->total_k, a->k_row, a->k_head, 1, smoe::kPaKeys)) ||
+            (rc = map_rows(&mv, a->v, a->head_dim, a->num_kv_heads, a->total_k, a->v_row, a->v_head, 1, smoe::kPaKeys)))
+            return rc;
+    } else {
+        mk = mv = mq;                            // no row has a key: never read
+    }
+    // at most one partial tile pair a sequence; the kernel counts them
+    const uint64_t ctas = (uint64_t(a->total_q) / (2 * p.tokens) + std::min(a->n_seqs, a->total_q)) * a->num_kv_heads;
+    if (ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_ARG, "packed attention: too many rows", long(a->total_q));
+    auto run = [&](auto kern, size_t smem) -> int {
+        const int r = smem_limit(c, kern, smem);
+        return r ? r : launch(c, kern, dim3(uint32_t(ctas)), dim3(smoe::kPaThreads), smem, mq, mk, mv, p);
+    };
+    return a->head_dim <= 64 ? run(smoe::k_attention_packed<64>, smoe::PackedSmem<64>::bytes())
+                             : run(smoe::k_attention_packed<128>, smoe::PackedSmem<128>::bytes());
 }
 
 uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim) {
