@@ -28,7 +28,7 @@ SMOE_DEVINL uint32_t kv4_page(const SmoeKv4Cache& c, uint32_t s, uint64_t e, uin
         serve_err(err, SMOE_DEVERR_BAD_PAGE);
         return ~0u;
     }
-    const uint32_t p = __ldg(c.table + size_t(s) * c.table_stride + e / kKvPage);
+    const uint32_t p = ld_plain(c.table + size_t(s) * c.table_stride + e / kKvPage);
     if (p >= c.n_pages) {
         serve_err(err, SMOE_DEVERR_BAD_PAGE);
         return ~0u;
@@ -42,8 +42,8 @@ SMOE_DEVINL uint32_t kv4_page(const SmoeKv4Cache& c, uint32_t s, uint64_t e, uin
 // group's loads (128 or 256 bytes) and stores (32) are whole sectors. A warp
 // takes two units of one row; the rows of a CTA are consecutive.
 SMOE_DEVINL float4 kv4_load4(const void* p, size_t at, int dtype) {
-    if (dtype == SMOE_DTYPE_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
+    if (dtype == SMOE_DTYPE_F32) return *(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
+    const uint2 u = *(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                        __uint_as_float(u.y & 0xffff0000u));
 }
@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(256) k_kv4_append(Kv4Args a, SmoeKv4Rows r) {
     if (row >= r.total) return;
     const uint32_t s = seq_of_row(r.cu, a.c.n_seqs, row, lane);
     if (s >= a.c.n_seqs) return;                 // rows past the last sequence
-    const uint32_t t = row - __ldg(r.cu + s);
-    const uint64_t e = uint64_t(__ldg(a.c.len + s)) + t;
+    const uint32_t t = row - ld_plain(r.cu + s);
+    const uint64_t e = uint64_t(ld_plain(a.c.len + s)) + t;
     const uint32_t page = kv4_page(a.c, s, e, a.err);
     if (page == ~0u) return;
     const uint32_t slot = uint32_t(e % kKvPage), units = a.c.num_kv_heads * 2 * G.ng;
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(Kv4Args a, SmoeKv4Rows r) {
                 uint32_t(__bfloat16_as_ushort(sb)) | uint32_t(__bfloat16_as_ushort(bb)) << 16;
             if (kv == 0 && g == 0) {
                 const size_t i = (size_t(page) * a.c.num_kv_heads + h) * kKvPage + slot;
-                if (a.c.pos) a.c.pos[i] = __ldg((a.c.seen ? a.c.seen : a.c.len) + s) + t;
+                if (a.c.pos) a.c.pos[i] = ld_plain((a.c.seen ? a.c.seen : a.c.len) + s) + t;
                 if (a.c.score) a.c.score[i] = 0.0f;
             }
         }
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* fir
     if (row >= r.total) return;
     const uint32_t s = seq_of_row(r.cu, a.c.n_seqs, row, lane);
     if (s >= a.c.n_seqs) return;
-    const uint64_t e = uint64_t(first ? __ldg(first + s) : 0u) + (row - __ldg(r.cu + s));
+    const uint64_t e = uint64_t(first ? ld_plain(first + s) : 0u) + (row - ld_plain(r.cu + s));
     const uint32_t page = kv4_page(a.c, s, e, a.err);
     if (page == ~0u) return;
     const uint32_t slot = uint32_t(e % kKvPage), units = a.c.num_kv_heads * 2 * G.ng;
@@ -130,16 +130,37 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* fir
 }
 
 // ---------------------------------------------------------------- attention
+// One query token per sequence. With a group's codes c (0..15), scales s and
+// biases b, and c' = c - 8, b' = b + 8 s:
+//   q . k = sum_g s_g (q_g . c'_g) + b'_g sum(q_g)
+//   sum_j p_j v_j = sum_j (p_j s_j) c'_j + sum_j p_j b'_j        (per group)
+// so the raw codes are the tensor cores' operands (c' is exact) and scales
+// and biases stay in fp32. q goes in as one (bf16 q) or two fp16 pieces, each
+// head scaled by a power of two so that its largest value is near 2^14; p s
+// as two bf16 pieces (its range is the values' own, too wide for fp16).
+// The entries are the M rows of both products and a KV head's query heads
+// the N columns (8 or 16), so a page is dequantised once for all of them.
+//
+// A CTA of 4 warps takes a stretch of pages of one (sequence, KV head), a
+// warp every fourth page: each warp copies its pages - one block, one bulk
+// copy - into a ring of its own, keeps its own running maximum and sums, and
+// the four are joined at the end. Bound by the cache's bytes.
+constexpr int kKaWarps = 4, kKaStages = 2;
+
 struct Kv4Attn {
     Kv4Args a;
     SmoeKv4AttnArgs t;
-    float* logits;                               // [n_seqs][num_heads][max_len rounded up to pages]
-    uint32_t stride;                             // floats of a logits row
+    uint32_t group, chunks;                      // query heads per KV head; CTAs of a KV head's query heads
+    uint32_t split_pages, splits;                // pages of a CTA, CTAs along a sequence of max_len
+    float* part;                                 // [n_seqs][num_heads][splits][head_dim + 2] (sums, maximum, sum), splits > 1 or weights
+    float* logits;                               // [n_seqs][num_kv_heads][row][gs] log2-scaled scores, with weights
+    uint32_t rows, gs;
+    float scale_log2;
 };
 
 // Entries of sequence s that the token attends to.
 SMOE_DEVINL uint32_t kv4_valid(const Kv4Attn& p, uint32_t s) {
-    const uint64_t n = uint64_t(__ldg(p.a.c.len + s)) + p.t.extra;
+    const uint64_t n = uint64_t(ld_plain(p.a.c.len + s)) + p.t.extra;
     if (n > p.t.max_len) {
         if (threadIdx.x == 0) serve_err(p.a.err, SMOE_DEVERR_BAD_RANGE);
         return p.t.max_len;
@@ -147,91 +168,479 @@ SMOE_DEVINL uint32_t kv4_valid(const Kv4Attn& p, uint32_t s) {
     return uint32_t(n);
 }
 
-SMOE_DEVINL float kv4_value(const uint8_t* blk, const Kv4Geom& G, uint32_t kv, uint32_t slot, uint32_t d) {
-    const uint32_t g = d >> 6, i = d & 63;
-    const uint32_t code = blk[G.codes(kv, g) + slot * 32 + (i >> 1)] >> (4 * (i & 1)) & 15u;
-    const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(kv, g) + slot * 4);
-    return fmaf(float(code), __uint_as_float(sb << 16), __uint_as_float(sb & 0xffff0000u));
+// 8 codes -> c - 8 as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c
+// are exact, and so is what the subtraction or the multiply-add makes of them.
+SMOE_DEVINL void kv4_half_codes(uint32_t w, uint32_t* r) {
+    constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u, ONE = 0x64006400u;
+    const uint32_t w8 = w >> 8;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[0]) : "r"(lop3_and_or(w, M0, ONE)), "r"(0x64086408u));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(lop3_and_or(w, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[2]) : "r"(lop3_and_or(w8, M0, ONE)), "r"(0x64086408u));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(lop3_and_or(w8, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
 }
+// Codes n = 0..3 of two entries (low and high halves of u) -> c - 8 as bf16 pairs.
+SMOE_DEVINL void kv4_bf16_codes(uint32_t u, uint32_t* r) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[n]) : "r"(lop3_and_or(u >> (4 * n), 0x000F000Fu, 0x43004300u)), "r"(0x43084308u));
+}
+SMOE_DEVINL void mma_f16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+SMOE_DEVINL void mma_bf16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+SMOE_DEVINL uint32_t movm_trans(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+SMOE_DEVINL float kv4_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+SMOE_DEVINL uint32_t cvt_bf16x2_rn(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+SMOE_DEVINL float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
+SMOE_DEVINL float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// One CTA per (KV head, sequence), its query heads one after the other:
-// scores of all entries, their maximum and sum, the weighted values.
-__global__ void __launch_bounds__(256) k_kv4_attention(Kv4Attn p) {
-    pdl_release();
-    pdl_acquire();
-    __shared__ float q[128], red[256];
+template <int NG, int NT>
+struct Kv4AttnSmem {
+    static constexpr uint32_t BLOCK = NG * 4608, HD = NG * 64, HEADS = NT * 8;
+    static constexpr uint32_t RING = 0, RING_BYTES = kKaWarps * kKaStages * BLOCK;
+    static constexpr uint32_t Q = RING + RING_BYTES;             // float [HEADS][HD + 4]
+    static constexpr uint32_t QROW = HD + 4;
+    static constexpr uint32_t QSUM = Q + HEADS * QROW * 4;       // float [NG][HEADS]
+    static constexpr uint32_t QINV = QSUM + NG * HEADS * 4;      // float [HEADS]: scale_log2 over the head's power of two
+    static constexpr uint32_t ML = QINV + HEADS * 4;             // float [warps][HEADS][2]
+    static constexpr uint32_t BAR = ML + kKaWarps * HEADS * 8;
+    static constexpr uint32_t BYTES = BAR + kKaWarps * kKaStages * 8;
+    static_assert(kKaWarps * HEADS * HD * 4 <= RING_BYTES, "the joined accumulators take the ring's place");
+};
+
+// NG groups of 64 (head_dim / 64), NT tiles of 8 query heads, QP pieces of q.
+template <int NG, int NT, int QP>
+__global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p) {
+    using SM = Kv4AttnSmem<NG, NT>;
+    constexpr uint32_t HD = SM::HD, HEADS = SM::HEADS;
+    extern __shared__ __align__(128) uint8_t kv4_smem[];
+    uint8_t* smem = kv4_smem;
     const SmoeKv4Cache& c = p.a.c;
-    const Kv4Geom G(c.head_dim);
-    const uint32_t kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, hd = c.head_dim;
-    const uint32_t group = p.t.num_heads / c.num_kv_heads, n = kv4_valid(p, s);
-    auto block_of = [&](uint32_t e) -> const uint8_t* {
-        const uint32_t page = kv4_page(c, s, e, p.a.err);
-        return page == ~0u ? nullptr : c.blocks + (size_t(page) * c.num_kv_heads + kvh) * G.block;
+    const Kv4Geom G(HD);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, cl = lane & 3;
+    const uint32_t split = blockIdx.x, kvh = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks, s = blockIdx.z;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR) + warp * kKaStages;
+    pdl_release();
+    if (lane == 0) {
+        for (int i = 0; i < kKaStages; ++i) mbar_init(bars + i, 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    pdl_acquire();
+    const uint32_t n = kv4_valid(p, s), pages = (n + kKvPage - 1) / kKvPage;
+    const uint32_t p0 = split * p.split_pages, p1 = min(pages, p0 + p.split_pages);
+    const uint32_t h0 = chunk * HEADS, heads = min(HEADS, p.group - h0);        // of this CTA, in the KV head's group
+    if (p0 >= p1 && !(n == 0 && p.splits == 1)) return;
+
+    // this warp's pages: p0 + warp, + 4, ..; their numbers are fetched 32 at a time
+    const uint32_t mine = p1 > p0 + warp ? (p1 - p0 - warp + kKaWarps - 1) / kKaWarps : 0u;
+    uint32_t ids = ~0u, ids_base = 0;
+    auto fetch_ids = [&](uint32_t base) {
+        ids_base = base;
+        ids = base + lane < mine ? kv4_page(c, s, uint64_t(p0 + warp + (base + lane) * kKaWarps) * kKvPage, p.a.err) : ~0u;
     };
-    for (uint32_t j = 0; j < group; ++j) {
-        const uint32_t h = kvh * group + j;
-        float* l = p.logits + (size_t(s) * p.t.num_heads + h) * p.stride;
-        __syncthreads();
-        if (tid < hd)
-            q[tid] = p.t.dtype == SMOE_DTYPE_F32
-                         ? static_cast<const float*>(p.t.q)[s * p.t.q_row + h * hd + tid]
-                         : bf16_bits_to_f32(static_cast<const uint16_t*>(p.t.q)[s * p.t.q_row + h * hd + tid]);
-        __syncthreads();
-        float m = -INFINITY;
-        for (uint32_t e = tid; e < n; e += 256) {
-            const uint8_t* blk = block_of(e);
-            float x = 0.0f;
-            for (uint32_t d = 0; blk && d < hd; ++d) x = fmaf(q[d], kv4_value(blk, G, 0, e % kKvPage, d), x);
-            x = blk ? x * p.t.scale : -INFINITY;
-            l[e] = x;
-            m = fmaxf(m, x);
+    if (mine) fetch_ids(0);
+    uint8_t* ring = smem + SM::RING + warp * kKaStages * SM::BLOCK;
+    auto issue = [&](uint32_t i) -> uint32_t {                   // whole warp; the page's number
+        if (i >= ids_base + 32) fetch_ids(i);
+        const uint32_t page = __shfl_sync(0xffffffffu, ids, i - ids_base);
+        if (lane == 0) {
+            if (page != ~0u) {
+                mbar_arrive_expect_tx(bars + i % kKaStages, SM::BLOCK);
+                bulk_g2s(ring + i % kKaStages * SM::BLOCK, c.blocks + (size_t(page) * c.num_kv_heads + kvh) * SM::BLOCK,
+                         SM::BLOCK, bars + i % kKaStages);
+            } else {
+                mbar_arrive(bars + i % kKaStages);               // nothing to wait for; its entries are masked
+            }
         }
-        red[tid] = m;
-        for (uint32_t o = 128; o; o >>= 1) {
-            __syncthreads();
-            if (tid < o) red[tid] = fmaxf(red[tid], red[tid + o]);
+        return page;
+    };
+    uint32_t good = 0;                                           // bit i % 32: page i can be read
+    for (uint32_t i = 0; i < uint32_t(kKaStages) && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
+
+    // q: fp32 in shared memory, each head times a power of two, its group sums
+    float* qs = reinterpret_cast<float*>(smem + SM::Q);
+    float* qsum = reinterpret_cast<float*>(smem + SM::QSUM);
+    float* qinv = reinterpret_cast<float*>(smem + SM::QINV);
+    for (uint32_t h = warp; h < HEADS; h += kKaWarps) {
+        float x[HD / 32], mx = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 32; ++i) {
+            const size_t at = s * p.t.q_row + (kvh * p.group + h0 + h) * HD + i * 32 + lane;
+            x[i] = h >= heads ? 0.0f : p.t.dtype == SMOE_DTYPE_F32 ? ld_plain(static_cast<const float*>(p.t.q) + at)
+                                                                    : bf16_bits_to_f32(ld_plain(static_cast<const uint16_t*>(p.t.q) + at));
+            mx = fmaxf(mx, fabsf(x[i]));
         }
-        __syncthreads();
-        m = red[0];
-        __syncthreads();
-        float sum = 0.0f;
-        for (uint32_t e = tid; e < n; e += 256) {
-            const float x = expf(l[e] - m);
-            l[e] = x;
-            sum += x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // 2^e with mx 2^e in [2^14, 2^15), kept within what fp32 can invert (an infinity or NaN in q stays one)
+        const int e = max(-100, min(100, 14 - (int(__float_as_uint(mx) >> 23) - 127)));
+        const float up = __uint_as_float(uint32_t(127 + e) << 23);
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 32; ++i) {
+            // the pieces that go to the tensor cores, and their sum
+            const float y = x[i] * up, hi = __half2float(__float2half_rn(y));
+            const float lo = QP == 2 ? __half2float(__float2half_rn(y - hi)) : 0.0f;
+            qs[h * SM::QROW + i * 32 + lane] = y;
+            x[i] = hi + lo;
         }
-        red[tid] = sum;
-        for (uint32_t o = 128; o; o >>= 1) {
-            __syncthreads();
-            if (tid < o) red[tid] += red[tid + o];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float t = x[2 * g] + x[2 * g + 1];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) qsum[g * HEADS + h] = t;
         }
-        __syncthreads();
-        const float inv = n ? 1.0f / red[0] : 0.0f;
-        __syncthreads();
-        float acc = 0.0f;
-        const uint32_t d = tid % hd, part = tid / hd, parts = 256 / hd;
-        for (uint32_t e = part; e < n; e += parts) {
-            const uint8_t* blk = block_of(e);
-            if (blk) acc = fmaf(l[e], kv4_value(blk, G, 1, e % kKvPage, d), acc);
-        }
-        red[tid] = acc;
-        __syncthreads();
-        if (tid < hd) {
-            for (uint32_t i = 1; i < parts; ++i) acc += red[tid + i * hd];
-            acc *= inv;
-            if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[s * p.t.out_row + h * hd + tid] = acc;
-            else static_cast<__nv_bfloat16*>(p.t.out)[s * p.t.out_row + h * hd + tid] = __float2bfloat16_rn(acc);
-        }
-        for (uint32_t e = tid; p.t.score_out && e < n; e += 256) l[e] *= inv;
+        if (lane == 0) qinv[h] = p.scale_log2 * __uint_as_float(uint32_t(127 - e) << 23);
     }
     __syncthreads();
-    for (uint32_t e = tid; p.t.score_out && e < n; e += 256) {
+    // this lane's fragments of q: head gr (+ 8), dimensions in the order kv4_half_codes gives the codes
+    uint32_t qf[NT][NG][4][QP][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const float* y = qs + (nt * 8 + gr) * SM::QROW + g * 64 + cl * 16 + st / 2 * 8 + st % 2 * 2 + b;
+                    const __half y0 = __float2half_rn(y[0]), y1 = __float2half_rn(y[4]);
+                    qf[nt][g][st][0][b] = pack_half2(y0, y1);
+                    if (QP == 2)
+                        qf[nt][g][st][QP - 1][b] = pack_half2(__float2half_rn(y[0] - __half2float(y0)), __float2half_rn(y[4] - __half2float(y1)));
+                }
+    float qsm[NT][NG][2], sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            sc[nt][k] = qinv[nt * 8 + 2 * cl + k];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsm[nt][g][k] = qsum[g * HEADS + nt * 8 + 2 * cl + k];
+        }
+
+    float m[NT][2], l[NT][2], bacc[NT][NG][2], o[NT][NG][4][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            m[nt][k] = -INFINITY;
+            l[nt][k] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                bacc[nt][g][k] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][g][i][k] = o[nt][g][i][2 + k] = 0.0f;
+            }
+        }
+    bool failed = false;
+    float* lrow = p.logits ? p.logits + ((size_t(s) * c.num_kv_heads + kvh) * p.rows) * p.gs : nullptr;
+#pragma unroll 1
+    for (uint32_t i = 0; i < mine; ++i) {
+        const uint8_t* blk = ring + i % kKaStages * SM::BLOCK;
+        if (!failed && !mbar_wait_bounded(bars + i % kKaStages, (i / kKaStages) & 1)) {
+            failed = true;                       // (the results are void, the error word says so)
+            atomicCAS(p.a.err, 0u, uint32_t(SMOE_DEVERR_MBAR_TIMEOUT));
+        }
+        const uint32_t e0 = (p0 + warp + i * kKaWarps) * kKvPage;
+        const uint32_t have = good >> (i % kKaStages) & 1u ? min(kKvPage, n - e0) : 0u;        // entries of this page
+        float x[4][NT][4];                       // scores: entry 16 mt + gr (0, 1) and + 8 (2, 3), heads 2 cl, 2 cl + 1
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            const uint32_t ka = mt * 16 + gr, kb = ka + 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[mt][nt][k] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint2 wa = *reinterpret_cast<const uint2*>(blk + G.codes(0, g) + ka * 32 + cl * 8);
+                const uint2 wb = *reinterpret_cast<const uint2*>(blk + G.codes(0, g) + kb * 32 + cl * 8);
+                const uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, g) + ka * 4);
+                const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, g) + kb * 4);
+                float d[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    uint32_t ra[4], rb[4];
+                    kv4_half_codes(w ? wa.y : wa.x, ra);
+                    kv4_half_codes(w ? wb.y : wb.x, rb);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t af[4] = {ra[2 * h], rb[2 * h], ra[2 * h + 1], rb[2 * h + 1]};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int q = 0; q < QP; ++q)
+                                mma_f16f32_16816(d[nt], af, qf[nt][g][w * 2 + h][q][0], qf[nt][g][w * 2 + h][q][1]);
+                    }
+                }
+                const float s0 = lo_f(sa), b0 = fmaf(8.0f, s0, hi_f(sa)), s1 = lo_f(sb), b1 = fmaf(8.0f, s1, hi_f(sb));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        x[mt][nt][k] = fmaf(s0, d[nt][k], fmaf(b0, qsm[nt][g][k], x[mt][nt][k]));
+                        x[mt][nt][2 + k] = fmaf(s1, d[nt][2 + k], fmaf(b1, qsm[nt][g][k], x[mt][nt][2 + k]));
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[mt][nt][k] = (k < 2 ? ka : kb) < have ? x[mt][nt][k] * sc[nt][k & 1] : -INFINITY;
+            if (lrow) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t h = nt * 8 + 2 * cl;
+                    float* at = lrow + size_t(e0 + ka) * p.gs + h0 + h;
+                    if (h < heads && e0 + ka < n) *reinterpret_cast<float2*>(at) = make_float2(x[mt][nt][0], x[mt][nt][1]);
+                    if (h < heads && e0 + kb < n) *reinterpret_cast<float2*>(at + size_t(8) * p.gs) = make_float2(x[mt][nt][2], x[mt][nt][3]);
+                }
+            }
+        }
+        // running maximum; moved only when it is 2^8 too low
+        float f[NT][2];
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float mx = x[0][nt][k];
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) mx = fmaxf(fmaxf(mx, x[mt][nt][k]), x[mt][nt][2 + k]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                f[nt][k] = 1.0f;
+                if (mx > m[nt][k] + 8.0f || (mx > m[nt][k] && m[nt][k] == -INFINITY)) {
+                    f[nt][k] = m[nt][k] == -INFINITY ? 0.0f : kv4_ex2(m[nt][k] - mx);
+                    m[nt][k] = mx;
+                    move = true;
+                }
+            }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    l[nt][k] *= f[nt][k];
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        bacc[nt][g][k] *= f[nt][k];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[nt][g][j][k] *= f[nt][k];
+                            o[nt][g][j][2 + k] *= f[nt][k];
+                        }
+                    }
+                }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            const uint32_t ka = mt * 16 + gr, kb = ka + 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float mm = m[nt][k & 1] == -INFINITY ? 0.0f : m[nt][k & 1];
+                    x[mt][nt][k] = kv4_ex2(x[mt][nt][k] - mm);
+                    l[nt][k & 1] += x[mt][nt][k];
+                }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                // entries past the last one may hold anything: their scales count as 0
+                const uint32_t sa = ka < have ? *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + ka * 4) : 0u;
+                const uint32_t sb = kb < have ? *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + kb * 4) : 0u;
+                const float s0 = lo_f(sa), b0 = fmaf(8.0f, s0, hi_f(sa)), s1 = lo_f(sb), b1 = fmaf(8.0f, s1, hi_f(sb));
+                // codes of this lane's 8 dimensions (8 gr ..) of the entries 2 cl, 2 cl + 1, 2 cl + 8, 2 cl + 9 of the tile;
+                // lanes cl >= 2 load the pair the other way round (the four entries of a load then lie in different banks)
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    w[k] = *reinterpret_cast<const uint32_t*>(blk + G.codes(1, g) + (mt * 16 + 2 * cl + ((k & 1) ^ (cl >> 1)) + (k >> 1) * 8) * 32 + gr * 4);
+                const uint32_t p_lo = cl < 2 ? 0x5410u : 0x1054u, p_hi = cl < 2 ? 0x7632u : 0x3276u;
+                uint32_t c0[8], c1[8];           // dimension n: entries (2 cl, 2 cl + 1), and + 8
+                kv4_bf16_codes(__byte_perm(w[0], w[1], p_lo), c0);
+                kv4_bf16_codes(__byte_perm(w[0], w[1], p_hi), c0 + 4);
+                kv4_bf16_codes(__byte_perm(w[2], w[3], p_lo), c1);
+                kv4_bf16_codes(__byte_perm(w[2], w[3], p_hi), c1 + 4);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    bacc[nt][g][0] = fmaf(x[mt][nt][0], b0, fmaf(x[mt][nt][2], b1, bacc[nt][g][0]));
+                    bacc[nt][g][1] = fmaf(x[mt][nt][1], b0, fmaf(x[mt][nt][3], b1, bacc[nt][g][1]));
+                    const float y0 = x[mt][nt][0] * s0, y1 = x[mt][nt][1] * s0, y2 = x[mt][nt][2] * s1, y3 = x[mt][nt][3] * s1;
+                    const uint32_t u0 = cvt_bf16x2_rn(y0, y1), u1 = cvt_bf16x2_rn(y2, y3);
+                    const uint32_t v0 = movm_trans(cvt_bf16x2_rn(y0 - lo_f(u0), y1 - hi_f(u0)));
+                    const uint32_t v1 = movm_trans(cvt_bf16x2_rn(y2 - lo_f(u1), y3 - hi_f(u1)));
+                    const uint32_t t0 = movm_trans(u0), t1 = movm_trans(u1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t af[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
+                        mma_bf16f32_16816(o[nt][g][j], af, t0, t1);
+                        mma_bf16f32_16816(o[nt][g][j], af, v0, v1);
+                    }
+                }
+            }
+        }
+        __syncwarp();                            // the stage has been read
+        if (i + kKaStages < mine) {
+            const uint32_t bit = i % kKaStages;
+            good = (good & ~(1u << bit)) | uint32_t(issue(i + kKaStages) != ~0u) << bit;
+        }
+    }
+    if (failed)                                  // no copy may be in flight when the CTA ends
+        for (uint32_t i = mine > uint32_t(kKaStages) ? mine - kKaStages : 0u; i < mine; ++i)
+            mbar_wait_bounded(bars + i % kKaStages, (i / kKaStages) & 1);
+
+    // join the lanes' sums, then the warps
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) bacc[nt][g][k] += __shfl_xor_sync(0xffffffffu, bacc[nt][g][k], d);
+            }
+    float* ml = reinterpret_cast<float*>(smem + SM::ML);
+    if (gr == 0)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float* at = ml + (warp * HEADS + nt * 8 + 2 * cl + k) * 2;
+                at[0] = m[nt][k];
+                at[1] = l[nt][k];
+            }
+    __syncthreads();                             // (every warp is done with its ring, too)
+    float* acc = reinterpret_cast<float*>(smem + SM::RING) + warp * HEADS * HD;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float* at = acc + (nt * 8 + 2 * cl + k) * HD + g * 64 + gr * 8 + 2 * j;
+                    *reinterpret_cast<float2*>(at) = make_float2(o[nt][g][j][k] + bacc[nt][g][k], o[nt][g][j][2 + k] + bacc[nt][g][k]);
+                }
+    __syncthreads();
+    acc = reinterpret_cast<float*>(smem + SM::RING);
+    for (uint32_t h = warp; h < heads; h += kKaWarps) {
+        float top = -INFINITY, sum = 0.0f, f[kKaWarps];
+#pragma unroll
+        for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, ml[(w * HEADS + h) * 2]);
+#pragma unroll
+        for (int w = 0; w < kKaWarps; ++w) {
+            const float mw = ml[(w * HEADS + h) * 2];
+            f[w] = mw == -INFINITY ? 0.0f : kv4_ex2(mw - top);
+            // (a warp without entries has zeros; one whose statistics are NaN passes them on)
+            sum = fmaf(ml[(w * HEADS + h) * 2 + 1], mw == -INFINITY ? 1.0f : f[w], sum);
+        }
+        const uint32_t head = kvh * p.group + h0 + h;
+        if (p.part) {
+            float* dst = p.part + ((size_t(s) * p.t.num_heads + head) * p.splits + split) * (HD + 2);
+#pragma unroll
+            for (uint32_t i = 0; i < HD / 32; ++i) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kKaWarps; ++w) v = fmaf(acc[(w * HEADS + h) * HD + i * 32 + lane], f[w], v);
+                dst[i * 32 + lane] = v;
+            }
+            if (lane == 0) {
+                dst[HD] = top;
+                dst[HD + 1] = sum;
+            }
+        } else {
+            const float inv = n ? 1.0f / sum : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < HD / 32; ++i) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kKaWarps; ++w) v = fmaf(acc[(w * HEADS + h) * HD + i * 32 + lane], f[w], v);
+                const size_t at = s * p.t.out_row + head * HD + i * 32 + lane;
+                if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v * inv;
+                else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v * inv);
+            }
+        }
+    }
+}
+
+// The parts of a (sequence, KV head): its query heads' results from the
+// splits in their order, and - with weights - each entry's new weight from
+// the stored scores and the heads' joined maximum and sum. grid (x, KV head,
+// sequence): every CTA forms the statistics again, and takes its share of
+// outputs and entries.
+constexpr int kKjThreads = 256;
+__global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p) {
+    extern __shared__ float kv4_join_smem[];     // [group] log2 of the sum of exponentials, [group] maximum, [group] 1 / sum
+    pdl_release();
+    pdl_acquire();
+    const SmoeKv4Cache& c = p.a.c;
+    const uint32_t kvh = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = c.head_dim;
+    const uint32_t n = kv4_valid(p, s), pages = (n + kKvPage - 1) / kKvPage;
+    const uint32_t splits = (pages + p.split_pages - 1) / p.split_pages;       // those that have entries
+    float *lse = kv4_join_smem, *top = lse + p.group, *inv = top + p.group;
+    const float* part = p.part + (size_t(s) * p.t.num_heads + kvh * p.group) * p.splits * (HD + 2);
+    for (uint32_t h = warp; h < p.group; h += kKjThreads / 32) {
+        const float* ph = part + size_t(h) * p.splits * (HD + 2) + HD;
+        float mx = -INFINITY, sum = 0.0f;
+        for (uint32_t i = lane; i < splits; i += 32) mx = fmaxf(mx, ph[size_t(i) * (HD + 2)]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (uint32_t i = lane; i < splits; i += 32) {
+            const float mi = ph[size_t(i) * (HD + 2)];
+            sum = fmaf(ph[size_t(i) * (HD + 2) + 1], mi == -INFINITY ? 1.0f : kv4_ex2(mi - mx), sum);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            lse[h] = mx + log2f(sum);
+            top[h] = mx;
+            inv[h] = n ? 1.0f / sum : 0.0f;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = blockIdx.x * kKjThreads + tid; i < p.group * HD; i += gridDim.x * kKjThreads) {
+        const uint32_t h = i / HD, d = i % HD;
+        const float* ph = part + size_t(h) * p.splits * (HD + 2);
+        float v = 0.0f;
+#pragma unroll 4
+        for (uint32_t j = 0; j < splits; ++j) {
+            const float mj = ph[size_t(j) * (HD + 2) + HD];
+            v = fmaf(ph[size_t(j) * (HD + 2) + d], mj == -INFINITY ? 0.0f : kv4_ex2(mj - top[h]), v);
+        }
+        const size_t at = s * p.t.out_row + (kvh * p.group + h) * HD + d;
+        if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v * inv[h];
+        else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v * inv[h]);
+    }
+    if (!p.logits) return;
+    const float* row = p.logits + (size_t(s) * c.num_kv_heads + kvh) * p.rows * p.gs;
+    for (uint32_t e = blockIdx.x * kKjThreads + tid; e < n; e += gridDim.x * kKjThreads) {
         const uint32_t page = kv4_page(c, s, e, p.a.err);
         if (page == ~0u) continue;
-        const size_t i = (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
         float w = 0.0f;
-        for (uint32_t j = 0; j < group; ++j)
-            w += p.logits[(size_t(s) * p.t.num_heads + kvh * group + j) * p.stride + e];
+        for (uint32_t h = 0; h < p.group; ++h) w += kv4_ex2(row[size_t(e) * p.gs + h] - lse[h]);
+        const size_t i = (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
         p.t.score_out[i] = c.score && p.t.decay != 0.0f ? fmaf(p.t.decay, c.score[i], w) : w;
     }
 }
@@ -268,7 +677,7 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict_select(Kv4Evict p) {
     const SmoeKv4Cache& c = p.a.c;
     const uint32_t kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t* list = p.lists + (size_t(s) * c.num_kv_heads + kvh) * p.stride;
-    uint32_t n = __ldg(c.len + s);
+    uint32_t n = ld_plain(c.len + s);
     if (n > p.max_len) {
         if (tid == 0) serve_err(p.a.err, SMOE_DEVERR_BAD_RANGE);
         n = p.max_len;
@@ -277,7 +686,7 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict_select(Kv4Evict p) {
         if (tid == 0) list[0] = 0;
         return;
     }
-    const uint32_t seen = __ldg((c.seen ? c.seen : c.len) + s);
+    const uint32_t seen = ld_plain((c.seen ? c.seen : c.len) + s);
     auto key_of = [&](uint32_t e) -> uint32_t {
         const uint32_t page = kv4_page(c, s, e, p.a.err);
         if (page == ~0u) return 0u;
@@ -388,7 +797,7 @@ __global__ void __launch_bounds__(256) k_kv4_evict_move(Kv4Evict p) {
         if (lane == 9) score_out[index(to, pt)] = c.score[index(from, pf)];
     }
     if (!p.pos_out) return;
-    uint32_t n = min(__ldg(c.len + s), min(p.max_len, p.keep));
+    uint32_t n = min(ld_plain(c.len + s), min(p.max_len, p.keep));
     for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
         uint32_t lo = 0, hi = moves;             // is e a target? (targets ascend)
         while (lo < hi) {

@@ -181,7 +181,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         uint32_t total = 0;
         auto pairs = [&](uint32_t s) -> uint32_t {
             if (s >= a.n_seqs) return 0u;
-            const uint32_t q0 = __ldg(a.cu_q + s), q1 = __ldg(a.cu_q + s + 1), k0 = __ldg(ck + s), k1 = __ldg(ck + s + 1);
+            const uint32_t q0 = ld_plain(a.cu_q + s), q1 = ld_plain(a.cu_q + s + 1), k0 = ld_plain(ck + s), k1 = ld_plain(ck + s + 1);
             if (q1 < q0 || q1 > a.total_q || k1 < k0 || k1 > a.total_k) {
                 if (blockIdx.x == 0) serve_err(p.err, SMOE_DEVERR_BAD_RANGE);
                 return 0u;
@@ -218,8 +218,8 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint32_t tmem = *tslot, seq = where[0];
     if (seq < a.n_seqs) {                        // (else: a CTA past the last tile pair)
         const uint32_t tok0 = where[1];
-        const PackedSeq S{__ldg(a.cu_q + seq), __ldg(ck + seq), __ldg(a.cu_q + seq + 1) - __ldg(a.cu_q + seq),
-                          __ldg(ck + seq + 1) - __ldg(ck + seq), a.causal, a.window};
+        const PackedSeq S{ld_plain(a.cu_q + seq), ld_plain(ck + seq), ld_plain(a.cu_q + seq + 1) - ld_plain(a.cu_q + seq),
+                          ld_plain(ck + seq + 1) - ld_plain(ck + seq), a.causal, a.window};
         // blocks of 128 keys: the pair's first one, and how many each tile takes from there
         const uint32_t b0 = S.lo(tok0) / kPaKeys;
         auto blocks = [&](uint32_t t) -> uint32_t {

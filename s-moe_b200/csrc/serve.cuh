@@ -26,6 +26,14 @@ int ctx_fail(int code, const char* msg, long v);         // sets the message of 
 SMOE_DEVINL void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 SMOE_DEVINL void pdl_acquire() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Every global read of these kernels is an ordinary load, never __ldg: a
+// dependent launch is resident before its predecessors end, so the read-only
+// path may hold lines that they have since rewritten (len, for one, is read
+// by every kernel of a step and advanced at its end), and only ordinary loads
+// are ordered by pdl_acquire.
+template <typename T>
+SMOE_DEVINL T ld_plain(const T* p) { return *p; }
+
 SMOE_DEVINL void serve_err(uint32_t* err, uint32_t code) { atomicCAS(err, 0u, code); }
 
 // The sequence s with cu[s] <= row < cu[s + 1] (cu ascending, cu[0] = 0), by
@@ -35,13 +43,13 @@ SMOE_DEVINL uint32_t seq_of_row(const uint32_t* cu, uint32_t n, uint32_t row, ui
     uint32_t lo = 0, span = n;           // the answer is in [lo, lo + span)
     while (span > 1) {
         const uint32_t step = (span + 31) / 32, at = lo + min((lane + 1) * step, span);
-        const uint32_t past = __ballot_sync(0xffffffffu, __ldg(cu + at) <= row);   // bounds at or below the row
+        const uint32_t past = __ballot_sync(0xffffffffu, ld_plain(cu + at) <= row);   // bounds at or below the row
         const uint32_t k = __popc(past);
         if (k * step >= span) return n;
         lo += k * step;
         span = min(step, span - k * step);
     }
-    return (span == 1 && __ldg(cu + lo) <= row && row < __ldg(cu + lo + 1)) ? lo : n;
+    return (span == 1 && ld_plain(cu + lo) <= row && row < ld_plain(cu + lo + 1)) ? lo : n;
 }
 
 }  // namespace smoe

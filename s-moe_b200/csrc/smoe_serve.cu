@@ -36,18 +36,18 @@ int launch(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size
     return SMOE_OK;
 }
 
-// Raise a kernel's shared-memory limit once per (kernel, device).
+// Raise a kernel's shared-memory limit once per (kernel, device); a call
+// inside a stream capture then makes no attribute call.
 template <typename K>
 int smem_limit(const CtxView& c, K kern, size_t smem) {
-    static thread_local uint64_t done = 0;                        // one per kernel type and pointer list below
-    static thread_local const void* last = nullptr;
     if (smem > c.smem_optin) return ctx_fail(SMOE_ERR_UNSUPPORTED, "kernel needs more shared memory than the device has", long(smem));
-    if (last == reinterpret_cast<const void*>(kern) && (c.device < 64 && (done >> c.device & 1))) return SMOE_OK;
+    static thread_local struct { const void* f; int dev; } seen[32];
+    static thread_local int nseen = 0;
+    for (int i = 0; i < nseen; ++i)
+        if (seen[i].f == reinterpret_cast<const void*>(kern) && seen[i].dev == c.device) return SMOE_OK;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return ctx_fail(SMOE_ERR_CUDA, cudaGetErrorString(e), long(e));
-    if (last != reinterpret_cast<const void*>(kern)) done = 0;
-    last = reinterpret_cast<const void*>(kern);
-    if (c.device < 64) done |= uint64_t(1) << c.device;
+    if (nseen < 32) seen[nseen++] = {reinterpret_cast<const void*>(kern), c.device};
     return SMOE_OK;
 }
 
@@ -100,6 +100,25 @@ int check_rows(const SmoeKv4Rows* r, const char* what) {
         return ctx_fail(SMOE_ERR_ARG, "rows need 16-byte aligned bases and strides that are multiples of 4", 0);
     return SMOE_OK;
 }
+
+// How a 4-bit attention call is cut, from its arguments alone (the workspace
+// is asked for without a context).
+struct AttnPlan {
+    uint32_t split_pages, splits, gs;
+    uint64_t part_bytes, logit_bytes;
+    AttnPlan(const SmoeKv4Cache& c, const SmoeKv4AttnArgs& t) {
+        const uint64_t pages = (uint64_t(t.max_len) + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE;
+        const uint64_t pairs = uint64_t(c.n_seqs) * c.num_kv_heads;
+        // about 900 CTAs (two rounds of three a SM), 16 pages (4 a warp) at least
+        uint64_t want = std::max<uint64_t>(1, 900 / std::max<uint64_t>(pairs, 1));
+        split_pages = uint32_t(std::max<uint64_t>(16, ((pages + want - 1) / want + 3) / 4 * 4));
+        splits = uint32_t(std::max<uint64_t>(1, (pages + split_pages - 1) / split_pages));
+        const uint32_t group = t.num_heads / c.num_kv_heads;
+        gs = (group + 1) & ~1u;
+        part_bytes = splits > 1 || t.score_out ? (pairs * group * splits * (c.head_dim + 2) * 4 + 255) / 256 * 256 : 0;
+        logit_bytes = t.score_out ? pairs * t.max_len * gs * 4 : 0;
+    }
+};
 
 }  // namespace
 
@@ -168,9 +187,9 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
 }
 
 uint64_t smoe_cuda_kv4_attention_workspace(const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
-    if (!cache || !t) return 0;
-    const uint64_t stride = (uint64_t(t->max_len) + 63) / 64 * 64;
-    return uint64_t(cache->n_seqs) * t->num_heads * stride * 4;
+    if (!cache || !t || cache->num_kv_heads == 0) return 0;
+    const AttnPlan plan(*cache, *t);
+    return plan.part_bytes + plan.logit_bytes;
 }
 
 int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
@@ -187,8 +206,39 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     if (need && (!t->workspace || t->workspace_bytes < need || !aligned(t->workspace, 16)))
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: workspace missing, too small or unaligned; bytes needed", long(need));
     const CtxView c = smoe::ctx_view(ctx);
-    smoe::Kv4Attn p{{*cache, c.err}, *t, static_cast<float*>(t->workspace), (t->max_len + 63) / 64 * 64};
-    return launch(c, smoe::k_kv4_attention, dim3(cache->num_kv_heads, cache->n_seqs), dim3(256), 0, p);
+    const AttnPlan plan(*cache, *t);
+    smoe::Kv4Attn p{};
+    p.a = {*cache, c.err};
+    p.t = *t;
+    p.group = t->num_heads / cache->num_kv_heads;
+    p.split_pages = plan.split_pages;
+    p.splits = plan.splits;
+    p.part = plan.part_bytes ? static_cast<float*>(t->workspace) : nullptr;
+    p.logits = plan.logit_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(t->workspace) + plan.part_bytes) : nullptr;
+    p.rows = t->max_len;
+    p.gs = plan.gs;
+    p.scale_log2 = t->scale * 1.4426950408889634f;
+    auto run = [&](auto kern, uint32_t smem, uint32_t heads) -> int {
+        p.chunks = (p.group + heads - 1) / heads;
+        if (uint64_t(p.chunks) * cache->num_kv_heads > 65535)
+            return ctx_fail(SMOE_ERR_ARG, "kv4_attention: too many heads", long(t->num_heads));
+        const int r = smem_limit(c, kern, smem);
+        return r ? r : launch(c, kern, dim3(plan.splits, p.chunks * cache->num_kv_heads, cache->n_seqs), dim3(smoe::kKaWarps * 32), smem, p);
+    };
+    const bool wide = p.group > 8, f32 = t->dtype == SMOE_DTYPE_F32;
+    using namespace smoe;
+#define SMOE_KV4_ATTN(NG)                                                                                        \
+    (wide ? f32 ? run(k_kv4_attention<NG, 2, 2>, Kv4AttnSmem<NG, 2>::BYTES, 16)                                  \
+                : run(k_kv4_attention<NG, 2, 1>, Kv4AttnSmem<NG, 2>::BYTES, 16)                                  \
+          : f32 ? run(k_kv4_attention<NG, 1, 2>, Kv4AttnSmem<NG, 1>::BYTES, 8)                                   \
+                : run(k_kv4_attention<NG, 1, 1>, Kv4AttnSmem<NG, 1>::BYTES, 8))
+    rc = cache->head_dim == 64 ? SMOE_KV4_ATTN(1) : SMOE_KV4_ATTN(2);
+#undef SMOE_KV4_ATTN
+    if (rc || !p.part) return rc;
+    const uint32_t outs = (p.group * cache->head_dim + kKjThreads - 1) / kKjThreads;
+    const uint32_t entries = p.logits ? (t->max_len + 4 * kKjThreads - 1) / (4 * kKjThreads) : 1u;
+    return launch(c, k_kv4_join, dim3(std::max(outs, entries), cache->num_kv_heads, cache->n_seqs), dim3(kKjThreads),
+                  size_t(p.group) * 12, p);
 }
 
 uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len) {
