@@ -131,20 +131,22 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* fir
 
 // ---------------------------------------------------------------- attention
 // One query token per sequence. With a group's codes c (0..15), scales s and
-// biases b, and c' = c - 8, b' = b + 8 s:
-//   q . k = sum_g s_g (q_g . c'_g) + b'_g sum(q_g)
-//   sum_j p_j v_j = sum_j (p_j s_j) c'_j + sum_j p_j b'_j        (per group)
-// so the raw codes are the tensor cores' operands (c' is exact) and scales
+// biases b:
+//   q . k = sum_g s_g (q_g . c_g) + b_g sum(q_g)
+//   sum_j p_j v_j = sum_j (p_j s_j) c_j + sum_j p_j b_j          (per group)
+// so the raw codes are the tensor cores' operands (exact in fp16) and scales
 // and biases stay in fp32. q goes in as one (bf16 q) or two fp16 pieces, each
 // head scaled by a power of two so that its largest value is near 2^14; p s
-// as two bf16 pieces (its range is the values' own, too wide for fp16).
+// as two fp16 pieces (22 bits), times a power of two per group that follows
+// the largest scale seen. (bf16 pieces need no such power, but three more
+// instructions for every 16 codes.)
 // The entries are the M rows of both products and a KV head's query heads
 // the N columns (8 or 16), so a page is dequantised once for all of them.
 //
 // A CTA of 4 warps takes a stretch of pages of one (sequence, KV head), a
 // warp every fourth page: each warp copies its pages - one block, one bulk
 // copy - into a ring of its own, keeps its own running maximum and sums, and
-// the four are joined at the end. Bound by the cache's bytes.
+// the four are joined at the end.
 constexpr int kKaWarps = 4, kKaStages = 2;
 
 struct Kv4Attn {
@@ -152,7 +154,8 @@ struct Kv4Attn {
     SmoeKv4AttnArgs t;
     uint32_t group, chunks;                      // query heads per KV head; CTAs of a KV head's query heads
     uint32_t split_pages, splits;                // pages of a CTA, CTAs along a sequence of max_len
-    float* part;                                 // [n_seqs][num_heads][splits][head_dim + 2] (sums, maximum, sum), splits > 1 or weights
+    float* part;                                 // [n_seqs][num_heads][splits][head_dim] weighted sums, splits > 1 or weights
+    float2* stat;                                // [n_seqs][num_heads][splits] maximum, sum
     float* logits;                               // [n_seqs][num_kv_heads][row][gs] log2-scaled scores, with weights
     uint32_t rows, gs;
     float scale_log2;
@@ -168,28 +171,18 @@ SMOE_DEVINL uint32_t kv4_valid(const Kv4Attn& p, uint32_t s) {
     return uint32_t(n);
 }
 
-// 8 codes -> c - 8 as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c
-// are exact, and so is what the subtraction or the multiply-add makes of them.
+// 8 codes as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c are
+// exact, and so is what the subtraction or the multiply-add makes of them.
 SMOE_DEVINL void kv4_half_codes(uint32_t w, uint32_t* r) {
     constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u, ONE = 0x64006400u;
     const uint32_t w8 = w >> 8;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[0]) : "r"(lop3_and_or(w, M0, ONE)), "r"(0x64086408u));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(lop3_and_or(w, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[2]) : "r"(lop3_and_or(w8, M0, ONE)), "r"(0x64086408u));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(lop3_and_or(w8, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
-}
-// Codes n = 0..3 of two entries (low and high halves of u) -> c - 8 as bf16 pairs.
-SMOE_DEVINL void kv4_bf16_codes(uint32_t u, uint32_t* r) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[n]) : "r"(lop3_and_or(u >> (4 * n), 0x000F000Fu, 0x43004300u)), "r"(0x43084308u));
+    r[0] = hsub_1024(lop3_and_or(w, M0, ONE));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(lop3_and_or(w, M1, ONE)), "r"(0x2C002C00u), "r"(0xD400D400u));
+    r[2] = hsub_1024(lop3_and_or(w8, M0, ONE));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(lop3_and_or(w8, M1, ONE)), "r"(0x2C002C00u), "r"(0xD400D400u));
 }
 SMOE_DEVINL void mma_f16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-SMOE_DEVINL void mma_bf16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 SMOE_DEVINL uint32_t movm_trans(uint32_t x) {
@@ -202,11 +195,13 @@ SMOE_DEVINL float kv4_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-SMOE_DEVINL uint32_t cvt_bf16x2_rn(float lo, float hi) {
+SMOE_DEVINL uint32_t cvt_f16x2(float lo, float hi) {
     uint32_t d;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
+SMOE_DEVINL float half_lo(uint32_t x) { return __half2float(__ushort_as_half(uint16_t(x))); }
+SMOE_DEVINL float half_hi(uint32_t x) { return __half2float(__ushort_as_half(uint16_t(x >> 16))); }
 SMOE_DEVINL float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 SMOE_DEVINL float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
@@ -214,9 +209,10 @@ template <int NG, int NT>
 struct Kv4AttnSmem {
     static constexpr uint32_t BLOCK = NG * 4608, HD = NG * 64, HEADS = NT * 8;
     static constexpr uint32_t RING = 0, RING_BYTES = kKaWarps * kKaStages * BLOCK;
-    static constexpr uint32_t Q = RING + RING_BYTES;             // float [HEADS][HD + 4]
-    static constexpr uint32_t QROW = HD + 4;
-    static constexpr uint32_t QSUM = Q + HEADS * QROW * 4;       // float [NG][HEADS]
+    // float [HEADS][HD + 4], in the last warp's last stage until the fragments are made: three CTAs then fit an SM
+    static constexpr uint32_t QROW = HD + 4, Q = RING + RING_BYTES - (HEADS * QROW * 4 + 127) / 128 * 128;
+    static_assert(HEADS * QROW * 4 <= (NT == 1 ? 1 : 2) * BLOCK, "q's place");
+    static constexpr uint32_t QSUM = RING + RING_BYTES;          // float [NG][HEADS]
     static constexpr uint32_t QINV = QSUM + NG * HEADS * 4;      // float [HEADS]: scale_log2 over the head's power of two
     static constexpr uint32_t ML = QINV + HEADS * 4;             // float [warps][HEADS][2]
     static constexpr uint32_t BAR = ML + kKaWarps * HEADS * 8;
@@ -226,7 +222,7 @@ struct Kv4AttnSmem {
 
 // NG groups of 64 (head_dim / 64), NT tiles of 8 query heads, QP pieces of q.
 template <int NG, int NT, int QP>
-__global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p) {
+__global__ void __launch_bounds__(kKaWarps * 32, NT == 1 && QP == 1 ? 3 : 2) k_kv4_attention(const Kv4Attn p) {
     using SM = Kv4AttnSmem<NG, NT>;
     constexpr uint32_t HD = SM::HD, HEADS = SM::HEADS;
     extern __shared__ __align__(128) uint8_t kv4_smem[];
@@ -271,8 +267,9 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
         }
         return page;
     };
-    uint32_t good = 0;                                           // bit i % 32: page i can be read
-    for (uint32_t i = 0; i < uint32_t(kKaStages) && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
+    uint32_t good = 0;                                           // bit st: the page in stage st can be read
+    const uint32_t early = warp + 1 < kKaWarps ? kKaStages : NT == 1 ? kKaStages - 1 : 0;   // stages that q is not in
+    for (uint32_t i = 0; i < early && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
 
     // q: fp32 in shared memory, each head times a power of two, its group sums
     float* qs = reinterpret_cast<float*>(smem + SM::Q);
@@ -326,6 +323,9 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
                     if (QP == 2)
                         qf[nt][g][st][QP - 1][b] = pack_half2(__float2half_rn(y[0] - __half2float(y0)), __float2half_rn(y[4] - __half2float(y1)));
                 }
+    if (early < uint32_t(kKaStages)) fence_proxy_async();        // q's place goes to the bulk copies
+    __syncthreads();
+    for (uint32_t i = early; i < uint32_t(kKaStages) && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
     float qsm[NT][NG][2], sc[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -336,7 +336,9 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
             for (int g = 0; g < NG; ++g) qsm[nt][g][k] = qsum[g * HEADS + nt * 8 + 2 * cl + k];
         }
 
-    float m[NT][2], l[NT][2], bacc[NT][NG][2], o[NT][NG][4][4];
+    float m[NT][2], l[NT][2], bacc[NT][NG][2], o[NT][NG][4][4], up[NG];      // up: the group's power of two in o
+#pragma unroll
+    for (int g = 0; g < NG; ++g) up[g] = 0.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
                                 mma_f16f32_16816(d[nt], af, qf[nt][g][w * 2 + h][q][0], qf[nt][g][w * 2 + h][q][1]);
                     }
                 }
-                const float s0 = lo_f(sa), b0 = fmaf(8.0f, s0, hi_f(sa)), s1 = lo_f(sb), b1 = fmaf(8.0f, s1, hi_f(sb));
+                const float s0 = lo_f(sa), b0 = hi_f(sa), s1 = lo_f(sb), b1 = hi_f(sb);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -405,16 +407,26 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[mt][nt][k] = (k < 2 ? ka : kb) < have ? x[mt][nt][k] * sc[nt][k & 1] : -INFINITY;
-            if (lrow) {
+                for (int k = 0; k < 4; ++k) x[mt][nt][k] *= sc[nt][k & 1];
+        }
+        if (have < kKvPage)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t h = nt * 8 + 2 * cl;
-                    float* at = lrow + size_t(e0 + ka) * p.gs + h0 + h;
-                    if (h < heads && e0 + ka < n) *reinterpret_cast<float2*>(at) = make_float2(x[mt][nt][0], x[mt][nt][1]);
-                    if (h < heads && e0 + kb < n) *reinterpret_cast<float2*>(at + size_t(8) * p.gs) = make_float2(x[mt][nt][2], x[mt][nt][3]);
-                }
-            }
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (mt * 16 + gr + (k < 2 ? 0 : 8) >= have) x[mt][nt][k] = -INFINITY;
+        if (lrow) {
+            float* at = lrow + size_t(e0 + gr) * p.gs + h0 + 2 * cl;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (nt * 8 + 2 * cl < heads && e0 + mt * 16 + k * 8 + gr < n)
+                            *reinterpret_cast<float2*>(at + (mt * 16 + k * 8) * p.gs + nt * 8) = make_float2(x[mt][nt][2 * k], x[mt][nt][2 * k + 1]);
         }
         // running maximum; moved only when it is 2^8 too low
         float f[NT][2];
@@ -452,6 +464,24 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
                     }
                 }
         }
+        // the power of two of a group's p s: its largest scale near 2^3, and below
+        // 2^7 as pages follow, so that with p <= 2^8 nothing passes fp16's range
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const uint2 w = *reinterpret_cast<const uint2*>(blk + G.sb(1, g) + lane * 8);
+            const uint32_t big = __reduce_max_sync(0xffffffffu, max(2 * lane < have ? w.x & 0x7fffu : 0u, 2 * lane + 1 < have ? w.y & 0x7fffu : 0u));
+            if (__uint_as_float(big << 16) * up[g] > 128.0f || up[g] == 0.0f) {
+                const float now = __uint_as_float(uint32_t(max(27, min(227, 257 - int(big >> 7)))) << 23);
+                const float r = up[g] == 0.0f ? 0.0f : now / up[g];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[nt][g][j][k] *= r;
+                up[g] = now;
+            }
+        }
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
             const uint32_t ka = mt * 16 + gr, kb = ka + 8;
@@ -466,35 +496,40 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 // entries past the last one may hold anything: their scales count as 0
-                const uint32_t sa = ka < have ? *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + ka * 4) : 0u;
-                const uint32_t sb = kb < have ? *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + kb * 4) : 0u;
-                const float s0 = lo_f(sa), b0 = fmaf(8.0f, s0, hi_f(sa)), s1 = lo_f(sb), b1 = fmaf(8.0f, s1, hi_f(sb));
+                uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + ka * 4);
+                uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + kb * 4);
+                if (have < kKvPage) {
+                    if (ka >= have) sa = 0u;
+                    if (kb >= have) sb = 0u;
+                }
+                const float s0 = lo_f(sa) * up[g], b0 = hi_f(sa), s1 = lo_f(sb) * up[g], b1 = hi_f(sb);
                 // codes of this lane's 8 dimensions (8 gr ..) of the entries 2 cl, 2 cl + 1, 2 cl + 8, 2 cl + 9 of the tile;
                 // lanes cl >= 2 load the pair the other way round (the four entries of a load then lie in different banks)
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     w[k] = *reinterpret_cast<const uint32_t*>(blk + G.codes(1, g) + (mt * 16 + 2 * cl + ((k & 1) ^ (cl >> 1)) + (k >> 1) * 8) * 32 + gr * 4);
+                // even and odd bytes of the pair side by side, so that a register's halves are the two entries' codes of one dimension
                 const uint32_t p_lo = cl < 2 ? 0x5410u : 0x1054u, p_hi = cl < 2 ? 0x7632u : 0x3276u;
                 uint32_t c0[8], c1[8];           // dimension n: entries (2 cl, 2 cl + 1), and + 8
-                kv4_bf16_codes(__byte_perm(w[0], w[1], p_lo), c0);
-                kv4_bf16_codes(__byte_perm(w[0], w[1], p_hi), c0 + 4);
-                kv4_bf16_codes(__byte_perm(w[2], w[3], p_lo), c1);
-                kv4_bf16_codes(__byte_perm(w[2], w[3], p_hi), c1 + 4);
+                kv4_half_codes(__byte_perm(w[0], w[1], p_lo), c0);
+                kv4_half_codes(__byte_perm(w[0], w[1], p_hi), c0 + 4);
+                kv4_half_codes(__byte_perm(w[2], w[3], p_lo), c1);
+                kv4_half_codes(__byte_perm(w[2], w[3], p_hi), c1 + 4);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     bacc[nt][g][0] = fmaf(x[mt][nt][0], b0, fmaf(x[mt][nt][2], b1, bacc[nt][g][0]));
                     bacc[nt][g][1] = fmaf(x[mt][nt][1], b0, fmaf(x[mt][nt][3], b1, bacc[nt][g][1]));
                     const float y0 = x[mt][nt][0] * s0, y1 = x[mt][nt][1] * s0, y2 = x[mt][nt][2] * s1, y3 = x[mt][nt][3] * s1;
-                    const uint32_t u0 = cvt_bf16x2_rn(y0, y1), u1 = cvt_bf16x2_rn(y2, y3);
-                    const uint32_t v0 = movm_trans(cvt_bf16x2_rn(y0 - lo_f(u0), y1 - hi_f(u0)));
-                    const uint32_t v1 = movm_trans(cvt_bf16x2_rn(y2 - lo_f(u1), y3 - hi_f(u1)));
+                    const uint32_t u0 = cvt_f16x2(y0, y1), u1 = cvt_f16x2(y2, y3);
                     const uint32_t t0 = movm_trans(u0), t1 = movm_trans(u1);
+                    const uint32_t v0 = movm_trans(cvt_f16x2(y0 - half_lo(u0), y1 - half_hi(u0)));
+                    const uint32_t v1 = movm_trans(cvt_f16x2(y2 - half_lo(u1), y3 - half_hi(u1)));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t af[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
-                        mma_bf16f32_16816(o[nt][g][j], af, t0, t1);
-                        mma_bf16f32_16816(o[nt][g][j], af, v0, v1);
+                        mma_f16f32_16816(o[nt][g][j], af, t0, t1);
+                        mma_f16f32_16816(o[nt][g][j], af, v0, v1);
                     }
                 }
             }
@@ -541,7 +576,8 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float* at = acc + (nt * 8 + 2 * cl + k) * HD + g * 64 + gr * 8 + 2 * j;
-                    *reinterpret_cast<float2*>(at) = make_float2(o[nt][g][j][k] + bacc[nt][g][k], o[nt][g][j][2 + k] + bacc[nt][g][k]);
+                    const float down = up[g] == 0.0f ? 0.0f : 1.0f / up[g];          // (exact: a power of two)
+                    *reinterpret_cast<float2*>(at) = make_float2(fmaf(o[nt][g][j][k], down, bacc[nt][g][k]), fmaf(o[nt][g][j][2 + k], down, bacc[nt][g][k]));
                 }
     __syncthreads();
     acc = reinterpret_cast<float*>(smem + SM::RING);
@@ -558,7 +594,8 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
         }
         const uint32_t head = kvh * p.group + h0 + h;
         if (p.part) {
-            float* dst = p.part + ((size_t(s) * p.t.num_heads + head) * p.splits + split) * (HD + 2);
+            const size_t at = (size_t(s) * p.t.num_heads + head) * p.splits + split;
+            float* dst = p.part + at * HD;
 #pragma unroll
             for (uint32_t i = 0; i < HD / 32; ++i) {
                 float v = 0.0f;
@@ -566,10 +603,7 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
                 for (int w = 0; w < kKaWarps; ++w) v = fmaf(acc[(w * HEADS + h) * HD + i * 32 + lane], f[w], v);
                 dst[i * 32 + lane] = v;
             }
-            if (lane == 0) {
-                dst[HD] = top;
-                dst[HD + 1] = sum;
-            }
+            if (lane == 0) p.stat[at] = make_float2(top, sum);
         } else {
             const float inv = n ? 1.0f / sum : 0.0f;
 #pragma unroll
@@ -588,61 +622,90 @@ __global__ void __launch_bounds__(kKaWarps * 32) k_kv4_attention(const Kv4Attn p
 // The parts of a (sequence, KV head): its query heads' results from the
 // splits in their order, and - with weights - each entry's new weight from
 // the stored scores and the heads' joined maximum and sum. grid (x, KV head,
-// sequence): every CTA forms the statistics again, and takes its share of
-// outputs and entries.
-constexpr int kKjThreads = 256;
-__global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p) {
-    extern __shared__ float kv4_join_smem[];     // [group] log2 of the sum of exponentials, [group] maximum, [group] 1 / sum
+// sequence): every CTA forms the statistics it needs again; the first
+// `outs` take kKjOuts outputs each (four threads an output, a quarter of
+// the splits each, so that the chain of loads is short), the others 1024
+// entries each.
+constexpr int kKjThreads = 256, kKjOuts = 64, kKjEntries = 4 * kKjThreads;
+__global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p, uint32_t outs) {
+    extern __shared__ float kv4_join_smem[];     // [group] log2 of the sum of exponentials; weights of the splits
+    __shared__ float part_sum[kKjThreads];
     pdl_release();
     pdl_acquire();
     const SmoeKv4Cache& c = p.a.c;
     const uint32_t kvh = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = c.head_dim;
     const uint32_t n = kv4_valid(p, s), pages = (n + kKvPage - 1) / kKvPage;
     const uint32_t splits = (pages + p.split_pages - 1) / p.split_pages;       // those that have entries
-    float *lse = kv4_join_smem, *top = lse + p.group, *inv = top + p.group;
-    const float* part = p.part + (size_t(s) * p.t.num_heads + kvh * p.group) * p.splits * (HD + 2);
-    for (uint32_t h = warp; h < p.group; h += kKjThreads / 32) {
-        const float* ph = part + size_t(h) * p.splits * (HD + 2) + HD;
+    const bool is_out = blockIdx.x < outs;
+    const uint32_t e0 = (blockIdx.x - outs) * kKjEntries;
+    if (!is_out && e0 >= n) return;
+    const size_t first = (size_t(s) * p.t.num_heads + kvh * p.group) * p.splits;
+    // an output CTA's 64 outputs belong to one head (head_dim is 64 or 128)
+    const uint32_t h_lo = is_out ? blockIdx.x * kKjOuts / HD : 0u, h_hi = is_out ? h_lo + 1 : p.group;
+    float* lse = kv4_join_smem;
+    float* wgt = kv4_join_smem + p.group;        // [splits] of the output CTA's head: its share of the whole
+    for (uint32_t h = h_lo + warp; h < h_hi; h += kKjThreads / 32) {
+        const float2* st = p.stat + first + size_t(h) * p.splits;
         float mx = -INFINITY, sum = 0.0f;
-        for (uint32_t i = lane; i < splits; i += 32) mx = fmaxf(mx, ph[size_t(i) * (HD + 2)]);
+        for (uint32_t i = lane; i < splits; i += 32) mx = fmaxf(mx, st[i].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        for (uint32_t i = lane; i < splits; i += 32) {
-            const float mi = ph[size_t(i) * (HD + 2)];
-            sum = fmaf(ph[size_t(i) * (HD + 2) + 1], mi == -INFINITY ? 1.0f : kv4_ex2(mi - mx), sum);
-        }
+        for (uint32_t i = lane; i < splits; i += 32)
+            sum = fmaf(st[i].y, st[i].x == -INFINITY ? 1.0f : kv4_ex2(st[i].x - mx), sum);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) {
-            lse[h] = mx + log2f(sum);
-            top[h] = mx;
-            inv[h] = n ? 1.0f / sum : 0.0f;
+        if (lane == 0) lse[h] = mx + log2f(sum);
+        if (is_out) {
+            const float inv = 1.0f / sum;
+            for (uint32_t i = lane; i < splits; i += 32) wgt[i] = st[i].x == -INFINITY ? sum * 0.0f : kv4_ex2(st[i].x - mx) * inv;
         }
     }
     __syncthreads();
-    for (uint32_t i = blockIdx.x * kKjThreads + tid; i < p.group * HD; i += gridDim.x * kKjThreads) {
-        const uint32_t h = i / HD, d = i % HD;
-        const float* ph = part + size_t(h) * p.splits * (HD + 2);
+    if (is_out) {
+        const uint32_t q = tid / kKjOuts, d = (blockIdx.x * kKjOuts + tid % kKjOuts) % HD;
+        const float* src = p.part + (first + size_t(h_lo) * p.splits) * HD + d;
         float v = 0.0f;
-#pragma unroll 4
-        for (uint32_t j = 0; j < splits; ++j) {
-            const float mj = ph[size_t(j) * (HD + 2) + HD];
-            v = fmaf(ph[size_t(j) * (HD + 2) + d], mj == -INFINITY ? 0.0f : kv4_ex2(mj - top[h]), v);
+#pragma unroll 8
+        for (uint32_t j = q; j < splits; j += kKjThreads / kKjOuts) v = fmaf(src[size_t(j) * HD], wgt[j], v);
+        part_sum[tid] = v;
+        __syncthreads();
+        if (tid < kKjOuts) {
+            v = (part_sum[tid] + part_sum[tid + kKjOuts]) + (part_sum[tid + 2 * kKjOuts] + part_sum[tid + 3 * kKjOuts]);
+            const size_t at = s * p.t.out_row + (kvh * p.group + h_lo) * HD + d;
+            if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v;
+            else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v);
         }
-        const size_t at = s * p.t.out_row + (kvh * p.group + h) * HD + d;
-        if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v * inv[h];
-        else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v * inv[h]);
+        return;
     }
-    if (!p.logits) return;
     const float* row = p.logits + (size_t(s) * c.num_kv_heads + kvh) * p.rows * p.gs;
-    for (uint32_t e = blockIdx.x * kKjThreads + tid; e < n; e += gridDim.x * kKjThreads) {
-        const uint32_t page = kv4_page(c, s, e, p.a.err);
-        if (page == ~0u) continue;
-        float w = 0.0f;
-        for (uint32_t h = 0; h < p.group; ++h) w += kv4_ex2(row[size_t(e) * p.gs + h] - lse[h]);
-        const size_t i = (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
-        p.t.score_out[i] = c.score && p.t.decay != 0.0f ? fmaf(p.t.decay, c.score[i], w) : w;
+    float w[4], old[4];
+    size_t at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t e = e0 + k * kKjThreads + tid, page = e < n ? kv4_page(c, s, e, p.a.err) : ~0u;
+        at[k] = page == ~0u ? ~size_t(0) : (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
+        old[k] = page != ~0u && c.score && p.t.decay != 0.0f ? c.score[at[k]] * p.t.decay : 0.0f;
+        w[k] = 0.0f;
     }
+    uint32_t h = 0;
+    if (p.gs % 4 == 0)
+        for (; h + 4 <= p.group; h += 4) {
+            float4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                y[k] = at[k] == ~size_t(0) ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                           : *reinterpret_cast<const float4*>(row + size_t(e0 + k * kKjThreads + tid) * p.gs + h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] += (kv4_ex2(y[k].x - lse[h]) + kv4_ex2(y[k].y - lse[h + 1])) + (kv4_ex2(y[k].z - lse[h + 2]) + kv4_ex2(y[k].w - lse[h + 3]));
+        }
+    for (; h < p.group; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (at[k] != ~size_t(0)) w[k] += kv4_ex2(row[size_t(e0 + k * kKjThreads + tid) * p.gs + h] - lse[h]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (at[k] != ~size_t(0)) p.t.score_out[at[k]] = old[k] + w[k];
 }
 
 // ----------------------------------------------------------------- eviction

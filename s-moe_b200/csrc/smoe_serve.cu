@@ -115,7 +115,7 @@ struct AttnPlan {
         splits = uint32_t(std::max<uint64_t>(1, (pages + split_pages - 1) / split_pages));
         const uint32_t group = t.num_heads / c.num_kv_heads;
         gs = (group + 1) & ~1u;
-        part_bytes = splits > 1 || t.score_out ? (pairs * group * splits * (c.head_dim + 2) * 4 + 255) / 256 * 256 : 0;
+        part_bytes = splits > 1 || t.score_out ? (pairs * group * splits * (c.head_dim + 2) * 4 + 255) / 256 * 256 : 0;   // sums, then statistics
         logit_bytes = t.score_out ? pairs * t.max_len * gs * 4 : 0;
     }
 };
@@ -214,6 +214,7 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     p.split_pages = plan.split_pages;
     p.splits = plan.splits;
     p.part = plan.part_bytes ? static_cast<float*>(t->workspace) : nullptr;
+    p.stat = reinterpret_cast<float2*>(p.part + (p.part ? uint64_t(cache->n_seqs) * t->num_heads * plan.splits * cache->head_dim : 0));
     p.logits = plan.logit_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(t->workspace) + plan.part_bytes) : nullptr;
     p.rows = t->max_len;
     p.gs = plan.gs;
@@ -235,10 +236,9 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     rc = cache->head_dim == 64 ? SMOE_KV4_ATTN(1) : SMOE_KV4_ATTN(2);
 #undef SMOE_KV4_ATTN
     if (rc || !p.part) return rc;
-    const uint32_t outs = (p.group * cache->head_dim + kKjThreads - 1) / kKjThreads;
-    const uint32_t entries = p.logits ? (t->max_len + 4 * kKjThreads - 1) / (4 * kKjThreads) : 1u;
-    return launch(c, k_kv4_join, dim3(std::max(outs, entries), cache->num_kv_heads, cache->n_seqs), dim3(kKjThreads),
-                  size_t(p.group) * 12, p);
+    const uint32_t outs = p.group * cache->head_dim / kKjOuts, entries = p.logits ? (t->max_len + kKjEntries - 1) / kKjEntries : 0u;
+    return launch(c, k_kv4_join, dim3(outs + entries, cache->num_kv_heads, cache->n_seqs), dim3(kKjThreads),
+                  (size_t(p.group) + plan.splits) * 4, p, outs);
 }
 
 uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len) {
