@@ -140,35 +140,88 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* fir
 // as two fp16 pieces (22 bits), times a power of two per group that follows
 // the largest scale seen. (bf16 pieces need no such power, but three more
 // instructions for every 16 codes.)
-// The entries are the M rows of both products and a KV head's query heads
-// the N columns (8 or 16), so a page is dequantised once for all of them.
+// The entries are the M rows of both products and 8 of a KV head's query
+// heads the N columns. (16 at a time halve the unpacking of wide groups, but
+// need 255 registers: 8 warps an SM instead of 16, and 1.2 times the time.)
 //
-// A CTA of 4 warps takes a stretch of pages of one (sequence, KV head), a
-// warp every fourth page: each warp copies its pages - one block, one bulk
-// copy - into a ring of its own, keeps its own running maximum and sums, and
-// the four are joined at the end.
-constexpr int kKaWarps = 4, kKaStages = 2;
+// All pages of all (sequence, KV head) pairs, in one line, are cut into equal
+// stretches, one a warp of a grid that fills the GPU once: ragged lengths do
+// not matter, and no warp waits for another. A warp copies its pages' keys and
+// values, by turns, into a ring of three of its own (216 KB an SM), and for
+// each pair that its stretch touches it keeps a running maximum, sums and
+// accumulators. A pair inside one stretch is done (unless weights are
+// wanted); the parts of the others are stored and joined by k_kv4_join. The
+// part of (warp, pair) has the number warp + pair: along the line at least
+// one of the two grows from a part to the next, so no two share one.
+constexpr int kKaWarps = 4, kKaStages = 3;
+#ifndef KA_CTAS
+#define KA_CTAS 3
+#endif
+constexpr uint32_t kKaCtas = KA_CTAS, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
 
 struct Kv4Attn {
     Kv4Args a;
     SmoeKv4AttnArgs t;
-    uint32_t group, chunks;                      // query heads per KV head; CTAs of a KV head's query heads
-    uint32_t split_pages, splits;                // pages of a CTA, CTAs along a sequence of max_len
-    float* part;                                 // [n_seqs][num_heads][splits][head_dim] weighted sums, splits > 1 or weights
-    float2* stat;                                // [n_seqs][num_heads][splits] maximum, sum
-    float* logits;                               // [n_seqs][num_kv_heads][row][gs] log2-scaled scores, with weights
-    uint32_t rows, gs;
-    float scale_log2;
+    uint32_t group, chunks;                      // query heads per KV head; rounds of 8 heads that makes
+    uint32_t warps;                              // of the grid
+    float* part;                                 // [warps + pairs][8 heads][head_dim] weighted sums
+    float2* stat;                                // [warps + pairs][8 heads] maximum, sum
+    uint2* meta;                                 // [pairs] first warp of a pair with entries, number of its parts
+    uint32_t lanes;                              // k_kv4_join: threads that share an output's parts (a power of two)
+    float* logits;                               // [n_seqs][num_heads][rows] log2-scaled scores, with weights
+    uint32_t rows;                               // max_len rounded up to a page
+    float scale_log2;                            // positive
 };
 
 // Entries of sequence s that the token attends to.
 SMOE_DEVINL uint32_t kv4_valid(const Kv4Attn& p, uint32_t s) {
     const uint64_t n = uint64_t(ld_plain(p.a.c.len + s)) + p.t.extra;
     if (n > p.t.max_len) {
-        if (threadIdx.x == 0) serve_err(p.a.err, SMOE_DEVERR_BAD_RANGE);
+        serve_err(p.a.err, SMOE_DEVERR_BAD_RANGE);
         return p.t.max_len;
     }
     return uint32_t(n);
+}
+SMOE_DEVINL uint32_t kv4_pages(uint32_t n) { return (n + kKvPage - 1) / kKvPage; }
+
+// The line of pages: sequence s starts at heads * (pages of the sequences
+// before it), `heads` pairs of equal length each.
+struct Kv4Line {
+    uint64_t total, per;                         // pages, pages of a stretch
+    SMOE_DEVINL uint64_t first(uint32_t w) const { return min(total, uint64_t(w) * per); }
+};
+// By a whole warp: the line, and the sequence that holds warp w's first page
+// with the page of the line that it starts at.
+SMOE_DEVINL Kv4Line kv4_line(const Kv4Attn& p, uint32_t heads, uint32_t lane, uint32_t w, uint32_t& seq, uint64_t& start) {
+    const uint32_t ns = p.a.c.n_seqs;
+    uint64_t total = 0, before = 0;
+    for (uint32_t b = 0; b < ns; b += 32) {
+        const uint32_t s = b + lane, n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;
+        total += __reduce_add_sync(0xffffffffu, n);
+    }
+    Kv4Line L{total * heads, max(uint64_t(1), (total * heads + p.warps - 1) / p.warps)};
+    const uint64_t want = L.first(w);
+    seq = ns;
+    if (want >= L.total) return L;
+    for (uint32_t b = 0; b < ns; b += 32) {
+        const uint32_t s = b + lane, n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;
+        uint32_t incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= uint32_t(o)) incl += v;
+        }
+        const uint64_t end = (before + incl) * heads;
+        const uint32_t hit = __ballot_sync(0xffffffffu, end > want);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            seq = b + l;
+            start = (before + __shfl_sync(0xffffffffu, incl - n, l)) * heads;
+            return L;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return L;
 }
 
 // 8 codes as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c are
@@ -184,6 +237,10 @@ SMOE_DEVINL void kv4_half_codes(uint32_t w, uint32_t* r) {
 SMOE_DEVINL void mma_f16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+SMOE_DEVINL void mma_f16f32_16816_z(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {      // from zero
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 SMOE_DEVINL uint32_t movm_trans(uint32_t x) {
     uint32_t y;
@@ -205,33 +262,44 @@ SMOE_DEVINL float half_hi(uint32_t x) { return __half2float(__ushort_as_half(uin
 SMOE_DEVINL float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 SMOE_DEVINL float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-template <int NG, int NT>
-struct Kv4AttnSmem {
-    static constexpr uint32_t BLOCK = NG * 4608, HD = NG * 64, HEADS = NT * 8;
-    static constexpr uint32_t RING = 0, RING_BYTES = kKaWarps * kKaStages * BLOCK;
-    // float [HEADS][HD + 4], in the last warp's last stage until the fragments are made: three CTAs then fit an SM
-    static constexpr uint32_t QROW = HD + 4, Q = RING + RING_BYTES - (HEADS * QROW * 4 + 127) / 128 * 128;
-    static_assert(HEADS * QROW * 4 <= (NT == 1 ? 1 : 2) * BLOCK, "q's place");
-    static constexpr uint32_t QSUM = RING + RING_BYTES;          // float [NG][HEADS]
-    static constexpr uint32_t QINV = QSUM + NG * HEADS * 4;      // float [HEADS]: scale_log2 over the head's power of two
-    static constexpr uint32_t ML = QINV + HEADS * 4;             // float [warps][HEADS][2]
-    static constexpr uint32_t BAR = ML + kKaWarps * HEADS * 8;
-    static constexpr uint32_t BYTES = BAR + kKaWarps * kKaStages * 8;
-    static_assert(kKaWarps * HEADS * HD * 4 <= RING_BYTES, "the joined accumulators take the ring's place");
-};
+// 16 consecutive values of a head's group, times `up`.
+SMOE_DEVINL void kv4_load_q(const void* q, size_t at, int dtype, float* x) {
+    if (dtype == SMOE_DTYPE_F32) {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = src[i];
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
+        }
+    } else {                                     // (q's rows are 8-byte aligned: strides are multiples of 4)
+        const uint2* src = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(q) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint2 v = src[i];
+            x[4 * i] = lo_f(v.x);
+            x[4 * i + 1] = hi_f(v.x);
+            x[4 * i + 2] = lo_f(v.y);
+            x[4 * i + 3] = hi_f(v.y);
+        }
+    }
+}
 
-// NG groups of 64 (head_dim / 64), NT tiles of 8 query heads, QP pieces of q.
-template <int NG, int NT, int QP>
-__global__ void __launch_bounds__(kKaWarps * 32, NT == 1 && QP == 1 ? 3 : 2) k_kv4_attention(const Kv4Attn p) {
-    using SM = Kv4AttnSmem<NG, NT>;
-    constexpr uint32_t HD = SM::HD, HEADS = SM::HEADS;
+template <int NG>
+constexpr uint32_t kv4_attn_smem() { return kKaWarps * kKaStages * (NG * 2304 + 8); }
+
+// NG groups of 64 (head_dim / 64), QP pieces of q.
+template <int NG, int QP>
+__global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const Kv4Attn p) {
+    constexpr uint32_t HD = NG * 64, UNIT = NG * 2304, SB = NG * kKvPlane;     // a unit: a page's keys or values, codes then scales
     extern __shared__ __align__(128) uint8_t kv4_smem[];
-    uint8_t* smem = kv4_smem;
     const SmoeKv4Cache& c = p.a.c;
-    const Kv4Geom G(HD);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, cl = lane & 3;
-    const uint32_t split = blockIdx.x, kvh = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks, s = blockIdx.z;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR) + warp * kKaStages;
+    const uint32_t me = blockIdx.x * kKaWarps + warp, nheads = c.num_kv_heads * p.chunks;        // pairs of a sequence
+    uint8_t* ring = kv4_smem + warp * kKaStages * UNIT;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(kv4_smem + kKaWarps * kKaStages * UNIT) + warp * kKaStages;
     pdl_release();
     if (lane == 0) {
         for (int i = 0; i < kKaStages; ++i) mbar_init(bars + i, 1);
@@ -239,246 +307,257 @@ __global__ void __launch_bounds__(kKaWarps * 32, NT == 1 && QP == 1 ? 3 : 2) k_k
     }
     __syncwarp();
     pdl_acquire();
-    const uint32_t n = kv4_valid(p, s), pages = (n + kKvPage - 1) / kKvPage;
-    const uint32_t p0 = split * p.split_pages, p1 = min(pages, p0 + p.split_pages);
-    const uint32_t h0 = chunk * HEADS, heads = min(HEADS, p.group - h0);        // of this CTA, in the KV head's group
-    if (p0 >= p1 && !(n == 0 && p.splits == 1)) return;
+    uint32_t seq;
+    uint64_t start;
+    const Kv4Line L = kv4_line(p, nheads, lane, me, seq, start);
+    const uint64_t t0 = L.first(me), t1 = L.first(me + 1);
+    if (t0 >= t1) return;
+    const uint32_t mine = uint32_t(t1 - t0);
 
-    // this warp's pages: p0 + warp, + 4, ..; their numbers are fetched 32 at a time
-    const uint32_t mine = p1 > p0 + warp ? (p1 - p0 - warp + kKaWarps - 1) / kKaWarps : 0u;
-    uint32_t ids = ~0u, ids_base = 0;
-    auto fetch_ids = [&](uint32_t base) {
-        ids_base = base;
-        ids = base + lane < mine ? kv4_page(c, s, uint64_t(p0 + warp + (base + lane) * kKaWarps) * kKvPage, p.a.err) : ~0u;
-    };
-    if (mine) fetch_ids(0);
-    uint8_t* ring = smem + SM::RING + warp * kKaStages * SM::BLOCK;
-    auto issue = [&](uint32_t i) -> uint32_t {                   // whole warp; the page's number
-        if (i >= ids_base + 32) fetch_ids(i);
-        const uint32_t page = __shfl_sync(0xffffffffu, ids, i - ids_base);
-        if (lane == 0) {
-            if (page != ~0u) {
-                mbar_arrive_expect_tx(bars + i % kKaStages, SM::BLOCK);
-                bulk_g2s(ring + i % kKaStages * SM::BLOCK, c.blocks + (size_t(page) * c.num_kv_heads + kvh) * SM::BLOCK,
-                         SM::BLOCK, bars + i % kKaStages);
+    // where the stretch starts, and the next unit to send for (ahead of the one in work)
+    uint32_t n = kv4_valid(p, seq), np = kv4_pages(n), hc = uint32_t((t0 - start) / np), pg = uint32_t((t0 - start) % np);
+    uint32_t a_seq = seq, a_np = np, a_hc = hc, a_pg = pg, sent = 0;
+    uint32_t a_page = 0, good = 0, slot = 0, phase = 0;          // good: bit i % 2, page i can be read; slot, phase: of the unit in work
+    auto send = [&](uint32_t st) {               // unit `sent`, into slot st
+        if (sent % 2 == 0) {
+            a_page = kv4_page(c, a_seq, uint64_t(a_pg) * kKvPage, p.a.err);
+            good = (good & ~(1u << (sent / 2 % 2))) | uint32_t(a_page != ~0u) << (sent / 2 % 2);
+        }
+        if (elect_one()) {
+            if (a_page != ~0u) {
+                const uint8_t* blk = c.blocks + (size_t(a_page) * c.num_kv_heads + a_hc / p.chunks) * (2 * UNIT);
+                mbar_arrive_expect_tx(bars + st, UNIT);
+                bulk_g2s(ring + st * UNIT, blk + sent % 2 * SB, SB, bars + st);
+                bulk_g2s(ring + st * UNIT + SB, blk + 2 * SB + sent % 2 * (UNIT - SB), UNIT - SB, bars + st);
             } else {
-                mbar_arrive(bars + i % kKaStages);               // nothing to wait for; its entries are masked
+                mbar_arrive(bars + st);          // nothing to wait for; its entries are masked
             }
         }
-        return page;
+        if (++sent % 2 == 0 && sent < 2 * mine && ++a_pg == a_np) {
+            a_pg = 0;
+            if (++a_hc == nheads) {
+                a_hc = 0;
+                do a_np = kv4_pages(kv4_valid(p, ++a_seq));
+                while (a_np == 0);               // (a page is still to come, so there is a sequence that has it)
+            }
+        }
     };
-    uint32_t good = 0;                                           // bit st: the page in stage st can be read
-    const uint32_t early = warp + 1 < kKaWarps ? kKaStages : NT == 1 ? kKaStages - 1 : 0;   // stages that q is not in
-    for (uint32_t i = 0; i < early && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
+    for (int i = 0; i < kKaStages; ++i)
+        if (sent < 2 * mine) send(i);
 
-    // q: fp32 in shared memory, each head times a power of two, its group sums
-    float* qs = reinterpret_cast<float*>(smem + SM::Q);
-    float* qsum = reinterpret_cast<float*>(smem + SM::QSUM);
-    float* qinv = reinterpret_cast<float*>(smem + SM::QINV);
-    for (uint32_t h = warp; h < HEADS; h += kKaWarps) {
-        float x[HD / 32], mx = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < HD / 32; ++i) {
-            const size_t at = s * p.t.q_row + (kvh * p.group + h0 + h) * HD + i * 32 + lane;
-            x[i] = h >= heads ? 0.0f : p.t.dtype == SMOE_DTYPE_F32 ? ld_plain(static_cast<const float*>(p.t.q) + at)
-                                                                    : bf16_bits_to_f32(ld_plain(static_cast<const uint16_t*>(p.t.q) + at));
-            mx = fmaxf(mx, fabsf(x[i]));
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        // 2^e with mx 2^e in [2^14, 2^15), kept within what fp32 can invert (an infinity or NaN in q stays one)
-        const int e = max(-100, min(100, 14 - (int(__float_as_uint(mx) >> 23) - 127)));
-        const float up = __uint_as_float(uint32_t(127 + e) << 23);
-#pragma unroll
-        for (uint32_t i = 0; i < HD / 32; ++i) {
-            // the pieces that go to the tensor cores, and their sum
-            const float y = x[i] * up, hi = __half2float(__float2half_rn(y));
-            const float lo = QP == 2 ? __half2float(__float2half_rn(y - hi)) : 0.0f;
-            qs[h * SM::QROW + i * 32 + lane] = y;
-            x[i] = hi + lo;
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float t = x[2 * g] + x[2 * g + 1];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (lane == 0) qsum[g * HEADS + h] = t;
-        }
-        if (lane == 0) qinv[h] = p.scale_log2 * __uint_as_float(uint32_t(127 - e) << 23);
-    }
-    __syncthreads();
-    // this lane's fragments of q: head gr (+ 8), dimensions in the order kv4_half_codes gives the codes
-    uint32_t qf[NT][NG][4][QP][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const float* y = qs + (nt * 8 + gr) * SM::QROW + g * 64 + cl * 16 + st / 2 * 8 + st % 2 * 2 + b;
-                    const __half y0 = __float2half_rn(y[0]), y1 = __float2half_rn(y[4]);
-                    qf[nt][g][st][0][b] = pack_half2(y0, y1);
-                    if (QP == 2)
-                        qf[nt][g][st][QP - 1][b] = pack_half2(__float2half_rn(y[0] - __half2float(y0)), __float2half_rn(y[4] - __half2float(y1)));
-                }
-    if (early < uint32_t(kKaStages)) fence_proxy_async();        // q's place goes to the bulk copies
-    __syncthreads();
-    for (uint32_t i = early; i < uint32_t(kKaStages) && i < mine; ++i) good |= uint32_t(issue(i) != ~0u) << i;
-    float qsm[NT][NG][2], sc[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            sc[nt][k] = qinv[nt * 8 + 2 * cl + k];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) qsm[nt][g][k] = qsum[g * HEADS + nt * 8 + 2 * cl + k];
-        }
-
-    float m[NT][2], l[NT][2], bacc[NT][NG][2], o[NT][NG][4][4], up[NG];      // up: the group's power of two in o
-#pragma unroll
-    for (int g = 0; g < NG; ++g) up[g] = 0.0f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            m[nt][k] = -INFINITY;
-            l[nt][k] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                bacc[nt][g][k] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[nt][g][i][k] = o[nt][g][i][2 + k] = 0.0f;
-            }
-        }
-    bool failed = false;
-    float* lrow = p.logits ? p.logits + ((size_t(s) * c.num_kv_heads + kvh) * p.rows) * p.gs : nullptr;
-#pragma unroll 1
-    for (uint32_t i = 0; i < mine; ++i) {
-        const uint8_t* blk = ring + i % kKaStages * SM::BLOCK;
-        if (!failed && !mbar_wait_bounded(bars + i % kKaStages, (i / kKaStages) & 1)) {
+    uint32_t qf[NG][4][QP][2];                   // fragments of q: head gr, dimensions in the order kv4_half_codes gives the codes
+    float qsm[NG][2], sc[2];                     // of the heads 2 cl, 2 cl + 1: the groups' sums; scale_log2 over the head's power of two
+    float m[2], l[2], bacc[NG][2], o[NG][4][4], up[NG];          // up: the group's power of two in o
+    bool failed = false, fresh = true;           // fresh: the pair starts with this page
+    uint32_t heads = 0, head0 = 0;               // of the pair: query heads and the first of them
+    float* lrow = nullptr;
+    auto arrived = [&]() {
+        if (!failed && !mbar_wait_bounded(bars + slot, phase)) {
             failed = true;                       // (the results are void, the error word says so)
             atomicCAS(p.a.err, 0u, uint32_t(SMOE_DEVERR_MBAR_TIMEOUT));
         }
-        const uint32_t e0 = (p0 + warp + i * kKaWarps) * kKvPage;
-        const uint32_t have = good >> (i % kKaStages) & 1u ? min(kKvPage, n - e0) : 0u;        // entries of this page
-        float x[4][NT][4];                       // scores: entry 16 mt + gr (0, 1) and + 8 (2, 3), heads 2 cl, 2 cl + 1
+    };
+    auto read = [&]() {                          // the unit in work has been read: its slot for the one three further on
+        __syncwarp();
+        if (sent < 2 * mine) send(slot);
+        if (++slot == uint32_t(kKaStages)) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; i < mine; ++i) {
+        if (fresh) {
+            fresh = false;
+            if (pg == 0 && lane == 0)            // this warp is the pair's first one
+                p.meta[uint64_t(seq) * nheads + hc] = make_uint2(me, uint32_t((t0 + i + np - 1) / L.per) - me + 1);
+            const uint32_t kvh = hc / p.chunks, h0 = hc % p.chunks * kKaHeads;
+            heads = min(kKaHeads, p.group - h0);
+            head0 = kvh * p.group + h0;
+            lrow = p.logits ? p.logits + (size_t(seq) * p.t.num_heads + head0 + 2 * cl) * p.rows + gr : nullptr;
+            float x[NG][16], mx = 0.0f, sum[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (gr < heads) kv4_load_q(p.t.q, seq * p.t.q_row + size_t(head0 + gr) * HD + g * 64 + cl * 16, p.t.dtype, x[g]);
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    if (gr >= heads) x[g][d] = 0.0f;
+                    mx = fmaxf(mx, fabsf(x[g][d]));
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // 2^e with mx 2^e in [2^14, 2^15), kept within what fp32 can invert (an infinity or NaN in q stays one)
+            const int e = max(-100, min(100, 14 - (int(__float_as_uint(mx) >> 23) - 127)));
+            const float by = __uint_as_float(uint32_t(127 + e) << 23), inv = p.scale_log2 * __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                sum[g] = 0.0f;
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int d = st / 2 * 8 + st % 2 * 2 + b;
+                        const float y0 = x[g][d] * by, y1 = x[g][d + 4] * by;
+                        const uint32_t hi = cvt_f16x2(y0, y1);
+                        qf[g][st][0][b] = hi;
+                        sum[g] += half_lo(hi) + half_hi(hi);
+                        if (QP == 2) {
+                            const uint32_t lo = cvt_f16x2(y0 - half_lo(hi), y1 - half_hi(hi));
+                            qf[g][st][QP - 1][b] = lo;
+                            sum[g] += half_lo(lo) + half_hi(lo);
+                        }
+                    }
+                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+                up[g] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int from = (2 * cl + k) * 4;
+                sc[k] = __shfl_sync(0xffffffffu, inv, from);
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    qsm[g][k] = __shfl_sync(0xffffffffu, sum[g], from);
+                    bacc[g][k] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[g][j][k] = o[g][j][2 + k] = 0.0f;
+                }
+            }
+        }
+        const uint32_t e0 = pg * kKvPage;
+        const uint32_t have = good >> (i % 2) & 1u ? min(kKvPage, n - e0) : 0u;                // entries of this page
+        const uint8_t* blk = ring + slot * UNIT;
+        arrived();
+        float x[4][4];                           // scores: entry 16 mt + gr (0, 1) and + 8 (2, 3), heads 2 cl, 2 cl + 1
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
             const uint32_t ka = mt * 16 + gr, kb = ka + 8;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[mt][nt][k] = 0.0f;
+            uint2 wa[NG], wb[NG];
+            uint32_t sa[NG], sb[NG];
+            float d[NG][4];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint2 wa = *reinterpret_cast<const uint2*>(blk + G.codes(0, g) + ka * 32 + cl * 8);
-                const uint2 wb = *reinterpret_cast<const uint2*>(blk + G.codes(0, g) + kb * 32 + cl * 8);
-                const uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, g) + ka * 4);
-                const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, g) + kb * 4);
-                float d[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    uint32_t ra[4], rb[4];
-                    kv4_half_codes(w ? wa.y : wa.x, ra);
-                    kv4_half_codes(w ? wb.y : wb.x, rb);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t af[4] = {ra[2 * h], rb[2 * h], ra[2 * h + 1], rb[2 * h + 1]};
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int q = 0; q < QP; ++q)
-                                mma_f16f32_16816(d[nt], af, qf[nt][g][w * 2 + h][q][0], qf[nt][g][w * 2 + h][q][1]);
-                    }
-                }
-                const float s0 = lo_f(sa), b0 = hi_f(sa), s1 = lo_f(sb), b1 = hi_f(sb);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        x[mt][nt][k] = fmaf(s0, d[nt][k], fmaf(b0, qsm[nt][g][k], x[mt][nt][k]));
-                        x[mt][nt][2 + k] = fmaf(s1, d[nt][2 + k], fmaf(b1, qsm[nt][g][k], x[mt][nt][2 + k]));
-                    }
+                wa[g] = *reinterpret_cast<const uint2*>(blk + g * kKvPlane + ka * 32 + cl * 8);
+                wb[g] = *reinterpret_cast<const uint2*>(blk + g * kKvPlane + kb * 32 + cl * 8);
+                sa[g] = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + ka * 4);
+                sb[g] = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + kb * 4);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int w = 0; w < 2; ++w) {        // (the groups' chains of products side by side)
+                uint32_t ra[NG][4], rb[NG][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[mt][nt][k] *= sc[nt][k & 1];
+                for (int g = 0; g < NG; ++g) {
+                    kv4_half_codes(w ? wa[g].y : wa[g].x, ra[g]);
+                    kv4_half_codes(w ? wb[g].y : wb[g].x, rb[g]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < QP; ++q)
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            const uint32_t af[4] = {ra[g][2 * h], rb[g][2 * h], ra[g][2 * h + 1], rb[g][2 * h + 1]};
+                            if (w + h + q == 0) mma_f16f32_16816_z(d[g], af, qf[g][0][0][0], qf[g][0][0][1]);
+                            else mma_f16f32_16816(d[g], af, qf[g][w * 2 + h][q][0], qf[g][w * 2 + h][q][1]);
+                        }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float s0 = lo_f(sa[g]), b0 = hi_f(sa[g]), s1 = lo_f(sb[g]), b1 = hi_f(sb[g]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    x[mt][k] = fmaf(s0, d[g][k], g ? fmaf(b0, qsm[g][k], x[mt][k]) : b0 * qsm[g][k]);
+                    x[mt][2 + k] = fmaf(s1, d[g][2 + k], g ? fmaf(b1, qsm[g][k], x[mt][2 + k]) : b1 * qsm[g][k]);
+                }
+            }
         }
+        read();
         if (have < kKvPage)
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (mt * 16 + gr + (k < 2 ? 0 : 8) >= have) x[mt][nt][k] = -INFINITY;
+                for (int k = 0; k < 4; ++k)
+                    if (mt * 16 + gr + (k < 2 ? 0 : 8) >= have) x[mt][k] = -INFINITY;
         if (lrow) {
-            float* at = lrow + size_t(e0 + gr) * p.gs + h0 + 2 * cl;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int k = 0; k < 2; ++k)
+                if (2 * cl + k < heads) {        // (the last page's rows are there, whatever its entries)
+                    float* at = lrow + size_t(k) * p.rows + e0;
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (nt * 8 + 2 * cl < heads && e0 + mt * 16 + k * 8 + gr < n)
-                            *reinterpret_cast<float2*>(at + (mt * 16 + k * 8) * p.gs + nt * 8) = make_float2(x[mt][nt][2 * k], x[mt][nt][2 * k + 1]);
-        }
-        // running maximum; moved only when it is 2^8 too low
-        float f[NT][2];
-        bool move = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float mx = x[0][nt][k];
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt) mx = fmaxf(fmaxf(mx, x[mt][nt][k]), x[mt][nt][2 + k]);
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                f[nt][k] = 1.0f;
-                if (mx > m[nt][k] + 8.0f || (mx > m[nt][k] && m[nt][k] == -INFINITY)) {
-                    f[nt][k] = m[nt][k] == -INFINITY ? 0.0f : kv4_ex2(m[nt][k] - mx);
-                    m[nt][k] = mx;
-                    move = true;
-                }
-            }
-        if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    l[nt][k] *= f[nt][k];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        bacc[nt][g][k] *= f[nt][k];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            o[nt][g][j][k] *= f[nt][k];
-                            o[nt][g][j][2 + k] *= f[nt][k];
-                        }
+                    for (int mt = 0; mt < 4; ++mt) {
+                        at[mt * 16] = x[mt][k] * sc[k];
+                        at[mt * 16 + 8] = x[mt][2 + k] * sc[k];
                     }
                 }
+        }
+        // running maximum (of the scaled scores); moved only when it is 2^8 too low
+        float f[2];
+        bool move = false;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float mx = x[0][k];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) mx = fmaxf(fmaxf(mx, x[mt][k]), x[mt][2 + k]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx *= sc[k];                         // (the scale is positive)
+            f[k] = 1.0f;
+            if (mx > m[k] + 8.0f || (mx > m[k] && m[k] == -INFINITY)) {
+                f[k] = m[k] == -INFINITY ? 0.0f : kv4_ex2(m[k] - mx);
+                m[k] = mx;
+                move = true;
+            }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                l[k] *= f[k];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    bacc[g][k] *= f[k];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        o[g][j][k] *= f[k];
+                        o[g][j][2 + k] *= f[k];
+                    }
+                }
+            }
+        }
+        const float mm[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[mt][k] = kv4_ex2(fmaf(x[mt][k], sc[k & 1], -mm[k & 1]));
+                l[k & 1] += x[mt][k];
+            }
+        blk = ring + slot * UNIT;
+        arrived();
+        if (have < kKvPage) {                    // entries past the last one may hold anything: their scales and biases become 0
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (uint32_t e = lane; e < kKvPage; e += 32)
+                    if (e >= have) *reinterpret_cast<uint32_t*>(ring + slot * UNIT + SB + g * 256 + e * 4) = 0u;
+            __syncwarp();
+            fence_proxy_async();                 // (the slot goes to a bulk copy next)
         }
         // the power of two of a group's p s: its largest scale near 2^3, and below
         // 2^7 as pages follow, so that with p <= 2^8 nothing passes fp16's range
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const uint2 w = *reinterpret_cast<const uint2*>(blk + G.sb(1, g) + lane * 8);
-            const uint32_t big = __reduce_max_sync(0xffffffffu, max(2 * lane < have ? w.x & 0x7fffu : 0u, 2 * lane + 1 < have ? w.y & 0x7fffu : 0u));
+            const uint2 w = *reinterpret_cast<const uint2*>(blk + SB + g * 256 + lane * 8);
+            const uint32_t big = __reduce_max_sync(0xffffffffu, max(w.x & 0x7fffu, w.y & 0x7fffu));
             if (__uint_as_float(big << 16) * up[g] > 128.0f || up[g] == 0.0f) {
                 const float now = __uint_as_float(uint32_t(max(27, min(227, 257 - int(big >> 7)))) << 23);
                 const float r = up[g] == 0.0f ? 0.0f : now / up[g];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) o[nt][g][j][k] *= r;
+                    for (int k = 0; k < 4; ++k) o[g][j][k] *= r;
                 up[g] = now;
             }
         }
@@ -486,226 +565,233 @@ __global__ void __launch_bounds__(kKaWarps * 32, NT == 1 && QP == 1 ? 3 : 2) k_k
         for (int mt = 0; mt < 4; ++mt) {
             const uint32_t ka = mt * 16 + gr, kb = ka + 8;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float mm = m[nt][k & 1] == -INFINITY ? 0.0f : m[nt][k & 1];
-                    x[mt][nt][k] = kv4_ex2(x[mt][nt][k] - mm);
-                    l[nt][k & 1] += x[mt][nt][k];
-                }
-#pragma unroll
             for (int g = 0; g < NG; ++g) {
-                // entries past the last one may hold anything: their scales count as 0
-                uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + ka * 4);
-                uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(1, g) + kb * 4);
-                if (have < kKvPage) {
-                    if (ka >= have) sa = 0u;
-                    if (kb >= have) sb = 0u;
-                }
+                const uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + ka * 4);
+                const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + kb * 4);
                 const float s0 = lo_f(sa) * up[g], b0 = hi_f(sa), s1 = lo_f(sb) * up[g], b1 = hi_f(sb);
                 // codes of this lane's 8 dimensions (8 gr ..) of the entries 2 cl, 2 cl + 1, 2 cl + 8, 2 cl + 9 of the tile;
                 // lanes cl >= 2 load the pair the other way round (the four entries of a load then lie in different banks)
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    w[k] = *reinterpret_cast<const uint32_t*>(blk + G.codes(1, g) + (mt * 16 + 2 * cl + ((k & 1) ^ (cl >> 1)) + (k >> 1) * 8) * 32 + gr * 4);
-                // even and odd bytes of the pair side by side, so that a register's halves are the two entries' codes of one dimension
+                    w[k] = *reinterpret_cast<const uint32_t*>(blk + g * kKvPlane + (mt * 16 + 2 * cl + ((k & 1) ^ (cl >> 1)) + (k >> 1) * 8) * 32 + gr * 4);
+                // halves of the pair's words side by side, so that a register's halves are the two entries' codes of one dimension
                 const uint32_t p_lo = cl < 2 ? 0x5410u : 0x1054u, p_hi = cl < 2 ? 0x7632u : 0x3276u;
                 uint32_t c0[8], c1[8];           // dimension n: entries (2 cl, 2 cl + 1), and + 8
                 kv4_half_codes(__byte_perm(w[0], w[1], p_lo), c0);
                 kv4_half_codes(__byte_perm(w[0], w[1], p_hi), c0 + 4);
                 kv4_half_codes(__byte_perm(w[2], w[3], p_lo), c1);
                 kv4_half_codes(__byte_perm(w[2], w[3], p_hi), c1 + 4);
+                bacc[g][0] = fmaf(x[mt][0], b0, fmaf(x[mt][2], b1, bacc[g][0]));
+                bacc[g][1] = fmaf(x[mt][1], b0, fmaf(x[mt][3], b1, bacc[g][1]));
+                const float y0 = x[mt][0] * s0, y1 = x[mt][1] * s0, y2 = x[mt][2] * s1, y3 = x[mt][3] * s1;
+                const uint32_t u0 = cvt_f16x2(y0, y1), u1 = cvt_f16x2(y2, y3);
+                const uint32_t v0 = movm_trans(cvt_f16x2(y0 - half_lo(u0), y1 - half_hi(u0)));
+                const uint32_t v1 = movm_trans(cvt_f16x2(y2 - half_lo(u1), y3 - half_hi(u1)));
+                const uint32_t z0 = movm_trans(u0), z1 = movm_trans(u1);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    bacc[nt][g][0] = fmaf(x[mt][nt][0], b0, fmaf(x[mt][nt][2], b1, bacc[nt][g][0]));
-                    bacc[nt][g][1] = fmaf(x[mt][nt][1], b0, fmaf(x[mt][nt][3], b1, bacc[nt][g][1]));
-                    const float y0 = x[mt][nt][0] * s0, y1 = x[mt][nt][1] * s0, y2 = x[mt][nt][2] * s1, y3 = x[mt][nt][3] * s1;
-                    const uint32_t u0 = cvt_f16x2(y0, y1), u1 = cvt_f16x2(y2, y3);
-                    const uint32_t t0 = movm_trans(u0), t1 = movm_trans(u1);
-                    const uint32_t v0 = movm_trans(cvt_f16x2(y0 - half_lo(u0), y1 - half_hi(u0)));
-                    const uint32_t v1 = movm_trans(cvt_f16x2(y2 - half_lo(u1), y3 - half_hi(u1)));
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t af[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
+                    mma_f16f32_16816(o[g][j], af, z0, z1);
+                }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t af[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
-                        mma_f16f32_16816(o[nt][g][j], af, t0, t1);
-                        mma_f16f32_16816(o[nt][g][j], af, v0, v1);
-                    }
+                for (int j = 0; j < 4; ++j) {    // (apart from the first pieces': those of one accumulator wait for one another)
+                    const uint32_t af[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
+                    mma_f16f32_16816(o[g][j], af, v0, v1);
                 }
             }
         }
-        __syncwarp();                            // the stage has been read
-        if (i + kKaStages < mine) {
-            const uint32_t bit = i % kKaStages;
-            good = (good & ~(1u << bit)) | uint32_t(issue(i + kKaStages) != ~0u) << bit;
+        read();
+        const bool whole = pg + 1 == np;         // the pair's last page
+        if (whole || i + 1 == mine) {
+            fresh = true;
+            const uint64_t pair = uint64_t(seq) * nheads + hc;
+            const bool alone = whole && i + 1 >= np && !p.logits;               // its first page was in this stretch, too
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) bacc[g][k] += __shfl_xor_sync(0xffffffffu, bacc[g][k], d);
+                }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t h = 2 * cl + k;
+                const float inv = 1.0f / l[k];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const float down = up[g] == 0.0f ? 0.0f : 1.0f / up[g];      // (exact: a power of two)
+                    float v[8];                  // dimensions 8 gr .. of the group
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[2 * j] = fmaf(o[g][j][k], down, bacc[g][k]);
+                        v[2 * j + 1] = fmaf(o[g][j][2 + k], down, bacc[g][k]);
+                    }
+                    if (!alone) {
+                        float4* dst = reinterpret_cast<float4*>(p.part + ((me + pair) * kKaHeads + h) * HD + g * 64 + gr * 8);
+                        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    } else if (h < heads) {
+                        const size_t at = seq * p.t.out_row + size_t(head0 + h) * HD + g * 64 + gr * 8;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] *= inv;
+                        if (p.t.dtype == SMOE_DTYPE_F32) {
+                            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.t.out) + at);
+                            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                        } else {                 // (rows are 8-byte aligned: strides are multiples of 4)
+                            uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.t.out) + at);
+                            dst[0] = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                            dst[1] = make_uint2(pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+                        }
+                    }
+                }
+                if (!alone && gr == 0) p.stat[(me + pair) * kKaHeads + h] = make_float2(m[k], l[k]);
+            }
+        }
+        if (i + 1 < mine && ++pg == np) {
+            pg = 0;
+            if (++hc == nheads) {
+                hc = 0;
+                do n = kv4_valid(p, ++seq), np = kv4_pages(n);
+                while (np == 0);
+            }
         }
     }
     if (failed)                                  // no copy may be in flight when the CTA ends
-        for (uint32_t i = mine > uint32_t(kKaStages) ? mine - kKaStages : 0u; i < mine; ++i)
-            mbar_wait_bounded(bars + i % kKaStages, (i / kKaStages) & 1);
-
-    // join the lanes' sums, then the warps
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) bacc[nt][g][k] += __shfl_xor_sync(0xffffffffu, bacc[nt][g][k], d);
-            }
-    float* ml = reinterpret_cast<float*>(smem + SM::ML);
-    if (gr == 0)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float* at = ml + (warp * HEADS + nt * 8 + 2 * cl + k) * 2;
-                at[0] = m[nt][k];
-                at[1] = l[nt][k];
-            }
-    __syncthreads();                             // (every warp is done with its ring, too)
-    float* acc = reinterpret_cast<float*>(smem + SM::RING) + warp * HEADS * HD;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float* at = acc + (nt * 8 + 2 * cl + k) * HD + g * 64 + gr * 8 + 2 * j;
-                    const float down = up[g] == 0.0f ? 0.0f : 1.0f / up[g];          // (exact: a power of two)
-                    *reinterpret_cast<float2*>(at) = make_float2(fmaf(o[nt][g][j][k], down, bacc[nt][g][k]), fmaf(o[nt][g][j][2 + k], down, bacc[nt][g][k]));
-                }
-    __syncthreads();
-    acc = reinterpret_cast<float*>(smem + SM::RING);
-    for (uint32_t h = warp; h < heads; h += kKaWarps) {
-        float top = -INFINITY, sum = 0.0f, f[kKaWarps];
-#pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, ml[(w * HEADS + h) * 2]);
-#pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) {
-            const float mw = ml[(w * HEADS + h) * 2];
-            f[w] = mw == -INFINITY ? 0.0f : kv4_ex2(mw - top);
-            // (a warp without entries has zeros; one whose statistics are NaN passes them on)
-            sum = fmaf(ml[(w * HEADS + h) * 2 + 1], mw == -INFINITY ? 1.0f : f[w], sum);
-        }
-        const uint32_t head = kvh * p.group + h0 + h;
-        if (p.part) {
-            const size_t at = (size_t(s) * p.t.num_heads + head) * p.splits + split;
-            float* dst = p.part + at * HD;
-#pragma unroll
-            for (uint32_t i = 0; i < HD / 32; ++i) {
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kKaWarps; ++w) v = fmaf(acc[(w * HEADS + h) * HD + i * 32 + lane], f[w], v);
-                dst[i * 32 + lane] = v;
-            }
-            if (lane == 0) p.stat[at] = make_float2(top, sum);
-        } else {
-            const float inv = n ? 1.0f / sum : 0.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < HD / 32; ++i) {
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kKaWarps; ++w) v = fmaf(acc[(w * HEADS + h) * HD + i * 32 + lane], f[w], v);
-                const size_t at = s * p.t.out_row + head * HD + i * 32 + lane;
-                if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v * inv;
-                else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v * inv);
-            }
-        }
-    }
+        for (uint32_t u = 2 * mine > uint32_t(kKaStages) ? 2 * mine - kKaStages : 0u; u < 2 * mine; ++u)
+            mbar_wait_bounded(bars + u % kKaStages, (u / kKaStages) & 1);
 }
 
-// The parts of a (sequence, KV head): its query heads' results from the
-// splits in their order, and - with weights - each entry's new weight from
-// the stored scores and the heads' joined maximum and sum. grid (x, KV head,
-// sequence): every CTA forms the statistics it needs again; the first
-// `outs` take kKjOuts outputs each (four threads an output, a quarter of
-// the splits each, so that the chain of loads is short), the others 1024
-// entries each.
-constexpr int kKjThreads = 256, kKjOuts = 64, kKjEntries = 4 * kKjThreads;
+// The parts of the pairs joined in their order, and with weights each entry's
+// new weight from the stored scores. grid (x, KV head, sequence): the first
+// `outs` CTAs take 1024 / lanes outputs each, 4 a thread, `lanes` threads
+// sharing the parts of an output (many parts, few outputs: the chain of loads
+// stays short); the others 1024 entries each, 4 a thread. Every CTA first
+// forms the maxima and sums of the heads that it needs from the parts'
+// (contiguous: a thread a head and every 32nd part).
+constexpr int kKjThreads = 256, kKjEntries = 4 * kKjThreads;
 __global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p, uint32_t outs) {
-    extern __shared__ float kv4_join_smem[];     // [group] log2 of the sum of exponentials; weights of the splits
-    __shared__ float part_sum[kKjThreads];
+    constexpr uint32_t heads = kKaHeads;
+    extern __shared__ float2 kv4_stat[];         // [chunks][heads] maximum; 1 / sum (outputs) or log2 of the sum (weights)
+    __shared__ float2 red[kKjThreads];
+    __shared__ float4 part_v[kKjThreads];
     pdl_release();
     pdl_acquire();
     const SmoeKv4Cache& c = p.a.c;
     const uint32_t kvh = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = c.head_dim;
-    const uint32_t n = kv4_valid(p, s), pages = (n + kKvPage - 1) / kKvPage;
-    const uint32_t splits = (pages + p.split_pages - 1) / p.split_pages;       // those that have entries
     const bool is_out = blockIdx.x < outs;
-    const uint32_t e0 = (blockIdx.x - outs) * kKjEntries;
-    if (!is_out && e0 >= n) return;
-    const size_t first = (size_t(s) * p.t.num_heads + kvh * p.group) * p.splits;
-    // an output CTA's 64 outputs belong to one head (head_dim is 64 or 128)
-    const uint32_t h_lo = is_out ? blockIdx.x * kKjOuts / HD : 0u, h_hi = is_out ? h_lo + 1 : p.group;
-    float* lse = kv4_join_smem;
-    float* wgt = kv4_join_smem + p.group;        // [splits] of the output CTA's head: its share of the whole
-    for (uint32_t h = h_lo + warp; h < h_hi; h += kKjThreads / 32) {
-        const float2* st = p.stat + first + size_t(h) * p.splits;
-        float mx = -INFINITY, sum = 0.0f;
-        for (uint32_t i = lane; i < splits; i += 32) mx = fmaxf(mx, st[i].x);
+    const uint32_t quads = kKjThreads / p.lanes, at = (blockIdx.x * quads + tid % quads) * 4, h = at / HD, d = at % HD;
+    // a CTA's outputs belong to one round of heads: 1024 / lanes divides heads x HD (lanes >= 2 at HD 64)
+    const uint32_t ch0 = is_out ? blockIdx.x * quads * 4 / HD / heads : 0u, ch1 = is_out ? ch0 + 1 : p.chunks;
+    const uint64_t pair0 = (uint64_t(s) * c.num_kv_heads + kvh) * p.chunks;
+    uint2 mt = p.meta[pair0 + ch0];              // (of a sequence without entries: anything)
+    const uint32_t n = kv4_valid(p, s), e = (blockIdx.x - outs) * kKjEntries + tid * 4;
+    if (!is_out && (blockIdx.x - outs) * kKjEntries >= n) return;
+    if (is_out && n && mt.y == 1 && !p.logits) return;           // one part: its warp has written the outputs
+    // the entries' page and old weights, fetched while the statistics come in
+    uint32_t page = ~0u;
+    size_t to = 0;
+    float old[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!is_out && e < n) {
+        page = kv4_page(c, s, e, p.a.err);       // (4 entries lie in one page)
+        to = (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
+        if (page != ~0u && c.score && p.t.decay != 0.0f)
 #pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        for (uint32_t i = lane; i < splits; i += 32)
-            sum = fmaf(st[i].y, st[i].x == -INFINITY ? 1.0f : kv4_ex2(st[i].x - mx), sum);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) lse[h] = mx + log2f(sum);
-        if (is_out) {
-            const float inv = 1.0f / sum;
-            for (uint32_t i = lane; i < splits; i += 32) wgt[i] = st[i].x == -INFINITY ? sum * 0.0f : kv4_ex2(st[i].x - mx) * inv;
-        }
+            for (int k = 0; k < 4; ++k)
+                if (e + k < n) old[k] = c.score[to + k] * p.t.decay;
     }
-    __syncthreads();
-    if (is_out) {
-        const uint32_t q = tid / kKjOuts, d = (blockIdx.x * kKjOuts + tid % kKjOuts) % HD;
-        const float* src = p.part + (first + size_t(h_lo) * p.splits) * HD + d;
-        float v = 0.0f;
-#pragma unroll 8
-        for (uint32_t j = q; j < splits; j += kKjThreads / kKjOuts) v = fmaf(src[size_t(j) * HD], wgt[j], v);
-        part_sum[tid] = v;
-        __syncthreads();
-        if (tid < kKjOuts) {
-            v = (part_sum[tid] + part_sum[tid + kKjOuts]) + (part_sum[tid + 2 * kKjOuts] + part_sum[tid + 3 * kKjOuts]);
-            const size_t at = s * p.t.out_row + (kvh * p.group + h_lo) * HD + d;
-            if (p.t.dtype == SMOE_DTYPE_F32) static_cast<float*>(p.t.out)[at] = v;
-            else static_cast<__nv_bfloat16*>(p.t.out)[at] = __float2bfloat16_rn(v);
+    for (uint32_t ch = ch0; ch < ch1; ++ch) {
+        if (ch > ch0) mt = p.meta[pair0 + ch];
+        const uint32_t parts = n ? mt.y : 0u;
+        const float2* st = p.stat + (mt.x + pair0 + ch) * heads + tid % heads;
+        float mx = -INFINITY, sum = 0.0f;
+        for (uint32_t j0 = tid / heads; j0 < parts; j0 += 8 * kKjThreads / heads) {
+            float2 t[8];
+            float now = mx;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t j = j0 + k * (kKjThreads / heads);
+                t[k] = j < parts ? st[uint64_t(j) * heads] : make_float2(-INFINITY, 0.0f);
+                now = fmaxf(now, t[k].x);
+            }
+            sum *= mx == -INFINITY ? 1.0f : kv4_ex2(mx - now);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = fmaf(t[k].y, t[k].x == -INFINITY ? 1.0f : kv4_ex2(t[k].x - now), sum);
+            mx = now;
         }
+        red[tid] = make_float2(mx, sum);
+        __syncthreads();
+        for (uint32_t k = warp; k < heads; k += kKjThreads / 32) {
+            const float2 t = lane < kKjThreads / heads ? red[lane * heads + k] : make_float2(-INFINITY, 0.0f);
+            float top = t.x;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float all = t.y * (t.x == -INFINITY ? 1.0f : kv4_ex2(t.x - top));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            if (lane == 0) kv4_stat[(ch - ch0) * heads + k] = make_float2(top, is_out ? 1.0f / all : top + log2f(all));
+        }
+        __syncthreads();
+    }
+    if (is_out) {
+        const uint32_t q = tid / quads, parts = n && h < p.group ? mt.y : 0u;
+        const uint64_t first = (mt.x + pair0 + ch0) * heads + h % heads;
+        const float2 all = kv4_stat[h % heads];
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (uint32_t j = q; j < parts; j += p.lanes) {
+            const uint64_t row = first + uint64_t(j) * heads;
+            const float4 x = *reinterpret_cast<const float4*>(p.part + row * HD + d);
+            const float mj = p.stat[row].x, f = mj == -INFINITY ? 0.0f : kv4_ex2(mj - all.x);
+            v.x = fmaf(x.x, f, v.x);
+            v.y = fmaf(x.y, f, v.y);
+            v.z = fmaf(x.z, f, v.z);
+            v.w = fmaf(x.w, f, v.w);
+        }
+        if (p.lanes > 1) {
+            part_v[tid] = v;
+            __syncthreads();
+        }
+        if (q != 0 || h >= p.group) return;
+        for (uint32_t i = 1; i < p.lanes; ++i) {
+            const float4 x = part_v[tid + i * quads];
+            v.x += x.x;
+            v.y += x.y;
+            v.z += x.z;
+            v.w += x.w;
+        }
+        const float inv = n ? all.y : 0.0f;
+        const size_t dst = s * p.t.out_row + size_t(kvh * p.group + h) * HD + d;
+        if (p.t.dtype == SMOE_DTYPE_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.t.out) + dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.t.out) + dst) =
+                make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
         return;
     }
-    const float* row = p.logits + (size_t(s) * c.num_kv_heads + kvh) * p.rows * p.gs;
-    float w[4], old[4];
-    size_t at[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t e = e0 + k * kKjThreads + tid, page = e < n ? kv4_page(c, s, e, p.a.err) : ~0u;
-        at[k] = page == ~0u ? ~size_t(0) : (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
-        old[k] = page != ~0u && c.score && p.t.decay != 0.0f ? c.score[at[k]] * p.t.decay : 0.0f;
-        w[k] = 0.0f;
+    if (page == ~0u) return;
+    float4 w = make_float4(old[0], old[1], old[2], old[3]);
+    const float* x = p.logits + (size_t(s) * p.t.num_heads + kvh * p.group) * p.rows + e;
+#pragma unroll 8
+    for (uint32_t k = 0; k < p.group; ++k) {
+        const float4 y = *reinterpret_cast<const float4*>(x + size_t(k) * p.rows);
+        const float l = kv4_stat[k].y;           // (rounds of heads follow one another)
+        w.x += kv4_ex2(y.x - l);
+        w.y += kv4_ex2(y.y - l);
+        w.z += kv4_ex2(y.z - l);
+        w.w += kv4_ex2(y.w - l);
     }
-    uint32_t h = 0;
-    if (p.gs % 4 == 0)
-        for (; h + 4 <= p.group; h += 4) {
-            float4 y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                y[k] = at[k] == ~size_t(0) ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                           : *reinterpret_cast<const float4*>(row + size_t(e0 + k * kKjThreads + tid) * p.gs + h);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[k] += (kv4_ex2(y[k].x - lse[h]) + kv4_ex2(y[k].y - lse[h + 1])) + (kv4_ex2(y[k].z - lse[h + 2]) + kv4_ex2(y[k].w - lse[h + 3]));
-        }
-    for (; h < p.group; ++h)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (at[k] != ~size_t(0)) w[k] += kv4_ex2(row[size_t(e0 + k * kKjThreads + tid) * p.gs + h] - lse[h]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (at[k] != ~size_t(0)) p.t.score_out[at[k]] = old[k] + w[k];
+    float* dst = p.t.score_out + to;
+    if (e + 4 <= n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+        *reinterpret_cast<float4*>(dst) = w;
+    } else {
+        dst[0] = w.x;
+        if (e + 1 < n) dst[1] = w.y;
+        if (e + 2 < n) dst[2] = w.z;
+        if (e + 3 < n) dst[3] = w.w;
+    }
 }
 
 // ----------------------------------------------------------------- eviction

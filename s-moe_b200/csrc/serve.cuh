@@ -34,6 +34,16 @@ SMOE_DEVINL void pdl_acquire() { asm volatile("griddepcontrol.wait;" ::: "memory
 template <typename T>
 SMOE_DEVINL T ld_plain(const T* p) { return *p; }
 
+// One lane of a converged warp. Bulk copies and tensor-core instructions take
+// their operands from uniform registers: under this predicate the compiler
+// moves them there once, under `lane == 0` it adds a loop over the lanes'
+// values to each (some 40 instructions a copy).
+SMOE_DEVINL bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 SMOE_DEVINL void serve_err(uint32_t* err, uint32_t code) { atomicCAS(err, 0u, code); }
 
 // The sequence s with cu[s] <= row < cu[s + 1] (cu ascending, cu[0] = 0), by

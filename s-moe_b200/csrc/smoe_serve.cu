@@ -101,23 +101,24 @@ int check_rows(const SmoeKv4Rows* r, const char* what) {
     return SMOE_OK;
 }
 
-// How a 4-bit attention call is cut, from its arguments alone (the workspace
-// is asked for without a context).
+// A 4-bit attention call's launch and workspace, from its arguments alone
+// (the workspace is asked for without a context).
 struct AttnPlan {
-    uint32_t split_pages, splits, gs;
-    uint64_t part_bytes, logit_bytes;
+    uint32_t group, chunks, rows;
+    uint64_t parts, part_bytes, stat_bytes, meta_bytes, logit_bytes;
     AttnPlan(const SmoeKv4Cache& c, const SmoeKv4AttnArgs& t) {
-        const uint64_t pages = (uint64_t(t.max_len) + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE;
-        const uint64_t pairs = uint64_t(c.n_seqs) * c.num_kv_heads;
-        // about 900 CTAs (two rounds of three a SM), 16 pages (4 a warp) at least
-        uint64_t want = std::max<uint64_t>(1, 900 / std::max<uint64_t>(pairs, 1));
-        split_pages = uint32_t(std::max<uint64_t>(16, ((pages + want - 1) / want + 3) / 4 * 4));
-        splits = uint32_t(std::max<uint64_t>(1, (pages + split_pages - 1) / split_pages));
-        const uint32_t group = t.num_heads / c.num_kv_heads;
-        gs = (group + 1) & ~1u;
-        part_bytes = splits > 1 || t.score_out ? (pairs * group * splits * (c.head_dim + 2) * 4 + 255) / 256 * 256 : 0;   // sums, then statistics
-        logit_bytes = t.score_out ? pairs * t.max_len * gs * 4 : 0;
+        group = t.num_heads / c.num_kv_heads;
+        chunks = (group + smoe::kKaHeads - 1) / smoe::kKaHeads;
+        rows = (t.max_len + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE * SMOE_KV4_PAGE;
+        const uint64_t pairs = uint64_t(c.n_seqs) * c.num_kv_heads * chunks, all_heads = uint64_t(c.n_seqs) * t.num_heads;
+        auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
+        parts = uint64_t(smoe::kKaGrid) * smoe::kKaWarps + pairs;
+        part_bytes = up(parts * smoe::kKaHeads * c.head_dim * 4);
+        stat_bytes = up(parts * smoe::kKaHeads * 8);
+        meta_bytes = up(pairs * 8);
+        logit_bytes = t.score_out ? all_heads * rows * 4 : 0;
     }
+    uint64_t bytes() const { return part_bytes + stat_bytes + meta_bytes + logit_bytes; }
 };
 
 }  // namespace
@@ -188,8 +189,7 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
 
 uint64_t smoe_cuda_kv4_attention_workspace(const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
     if (!cache || !t || cache->num_kv_heads == 0) return 0;
-    const AttnPlan plan(*cache, *t);
-    return plan.part_bytes + plan.logit_bytes;
+    return AttnPlan(*cache, *t).bytes();
 }
 
 int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
@@ -198,6 +198,7 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     if (rc) return rc;
     if (!t->q || !t->out || t->num_heads == 0 || t->num_heads % cache->num_kv_heads || t->max_len > 0x7fffffffu)
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: bad arguments", t->num_heads);
+    if (!(t->scale >= 0.0f) || std::isinf(t->scale)) return ctx_fail(SMOE_ERR_ARG, "kv4_attention needs a finite scale >= 0", 0);
     if (t->dtype != SMOE_DTYPE_F32 && t->dtype != SMOE_DTYPE_BF16)
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: q and out are fp32 or bf16", t->dtype);
     if (!aligned(t->q, 16) || !aligned(t->out, 16) || (t->q_row | t->out_row) % 4)
@@ -211,34 +212,35 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     p.a = {*cache, c.err};
     p.t = *t;
     p.group = t->num_heads / cache->num_kv_heads;
-    p.split_pages = plan.split_pages;
-    p.splits = plan.splits;
-    p.part = plan.part_bytes ? static_cast<float*>(t->workspace) : nullptr;
-    p.stat = reinterpret_cast<float2*>(p.part + (p.part ? uint64_t(cache->n_seqs) * t->num_heads * plan.splits * cache->head_dim : 0));
-    p.logits = plan.logit_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(t->workspace) + plan.part_bytes) : nullptr;
-    p.rows = t->max_len;
-    p.gs = plan.gs;
-    p.scale_log2 = t->scale * 1.4426950408889634f;
-    auto run = [&](auto kern, uint32_t smem, uint32_t heads) -> int {
-        p.chunks = (p.group + heads - 1) / heads;
-        if (uint64_t(p.chunks) * cache->num_kv_heads > 65535)
-            return ctx_fail(SMOE_ERR_ARG, "kv4_attention: too many heads", long(t->num_heads));
+    p.chunks = plan.chunks;
+    p.warps = smoe::kKaGrid * smoe::kKaWarps;
+    uint8_t* ws = static_cast<uint8_t*>(t->workspace);
+    p.part = reinterpret_cast<float*>(ws);
+    p.stat = reinterpret_cast<float2*>(ws + plan.part_bytes);
+    p.meta = reinterpret_cast<uint2*>(ws + plan.part_bytes + plan.stat_bytes);
+    p.logits = plan.logit_bytes ? reinterpret_cast<float*>(ws + plan.part_bytes + plan.stat_bytes + plan.meta_bytes) : nullptr;
+    p.rows = plan.rows;
+    // (a scale of 0 must still keep the masked scores' -inf: 1e-35 times any finite score is 0 to the exponential)
+    p.scale_log2 = std::max(t->scale * 1.4426950408889634f, 1e-35f);
+    auto run = [&](auto kern, uint32_t smem) -> int {
         const int r = smem_limit(c, kern, smem);
-        return r ? r : launch(c, kern, dim3(plan.splits, p.chunks * cache->num_kv_heads, cache->n_seqs), dim3(smoe::kKaWarps * 32), smem, p);
+        return r ? r : launch(c, kern, dim3(smoe::kKaGrid), dim3(smoe::kKaWarps * 32), smem, p);
     };
-    const bool wide = p.group > 8, f32 = t->dtype == SMOE_DTYPE_F32;
     using namespace smoe;
-#define SMOE_KV4_ATTN(NG)                                                                                        \
-    (wide ? f32 ? run(k_kv4_attention<NG, 2, 2>, Kv4AttnSmem<NG, 2>::BYTES, 16)                                  \
-                : run(k_kv4_attention<NG, 2, 1>, Kv4AttnSmem<NG, 2>::BYTES, 16)                                  \
-          : f32 ? run(k_kv4_attention<NG, 1, 2>, Kv4AttnSmem<NG, 1>::BYTES, 8)                                   \
-                : run(k_kv4_attention<NG, 1, 1>, Kv4AttnSmem<NG, 1>::BYTES, 8))
-    rc = cache->head_dim == 64 ? SMOE_KV4_ATTN(1) : SMOE_KV4_ATTN(2);
-#undef SMOE_KV4_ATTN
-    if (rc || !p.part) return rc;
-    const uint32_t outs = p.group * cache->head_dim / kKjOuts, entries = p.logits ? (t->max_len + kKjEntries - 1) / kKjEntries : 0u;
+    const bool f32 = t->dtype == SMOE_DTYPE_F32;
+    if (cache->head_dim == 64) rc = f32 ? run(k_kv4_attention<1, 2>, kv4_attn_smem<1>()) : run(k_kv4_attention<1, 1>, kv4_attn_smem<1>());
+    else rc = f32 ? run(k_kv4_attention<2, 2>, kv4_attn_smem<2>()) : run(k_kv4_attention<2, 1>, kv4_attn_smem<2>());
+    if (rc) return rc;
+    // threads an output: about a quarter of the parts that a pair has when all are equally long
+    const uint32_t pages = (t->max_len + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE;
+    const uint64_t pairs = uint64_t(cache->n_seqs) * cache->num_kv_heads * plan.chunks;
+    const uint64_t usual = std::min<uint64_t>(p.warps / pairs + 2, pages);
+    p.lanes = cache->head_dim == 64 ? 2 : 1;                      // (1024 / lanes outputs: within one round of heads)
+    while (p.lanes < 64 && p.lanes * 4 < usual) p.lanes *= 2;
+    const uint32_t per = 4 * kKjThreads / p.lanes, outs = (p.group * cache->head_dim + per - 1) / per;
+    const uint32_t entries = p.logits ? (t->max_len + kKjEntries - 1) / kKjEntries : 0u;
     return launch(c, k_kv4_join, dim3(outs + entries, cache->num_kv_heads, cache->n_seqs), dim3(kKjThreads),
-                  (size_t(p.group) + plan.splits) * 4, p, outs);
+                  size_t(plan.chunks) * kKaHeads * 8, p, outs);
 }
 
 uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len) {
