@@ -1,6 +1,8 @@
 // kv4.cuh - the paged 4-bit KV cache: quantised append, read-back, attention
 // of one query token per sequence, eviction by accumulated attention weight.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "serve.cuh"
 
 namespace smoe {
@@ -800,8 +802,9 @@ struct Kv4Evict {
     uint32_t keep, recent, max_len;
     uint32_t* pos_out;                           // null: in place
     float* score_out;
-    uint32_t* lists;                             // per (sequence, KV head): moved count, then targets, then sources
-    uint32_t cap, stride;                        // moves a pair can have, u32s of one pair's list
+    uint32_t* lists;                             // per (sequence, KV head): targets, then sources
+    uint32_t cap;                                // moves that a pair can have
+    uint32_t cached;                             // keys that a CTA's shared memory holds
 };
 
 // Order of the scores as unsigned integers, NaN lowest; -0 and 0 are equal.
@@ -812,153 +815,243 @@ SMOE_DEVINL uint32_t kv4_rank_key(float x) {
 }
 constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays for its position (above +inf's)
 
-constexpr int kEvThreads = 1024;
+// A cluster of CTAs per (KV head, sequence), each CTA a stretch of the
+// entries, a warp a stretch of those.
+//  1. Keys (a score's order, or kKvLate) into shared memory; the first of
+//     three histograms - 11, 11 and 10 bits of the key - with them.
+//  2. The keep-th largest key: after each histogram every CTA adds up all of
+//     the cluster's and finds the digit; the next one counts the keys that
+//     share the digits so far. Entries above the key stay, and of those
+//     equal to it the lowest.
+//  3. Each warp walks its words of 32 entries (ballots and population counts
+//     give the ranks): first counting, then - with what the warps and CTAs
+//     before it counted - listing free entries below `keep` and kept ones
+//     past it, both ascending.
+//  4. The j-th kept entry goes to the j-th free one: a warp takes 32 moves,
+//     looks up their pages a lane each, and copies eight at a time, 128 bytes
+//     of codes as a word a lane, scales, biases, pos and score by the lanes
+//     after. Sources are past `keep` and targets below it: no move reads what
+//     another writes.
+// Bound by the chain of steps for short sequences and by the moves' bytes for
+// long ones.
+constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvDigits = 3;
+constexpr uint32_t kEvBins = 2048;
+__host__ __device__ constexpr uint32_t kv4_evict_smem(uint32_t cached) { return (kEvDigits * kEvBins + cached) * 4; }
 
-// One CTA per (KV head, sequence). The keep-th largest key comes out of four
-// passes over histograms of its bytes; the entries above it stay, and of
-// those equal to it the lowest. Then each warp walks its own stretch of
-// entries 32 at a time (ballots and population counts give the ranks) and
-// lists free entries below `keep` and kept ones past it, both ascending.
-__global__ void __launch_bounds__(kEvThreads) k_kv4_evict_select(Kv4Evict p) {
+// Exclusive sum over the threads of a CTA of two counts at once; totals in `all`.
+SMOE_DEVINL uint2 ev_scan(uint2 v, uint2* warp_sums, uint32_t warp, uint32_t lane, uint2& all) {
+    uint2 incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+        if (lane >= uint32_t(o)) incl.x += x, incl.y += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    const uint2 w = warp_sums[lane];             // (32 warps)
+    uint2 wi = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, wi.x, o), y = __shfl_up_sync(0xffffffffu, wi.y, o);
+        if (lane >= uint32_t(o)) wi.x += x, wi.y += y;
+    }
+    all = make_uint2(__shfl_sync(0xffffffffu, wi.x, 31), __shfl_sync(0xffffffffu, wi.y, 31));
+    const uint32_t bx = __shfl_sync(0xffffffffu, wi.x - w.x, warp), by = __shfl_sync(0xffffffffu, wi.y - w.y, warp);
+    return make_uint2(bx + incl.x - v.x, by + incl.y - v.y);
+}
+
+__global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint32_t ev_smem[];
+    __shared__ uint2 warp_sums[32], counts[2];
+    __shared__ uint32_t pick[2];
+    cg::cluster_group cluster = cg::this_cluster();
     pdl_release();
-    pdl_acquire();
-    __shared__ uint32_t hist[256], wsum[32], wsum2[32], pick[2];
     const SmoeKv4Cache& c = p.a.c;
-    const uint32_t kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t* list = p.lists + (size_t(s) * c.num_kv_heads + kvh) * p.stride;
+    const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t kvh = blockIdx.x / ctas, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t *hist = ev_smem, *keys = ev_smem + kEvDigits * kEvBins;
+    for (uint32_t i = tid; i < kEvDigits * kEvBins; i += kEvThreads) hist[i] = 0;
+    __syncthreads();
+    pdl_acquire();
+    uint32_t* to_list = p.lists + (size_t(s) * c.num_kv_heads + kvh) * 2 * p.cap;
+    uint32_t* from_list = to_list + p.cap;
     uint32_t n = ld_plain(c.len + s);
     if (n > p.max_len) {
         if (tid == 0) serve_err(p.a.err, SMOE_DEVERR_BAD_RANGE);
         n = p.max_len;
     }
-    if (n <= p.keep) {
-        if (tid == 0) list[0] = 0;
+    const uint32_t seen = ld_plain((c.seen ? c.seen : c.len) + s);
+    // this CTA's entries: whole words of 32
+    const uint32_t words = (n + 31) / 32, wper = (words + ctas - 1) / ctas;
+    const uint32_t e0 = min(n, rank * wper * 32), e1 = min(n, e0 + wper * 32);
+    auto place = [&](uint32_t e) -> size_t {     // index of entry e in pos and score, ~0 when it has none
+        const uint32_t page = kv4_page(c, s, e, p.a.err);
+        return page == ~0u ? ~size_t(0) : (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
+    };
+    if (n <= p.keep) {                           // all stay (the whole cluster returns)
+        if (p.pos_out)
+            for (uint32_t e = e0 + tid; e < e1; e += kEvThreads) {
+                const size_t i = place(e);
+                if (i != ~size_t(0)) p.pos_out[i] = c.pos[i], p.score_out[i] = c.score[i];
+            }
         return;
     }
-    const uint32_t seen = ld_plain((c.seen ? c.seen : c.len) + s);
-    auto key_of = [&](uint32_t e) -> uint32_t {
-        const uint32_t page = kv4_page(c, s, e, p.a.err);
-        if (page == ~0u) return 0u;
-        const size_t i = (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage;
-        return uint64_t(c.pos[i]) + p.recent >= seen ? kKvLate : kv4_rank_key(c.score[i]);
+    auto key_at = [&](size_t i) -> uint32_t {
+        if (i == ~size_t(0)) return 0u;
+        const uint32_t pos = c.pos[i];
+        const float score = c.score[i];
+        return uint64_t(pos) + p.recent >= seen ? kKvLate : kv4_rank_key(score);
     };
-    uint32_t prefix = 0, need = p.keep;          // need: kept entries among those that share the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = tid; i < 256; i += kEvThreads) hist[i] = 0;
-        __syncthreads();
-        for (uint32_t e = tid; e < n; e += kEvThreads) {
-            const uint32_t k = key_of(e);
-            if (shift == 24 || (k ^ prefix) >> (shift + 8) == 0) atomicAdd(&hist[k >> shift & 255u], 1u);
+    auto key_of = [&](uint32_t e) -> uint32_t { return e - e0 < p.cached ? keys[e - e0] : key_at(place(e)); };
+
+    uint32_t prefix = 0, need = p.keep;          // need: kept entries among those that share the digits so far
+#pragma unroll
+    for (int d = 0; d < kEvDigits; ++d) {
+        constexpr int kShift[kEvDigits] = {21, 10, 0};
+        const int shift = kShift[d], up = d == 0 ? 32 : kShift[d > 0 ? d - 1 : 0];
+        const uint32_t mask = d == 2 ? 1023u : 2047u;
+        uint32_t* h = hist + d * kEvBins;
+        if (d == 0) {                            // four entries a thread and round: they share a page
+            for (uint32_t e = e0 + tid * 4; e < e1; e += 4 * kEvThreads) {
+                const size_t i = place(e);
+                uint32_t k[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) k[q] = e + q < e1 ? key_at(i == ~size_t(0) ? i : i + q) : 0u;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (e + q < e1) {
+                        if (e + q - e0 < p.cached) keys[e + q - e0] = k[q];
+                        atomicAdd(h + (k[q] >> shift), 1u);
+                    }
+            }
+        } else {
+            for (uint32_t e = e0 + tid; e < e1; e += kEvThreads) {
+                const uint32_t k = key_of(e);
+                if ((k ^ prefix) >> up == 0) atomicAdd(h + (k >> shift & mask), 1u);
+            }
         }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t left = need, b = 255;
-            while (b && hist[b] < left) left -= hist[b--];
-            pick[0] = b;
-            pick[1] = left;
+        cluster.sync();
+        // bins from the top, two a thread: where the sum passes `need`
+        uint2 mine = make_uint2(0u, 0u);
+        const uint32_t b = kEvBins - 2 - 2 * tid;                // this thread's bins b + 1, b
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(h, r) + b);
+            mine.x += v.x;
+            mine.y += v.y;
+        }
+        uint2 all;
+        const uint32_t above = ev_scan(make_uint2(mine.x + mine.y, 0u), warp_sums, warp, lane, all).x;
+        if (above < need && above + mine.x + mine.y >= need) {
+            const bool upper = above + mine.y >= need;
+            pick[0] = upper ? b + 1 : b;
+            pick[1] = need - above - (upper ? 0u : mine.y);
         }
         __syncthreads();
         prefix |= pick[0] << shift;
         need = pick[1];
-        __syncthreads();
     }
-    // the warp's stretch of entries, whole words of 32
-    const uint32_t words = (n + 31) / 32, per = (words + 31) / 32, w0 = min(words, warp * per), w1 = min(words, w0 + per);
+    // the warp's words of the CTA's
+    const uint32_t cw = (e1 - e0 + 31) / 32, per = (cw + kEvWarps - 1) / kEvWarps, w0 = min(cw, warp * per), w1 = min(cw, w0 + per);
+    const uint32_t low = (1u << lane) - 1u;
     uint32_t equal = 0;
     for (uint32_t w = w0; w < w1; ++w) {
-        const uint32_t e = w * 32 + lane;
-        equal += __popc(__ballot_sync(0xffffffffu, e < n && key_of(e) == prefix));
+        const uint32_t e = e0 + w * 32 + lane;
+        equal += __popc(__ballot_sync(0xffffffffu, e < e1 && key_of(e) == prefix));
     }
-    if (lane == 0) wsum[warp] = equal;
-    __syncthreads();
-    uint32_t before = 0;
-    for (uint32_t i = 0; i < warp; ++i) before += wsum[i];
-    __syncthreads();
-    for (int pass = 0; pass < 2; ++pass) {       // 0: counts of the stretch, 1: the lists
-        uint32_t eq = before, nfree = 0, nfar = 0, free0 = 0, far0 = 0;
-        if (pass) {
-            for (uint32_t i = 0; i < warp; ++i) {
-                free0 += wsum[i];
-                far0 += wsum2[i];
-            }
-            if (tid == 0) {
-                uint32_t all = 0;
-                for (uint32_t i = 0; i < 32; ++i) all += wsum2[i];
-                list[0] = min(all, p.cap);
-            }
-        }
+    uint2 all;
+    uint32_t eq0 = ev_scan(make_uint2(lane == 0 ? equal : 0u, 0u), warp_sums, warp, lane, all).x;
+    eq0 = __shfl_sync(0xffffffffu, eq0, 0);
+    if (tid == 0) counts[0] = all;
+    cluster.sync();
+    for (uint32_t r = 0; r < rank; ++r) eq0 += cluster.map_shared_rank(counts, r)[0].x;
+    uint2 first = make_uint2(0u, 0u);            // free and far entries before this warp's
+    uint32_t moves = 0;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {       // counts, then lists
+        uint32_t eq = eq0, nfree = 0, nfar = 0;
         for (uint32_t w = w0; w < w1; ++w) {
-            const uint32_t e = w * 32 + lane, k = e < n ? key_of(e) : 0u;
-            const uint32_t eqs = __ballot_sync(0xffffffffu, e < n && k == prefix), low = (1u << lane) - 1u;
-            const bool stays = e < n && (k > prefix || (k == prefix && eq + __popc(eqs & low) < need));
+            const uint32_t e = e0 + w * 32 + lane, k = e < e1 ? key_of(e) : 0u;
+            const uint32_t eqs = __ballot_sync(0xffffffffu, e < e1 && k == prefix);
+            const bool stays = e < e1 && (k > prefix || (k == prefix && eq + __popc(eqs & low) < need));
             eq += __popc(eqs);
-            const bool is_free = e < n && e < p.keep && !stays, is_far = stays && e >= p.keep;
+            const bool is_free = e < e1 && e < p.keep && !stays, is_far = stays && e >= p.keep;
             const uint32_t frees = __ballot_sync(0xffffffffu, is_free), fars = __ballot_sync(0xffffffffu, is_far);
             if (pass) {
-                const uint32_t i = free0 + nfree + __popc(frees & low), j = far0 + nfar + __popc(fars & low);
-                if (is_free && i < p.cap) list[1 + i] = e;
-                if (is_far && j < p.cap) list[1 + p.cap + j] = e;
+                const uint32_t i = first.x + nfree + __popc(frees & low), j = first.y + nfar + __popc(fars & low);
+                if (is_free && i < p.cap) to_list[i] = e;
+                if (is_far && j < p.cap) from_list[j] = e;
+                if (p.pos_out && stays && e < p.keep) {
+                    const size_t at = place(e);
+                    if (at != ~size_t(0)) p.pos_out[at] = c.pos[at], p.score_out[at] = c.score[at];
+                }
             }
             nfree += __popc(frees);
             nfar += __popc(fars);
         }
-        if (!pass) {
-            if (lane == 0) {
-                wsum[warp] = nfree;
-                wsum2[warp] = nfar;
+        if (pass == 0) {
+            first = ev_scan(lane == 0 ? make_uint2(nfree, nfar) : make_uint2(0u, 0u), warp_sums, warp, lane, all);
+            first.x = __shfl_sync(0xffffffffu, first.x, 0);
+            first.y = __shfl_sync(0xffffffffu, first.y, 0);
+            if (tid == 0) counts[1] = all;
+            cluster.sync();
+            for (uint32_t r = 0; r < ctas; ++r) {
+                const uint2 v = cluster.map_shared_rank(counts, r)[1];
+                if (r < rank) first.x += v.x, first.y += v.y;
+                moves += v.y;
             }
-            __syncthreads();
+            moves = min(moves, p.cap);
         }
     }
-}
+    cluster.sync();                              // the lists are written (and no CTA reads another's memory after this)
 
-// The moves of a (KV head, sequence): one warp a pair, 128 bytes of codes as
-// one word a lane (head_dim 128), scales and biases, pos and score by the
-// lanes after. Sources are past `keep` and targets below it, so no move reads
-// what another writes. With separate outputs, pos and score of every entry
-// below min(len, keep) are written: first all, then the moved ones by the
-// warps that move them - of an entry only one of the two.
-__global__ void __launch_bounds__(256) k_kv4_evict_move(Kv4Evict p) {
-    pdl_release();
-    pdl_acquire();
-    const SmoeKv4Cache& c = p.a.c;
     const Kv4Geom G(c.head_dim);
-    const uint32_t kvh = blockIdx.y, s = blockIdx.z, lane = threadIdx.x & 31;
-    const uint32_t* list = p.lists + (size_t(s) * c.num_kv_heads + kvh) * p.stride;
-    const uint32_t moves = list[0], warps = gridDim.x * 8;
-    auto index = [&](uint32_t e, uint32_t page) { return (size_t(page) * c.num_kv_heads + kvh) * kKvPage + e % kKvPage; };
     float* score_out = p.score_out ? p.score_out : c.score;
     uint32_t* pos_out = p.pos_out ? p.pos_out : c.pos;
-    for (uint32_t m = blockIdx.x * 8 + (threadIdx.x >> 5); m < moves; m += warps) {
-        const uint32_t to = list[1 + m], from = list[1 + p.cap + m];
-        const uint32_t pt = kv4_page(c, s, to, p.a.err), pf = kv4_page(c, s, from, p.a.err);
-        if (pt == ~0u || pf == ~0u) continue;
-        uint8_t* bt = c.blocks + (size_t(pt) * c.num_kv_heads + kvh) * G.block;
-        const uint8_t* bf = c.blocks + (size_t(pf) * c.num_kv_heads + kvh) * G.block;
-        const uint32_t st = to % kKvPage, sf = from % kKvPage;
-        if (lane < G.ng * 16)                    // plane lane / 8, word lane % 8 of its 32 bytes
-            *reinterpret_cast<uint32_t*>(bt + lane / 8 * kKvPlane + st * 32 + lane % 8 * 4) =
-                *reinterpret_cast<const uint32_t*>(bf + lane / 8 * kKvPlane + sf * 32 + lane % 8 * 4);
-        if (lane < G.ng * 2)
-            *reinterpret_cast<uint32_t*>(bt + G.sb(0, 0) + lane * kKvPage * 4 + st * 4) =
-                *reinterpret_cast<const uint32_t*>(bf + G.sb(0, 0) + lane * kKvPage * 4 + sf * 4);
-        if (lane == 8) pos_out[index(to, pt)] = c.pos[index(from, pf)];
-        if (lane == 9) score_out[index(to, pt)] = c.score[index(from, pf)];
-    }
-    if (!p.pos_out) return;
-    uint32_t n = min(ld_plain(c.len + s), min(p.max_len, p.keep));
-    for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
-        uint32_t lo = 0, hi = moves;             // is e a target? (targets ascend)
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (list[1 + mid] < e) lo = mid + 1;
-            else hi = mid;
+    const bool codes = lane < G.ng * 16;         // plane lane / 8, word lane % 8 of its 32 bytes
+    // lanes after: G.ng * 2 (scale, bias) words, pos, score - lane 31 - x
+    const uint32_t x = 31 - lane;
+    for (uint32_t m0 = (rank * kEvWarps + warp) * 32; m0 < moves; m0 += ctas * kEvWarps * 32) {
+        uint32_t tp = ~0u, fp = ~0u, te = 0, fe = 0;
+        if (m0 + lane < moves) {
+            te = to_list[m0 + lane];
+            fe = from_list[m0 + lane];
+            tp = kv4_page(c, s, te, p.a.err);
+            fp = kv4_page(c, s, fe, p.a.err);
         }
-        if (lo < moves && list[1 + lo] == e) continue;
-        const uint32_t page = kv4_page(c, s, e, p.a.err);
-        if (page == ~0u) continue;
-        pos_out[index(e, page)] = c.pos[index(e, page)];
-        score_out[index(e, page)] = c.score[index(e, page)];
+        const uint32_t have = min(32u, moves - m0);
+        for (uint32_t q0 = 0; q0 < have; q0 += 8) {
+            uint32_t code[8], rest[8];
+            size_t at_t[8], at_f[8];             // page and KV head of target and source, ~0: none
+            uint32_t st[8], sf[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int from = min(int(q0) + q, 31);
+                const uint32_t pt = __shfl_sync(0xffffffffu, tp, from), pf = __shfl_sync(0xffffffffu, fp, from);
+                st[q] = __shfl_sync(0xffffffffu, te, from) % kKvPage;
+                sf[q] = __shfl_sync(0xffffffffu, fe, from) % kKvPage;
+                const bool ok = q0 + q < have && pt != ~0u && pf != ~0u;
+                at_t[q] = ok ? size_t(pt) * c.num_kv_heads + kvh : ~size_t(0);
+                at_f[q] = ok ? size_t(pf) * c.num_kv_heads + kvh : ~size_t(0);
+                code[q] = rest[q] = 0u;
+                if (!ok) continue;
+                const uint8_t* blk = c.blocks + at_f[q] * G.block;
+                if (codes) code[q] = *reinterpret_cast<const uint32_t*>(blk + lane / 8 * kKvPlane + sf[q] * 32 + lane % 8 * 4);
+                if (x < G.ng * 2) rest[q] = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, 0) + x * kKvPage * 4 + sf[q] * 4);
+                else if (x == G.ng * 2) rest[q] = c.pos[at_f[q] * kKvPage + sf[q]];
+                else if (x == G.ng * 2 + 1) rest[q] = __float_as_uint(c.score[at_f[q] * kKvPage + sf[q]]);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (at_t[q] == ~size_t(0)) continue;
+                uint8_t* blk = c.blocks + at_t[q] * G.block;
+                if (codes) *reinterpret_cast<uint32_t*>(blk + lane / 8 * kKvPlane + st[q] * 32 + lane % 8 * 4) = code[q];
+                if (x < G.ng * 2) *reinterpret_cast<uint32_t*>(blk + G.sb(0, 0) + x * kKvPage * 4 + st[q] * 4) = rest[q];
+                else if (x == G.ng * 2) pos_out[at_t[q] * kKvPage + st[q]] = rest[q];
+                else if (x == G.ng * 2 + 1) score_out[at_t[q] * kKvPage + st[q]] = __uint_as_float(rest[q]);
+            }
+        }
     }
 }
 

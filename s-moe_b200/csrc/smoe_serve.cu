@@ -19,21 +19,28 @@ using smoe::CtxView;
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 template <typename... KArgs, typename... Args>
-int launch(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+int launch_cluster(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, uint32_t cluster, Args... args) {
     cudaLaunchConfig_t lc{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     lc.gridDim = grid;
     lc.blockDim = block;
     lc.dynamicSmemBytes = smem;
     lc.stream = c.stream;
     lc.attrs = at;
-    lc.numAttrs = 1;
+    lc.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&lc, kern, KArgs(args)...);
     if (e != cudaSuccess) return ctx_fail(SMOE_ERR_CUDA, cudaGetErrorString(e), long(e));
     *c.dispatches += 1;
     return SMOE_OK;
+}
+template <typename... KArgs, typename... Args>
+int launch(const CtxView& c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+    return launch_cluster(c, kern, grid, block, smem, 1u, args...);
 }
 
 // Raise a kernel's shared-memory limit once per (kernel, device); a call
@@ -245,7 +252,7 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
 
 uint64_t smoe_cuda_kv4_evict_workspace(const SmoeKv4Cache* cache, uint32_t max_len) {
     // a pair moves at most min(keep, len - keep) <= len / 2 entries
-    return cache ? uint64_t(cache->n_seqs) * cache->num_kv_heads * (uint64_t(max_len / 2) * 2 + 4) * 4 : 0;
+    return cache ? uint64_t(cache->n_seqs) * cache->num_kv_heads * (uint64_t(max_len / 2) * 2 + 2) * 4 : 0;
 }
 
 int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t keep, uint32_t recent, uint32_t max_len,
@@ -263,13 +270,16 @@ int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t ke
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return ctx_fail(SMOE_ERR_ARG, "kv4_evict: workspace missing, too small or unaligned; bytes needed", long(need));
     const CtxView c = smoe::ctx_view(ctx);
-    const uint32_t cap = max_len / 2;
-    smoe::Kv4Evict p{{*cache, c.err}, keep, recent, max_len, pos_out, score_out, static_cast<uint32_t*>(workspace), cap, cap * 2 + 4};
-    const dim3 pairs(cache->num_kv_heads, cache->n_seqs);
-    if ((rc = launch(c, smoe::k_kv4_evict_select, pairs, dim3(smoe::kEvThreads), 0, p))) return rc;
-    const uint32_t work = std::max(std::min(keep, max_len) / 256u, 1u), pairs_n = pairs.x * pairs.y;
-    const uint32_t split = std::max(1u, std::min(work, uint32_t(c.num_sms) * 8u / pairs_n));
-    return launch(c, smoe::k_kv4_evict_move, dim3(split, pairs.x, pairs.y), dim3(256), 0, p);
+    // CTAs of a pair: 8192 entries each, 8 at most; past what their shared memory holds keys are read again each time
+    uint32_t ctas = 1;
+    while (ctas < 8 && uint64_t(ctas) * 8192 < max_len) ctas *= 2;
+    const uint32_t cached = std::min<uint32_t>(49152, (max_len / ctas + 64 + 31) / 32 * 32);
+    if (uint64_t(cache->num_kv_heads) * ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_ARG, "kv4_evict: too many KV heads", cache->num_kv_heads);
+    if ((rc = smem_limit(c, smoe::k_kv4_evict, smoe::kv4_evict_smem(49152)))) return rc;
+    smoe::Kv4Evict p{{*cache, c.err}, keep, recent, max_len, pos_out, score_out, static_cast<uint32_t*>(workspace),
+                     std::max(1u, max_len / 2), cached};
+    return launch_cluster(c, smoe::k_kv4_evict, dim3(cache->num_kv_heads * ctas, cache->n_seqs), dim3(smoe::kEvThreads),
+                          smoe::kv4_evict_smem(cached), ctas, p);
 }
 
 int smoe_cuda_kv4_advance(SmoeCudaCtx* ctx, uint32_t* len, uint32_t* seen, uint32_t n_seqs, const uint32_t* cu,
