@@ -529,7 +529,8 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
  * different sequences are distinct. len (entries held before this step),
  * seen (tokens ever appended) and table are shared by all layers and change
  * once a step (smoe_cuda_kv4_advance). pos and score are per layer, paged
- * like the blocks, and only needed for eviction. head_dim 64 or 128. */
+ * like the blocks, 16-byte aligned, and only needed for eviction. head_dim 64
+ * or 128. */
 #define SMOE_KV4_PAGE 64
 typedef struct SmoeKv4Cache {
     uint8_t*        blocks;       /* [n_pages][num_kv_heads][block bytes], 16-byte aligned */

@@ -829,9 +829,10 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     past it, both ascending.
 //  4. The j-th kept entry goes to the j-th free one: a warp takes 32 moves,
 //     looks up their pages a lane each, and copies eight at a time, 128 bytes
-//     of codes as a word a lane, scales, biases, pos and score by the lanes
-//     after. Sources are past `keep` and targets below it: no move reads what
-//     another writes.
+//     of codes as a word a lane, scales, biases, pos and score another.
+//     Sources are past `keep` and targets below it: no move reads what
+//     another writes. (Separate outputs have pos and score of all entries
+//     below `keep` from step 1, before the moved ones' overwrite them.)
 // Bound by the chain of steps for short sequences and by the moves' bytes for
 // long ones.
 constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvDigits = 3;
@@ -898,13 +899,12 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
             }
         return;
     }
-    auto key_at = [&](size_t i) -> uint32_t {
-        if (i == ~size_t(0)) return 0u;
-        const uint32_t pos = c.pos[i];
-        const float score = c.score[i];
-        return uint64_t(pos) + p.recent >= seen ? kKvLate : kv4_rank_key(score);
+    auto key = [&](uint32_t pos, float score) { return uint64_t(pos) + p.recent >= seen ? kKvLate : kv4_rank_key(score); };
+    auto key_of = [&](uint32_t e) -> uint32_t {
+        if (e - e0 < p.cached) return keys[e - e0];
+        const size_t i = place(e);
+        return i == ~size_t(0) ? 0u : key(c.pos[i], c.score[i]);
     };
-    auto key_of = [&](uint32_t e) -> uint32_t { return e - e0 < p.cached ? keys[e - e0] : key_at(place(e)); };
 
     uint32_t prefix = 0, need = p.keep;          // need: kept entries among those that share the digits so far
 #pragma unroll
@@ -913,18 +913,47 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
         const int shift = kShift[d], up = d == 0 ? 32 : kShift[d > 0 ? d - 1 : 0];
         const uint32_t mask = d == 2 ? 1023u : 2047u;
         uint32_t* h = hist + d * kEvBins;
-        if (d == 0) {                            // four entries a thread and round: they share a page
-            for (uint32_t e = e0 + tid * 4; e < e1; e += 4 * kEvThreads) {
-                const size_t i = place(e);
-                uint32_t k[4];
+        if (d == 0) {                            // four entries a thread at a time - they share a page - and two such at once
+            for (uint32_t eb = e0 + tid * 4; eb < e1; eb += 8 * kEvThreads) {
+                size_t at[2];
+                uint4 ps[2];
+                float4 sc[2];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) k[q] = e + q < e1 ? key_at(i == ~size_t(0) ? i : i + q) : 0u;
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t e = eb + u * 4 * kEvThreads;
+                    at[u] = e < e1 ? place(e) : ~size_t(0);
+                }
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (e + q < e1) {
-                        if (e + q - e0 < p.cached) keys[e + q - e0] = k[q];
-                        atomicAdd(h + (k[q] >> shift), 1u);
+                for (int u = 0; u < 2; ++u)
+                    if (at[u] != ~size_t(0)) {   // (whole quads: past the last entry the page goes on)
+                        ps[u] = *reinterpret_cast<const uint4*>(c.pos + at[u]);
+                        sc[u] = *reinterpret_cast<const float4*>(c.score + at[u]);
                     }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t e = eb + u * 4 * kEvThreads, m = e < e1 ? min(4u, e1 - e) : 0u;
+                    const bool ok = at[u] != ~size_t(0);
+                    const uint32_t k[4] = {ok ? key(ps[u].x, sc[u].x) : 0u, ok ? key(ps[u].y, sc[u].y) : 0u,
+                                           ok ? key(ps[u].z, sc[u].z) : 0u, ok ? key(ps[u].w, sc[u].w) : 0u};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (q < m) {
+                            if (e + q - e0 < p.cached) keys[e + q - e0] = k[q];
+                            atomicAdd(h + (k[q] >> shift), 1u);
+                        }
+                    if (p.pos_out && ok && e < p.keep) {
+                        if (e + 4 <= p.keep) {   // (n > keep: the whole quad is there)
+                            *reinterpret_cast<uint4*>(p.pos_out + at[u]) = ps[u];
+                            *reinterpret_cast<float4*>(p.score_out + at[u]) = sc[u];
+                        } else {
+                            const uint32_t pq[3] = {ps[u].x, ps[u].y, ps[u].z};
+                            const float sq[3] = {sc[u].x, sc[u].y, sc[u].z};
+#pragma unroll
+                            for (int q = 0; q < 3; ++q)
+                                if (e + q < p.keep) p.pos_out[at[u] + q] = pq[q], p.score_out[at[u] + q] = sq[q];
+                        }
+                    }
+                }
             }
         } else {
             for (uint32_t e = e0 + tid; e < e1; e += kEvThreads) {
@@ -982,10 +1011,6 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
                 const uint32_t i = first.x + nfree + __popc(frees & low), j = first.y + nfar + __popc(fars & low);
                 if (is_free && i < p.cap) to_list[i] = e;
                 if (is_far && j < p.cap) from_list[j] = e;
-                if (p.pos_out && stays && e < p.keep) {
-                    const size_t at = place(e);
-                    if (at != ~size_t(0)) p.pos_out[at] = c.pos[at], p.score_out[at] = c.score[at];
-                }
             }
             nfree += __popc(frees);
             nfar += __popc(fars);
@@ -1006,50 +1031,49 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
     }
     cluster.sync();                              // the lists are written (and no CTA reads another's memory after this)
 
+    // What a lane copies of a move, at base + (page and KV head) * step + slot * width: a word of codes (plane lane / 8,
+    // word lane % 8 of its 32 bytes), and from lane 31 downwards the scale and bias pairs, pos and score.
     const Kv4Geom G(c.head_dim);
-    float* score_out = p.score_out ? p.score_out : c.score;
-    uint32_t* pos_out = p.pos_out ? p.pos_out : c.pos;
-    const bool codes = lane < G.ng * 16;         // plane lane / 8, word lane % 8 of its 32 bytes
-    // lanes after: G.ng * 2 (scale, bias) words, pos, score - lane 31 - x
     const uint32_t x = 31 - lane;
+    const bool codes = lane < G.ng * 16, rest = x < G.ng * 2 + 2;
+    uint8_t* const code_base = c.blocks + lane / 8 * kKvPlane + lane % 8 * 4;
+    const uint32_t step = x < G.ng * 2 ? G.block : kKvPage * 4;
+    const uint8_t* rest_from = x < G.ng * 2 ? c.blocks + G.sb(0, 0) + x * kKvPage * 4
+                               : x == G.ng * 2 ? reinterpret_cast<const uint8_t*>(c.pos) : reinterpret_cast<const uint8_t*>(c.score);
+    uint8_t* rest_to = x < G.ng * 2 ? c.blocks + G.sb(0, 0) + x * kKvPage * 4
+                       : x == G.ng * 2 ? reinterpret_cast<uint8_t*>(p.pos_out ? p.pos_out : c.pos)
+                                       : reinterpret_cast<uint8_t*>(p.score_out ? p.score_out : c.score);
     for (uint32_t m0 = (rank * kEvWarps + warp) * 32; m0 < moves; m0 += ctas * kEvWarps * 32) {
-        uint32_t tp = ~0u, fp = ~0u, te = 0, fe = 0;
-        if (m0 + lane < moves) {
+        uint32_t te = 0, fe = 0, tb = 0, fb = 0;
+        bool ok = m0 + lane < moves;
+        if (ok) {
             te = to_list[m0 + lane];
             fe = from_list[m0 + lane];
-            tp = kv4_page(c, s, te, p.a.err);
-            fp = kv4_page(c, s, fe, p.a.err);
+            const uint32_t tp = kv4_page(c, s, te, p.a.err), fp = kv4_page(c, s, fe, p.a.err);
+            ok = tp != ~0u && fp != ~0u;
+            tb = tp;
+            fb = fp;
         }
-        const uint32_t have = min(32u, moves - m0);
-        for (uint32_t q0 = 0; q0 < have; q0 += 8) {
-            uint32_t code[8], rest[8];
-            size_t at_t[8], at_f[8];             // page and KV head of target and source, ~0: none
-            uint32_t st[8], sf[8];
+        const uint32_t oks = __ballot_sync(0xffffffffu, ok);
+#pragma unroll 1
+        for (uint32_t q0 = 0; q0 < 32 && oks >> q0; q0 += 8) {
+            uint32_t code[8], word[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                const int from = min(int(q0) + q, 31);
-                const uint32_t pt = __shfl_sync(0xffffffffu, tp, from), pf = __shfl_sync(0xffffffffu, fp, from);
-                st[q] = __shfl_sync(0xffffffffu, te, from) % kKvPage;
-                sf[q] = __shfl_sync(0xffffffffu, fe, from) % kKvPage;
-                const bool ok = q0 + q < have && pt != ~0u && pf != ~0u;
-                at_t[q] = ok ? size_t(pt) * c.num_kv_heads + kvh : ~size_t(0);
-                at_f[q] = ok ? size_t(pf) * c.num_kv_heads + kvh : ~size_t(0);
-                code[q] = rest[q] = 0u;
-                if (!ok) continue;
-                const uint8_t* blk = c.blocks + at_f[q] * G.block;
-                if (codes) code[q] = *reinterpret_cast<const uint32_t*>(blk + lane / 8 * kKvPlane + sf[q] * 32 + lane % 8 * 4);
-                if (x < G.ng * 2) rest[q] = *reinterpret_cast<const uint32_t*>(blk + G.sb(0, 0) + x * kKvPage * 4 + sf[q] * 4);
-                else if (x == G.ng * 2) rest[q] = c.pos[at_f[q] * kKvPage + sf[q]];
-                else if (x == G.ng * 2 + 1) rest[q] = __float_as_uint(c.score[at_f[q] * kKvPage + sf[q]]);
+                const uint32_t e = __shfl_sync(0xffffffffu, fe, q0 + q), page = __shfl_sync(0xffffffffu, fb, q0 + q);
+                const bool has = oks >> (q0 + q) & 1u;
+                const size_t at = size_t(page) * c.num_kv_heads + kvh;
+                code[q] = word[q] = 0u;
+                if (has && codes) code[q] = *reinterpret_cast<const uint32_t*>(code_base + at * G.block + e % kKvPage * 32);
+                if (has && rest) word[q] = *reinterpret_cast<const uint32_t*>(rest_from + at * step + e % kKvPage * 4);
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                if (at_t[q] == ~size_t(0)) continue;
-                uint8_t* blk = c.blocks + at_t[q] * G.block;
-                if (codes) *reinterpret_cast<uint32_t*>(blk + lane / 8 * kKvPlane + st[q] * 32 + lane % 8 * 4) = code[q];
-                if (x < G.ng * 2) *reinterpret_cast<uint32_t*>(blk + G.sb(0, 0) + x * kKvPage * 4 + st[q] * 4) = rest[q];
-                else if (x == G.ng * 2) pos_out[at_t[q] * kKvPage + st[q]] = rest[q];
-                else if (x == G.ng * 2 + 1) score_out[at_t[q] * kKvPage + st[q]] = __uint_as_float(rest[q]);
+                const uint32_t e = __shfl_sync(0xffffffffu, te, q0 + q), page = __shfl_sync(0xffffffffu, tb, q0 + q);
+                const bool has = oks >> (q0 + q) & 1u;
+                const size_t at = size_t(page) * c.num_kv_heads + kvh;
+                if (has && codes) *reinterpret_cast<uint32_t*>(code_base + at * G.block + e % kKvPage * 32) = code[q];
+                if (has && rest) *reinterpret_cast<uint32_t*>(rest_to + at * step + e % kKvPage * 4) = word[q];
             }
         }
     }

@@ -93,7 +93,8 @@ int check_cache(const SmoeKv4Cache* c, const char* what) {
         return ctx_fail(SMOE_ERR_ARG, what, 0);
     if (!smoe_cuda_kv4_block_bytes(c->head_dim))
         return ctx_fail(SMOE_ERR_UNSUPPORTED, "the 4-bit cache takes head_dim 64 or 128", c->head_dim);
-    if (!aligned(c->blocks, 16)) return ctx_fail(SMOE_ERR_ARG, "cache blocks must be 16-byte aligned", 0);
+    if (!aligned(c->blocks, 16) || !aligned(c->pos, 16) || !aligned(c->score, 16))
+        return ctx_fail(SMOE_ERR_ARG, "cache blocks, pos and score must be 16-byte aligned", 0);
     if (c->n_seqs > 65535 || c->num_kv_heads > 65535)
         return ctx_fail(SMOE_ERR_ARG, "at most 65535 sequences and KV heads", c->n_seqs);
     return SMOE_OK;
@@ -266,6 +267,8 @@ int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t ke
         // one of the two alone, or the cache's own array: in place is asked for with NULL
         return ctx_fail(SMOE_ERR_ARG, "kv4_evict: pos_out and score_out are both NULL or both separate arrays", 0);
     }
+    if (!aligned(pos_out, 16) || !aligned(score_out, 16))
+        return ctx_fail(SMOE_ERR_ARG, "kv4_evict: pos_out and score_out must be 16-byte aligned", 0);
     const uint64_t need = smoe_cuda_kv4_evict_workspace(cache, max_len);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return ctx_fail(SMOE_ERR_ARG, "kv4_evict: workspace missing, too small or unaligned; bytes needed", long(need));
