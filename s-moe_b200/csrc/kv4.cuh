@@ -823,10 +823,10 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     the cluster's and finds the digit; the next one counts the keys that
 //     share the digits so far. Entries above the key stay, and of those
 //     equal to it the lowest.
-//  3. Each warp walks its words of 32 entries (ballots and population counts
-//     give the ranks): first counting, then - with what the warps and CTAs
-//     before it counted - listing free entries below `keep` and kept ones
-//     past it, both ascending.
+//  3. Each warp turns its words of 32 entries into masks of those that stay
+//     (a ballot each, lane i keeps the i-th), counts free entries below `keep`
+//     and kept ones past it, and - with what the warps and CTAs before it
+//     counted - lists both, ascending.
 //  4. The j-th kept entry goes to the j-th free one: a warp takes 32 moves,
 //     looks up their pages a lane each, and copies eight at a time, 128 bytes
 //     of codes as a word a lane, scales, biases, pos and score another.
@@ -835,7 +835,7 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     below `keep` from step 1, before the moved ones' overwrite them.)
 // Bound by the chain of steps for short sequences and by the moves' bytes for
 // long ones.
-constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvDigits = 3;
+constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvDigits = 3;
 constexpr uint32_t kEvBins = 2048;
 __host__ __device__ constexpr uint32_t kv4_evict_smem(uint32_t cached) { return (kEvDigits * kEvBins + cached) * 4; }
 
@@ -850,7 +850,7 @@ SMOE_DEVINL uint2 ev_scan(uint2 v, uint2* warp_sums, uint32_t warp, uint32_t lan
     __syncthreads();
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    const uint2 w = warp_sums[lane];             // (32 warps)
+    const uint2 w = lane < uint32_t(kEvWarps) ? warp_sums[lane] : make_uint2(0u, 0u);
     uint2 wi = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t ev_smem[];
     __shared__ uint2 warp_sums[32], counts[2];
-    __shared__ uint32_t pick[2];
+    __shared__ uint32_t pick[3];
     cg::cluster_group cluster = cg::this_cluster();
     pdl_release();
     const SmoeKv4Cache& c = p.a.c;
@@ -962,20 +962,27 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
             }
         }
         cluster.sync();
-        // bins from the top, two a thread: where the sum passes `need`
-        uint2 mine = make_uint2(0u, 0u);
-        const uint32_t b = kEvBins - 2 - 2 * tid;                // this thread's bins b + 1, b
+        // bins from the top, four a thread: where the sum passes `need`
+        uint32_t mine[4] = {0u, 0u, 0u, 0u};
+        const uint32_t b = kEvBins - 4 - 4 * tid;
+        static_assert(kEvBins == 4 * kEvThreads, "four bins a thread");
         for (uint32_t r = 0; r < ctas; ++r) {
-            const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(h, r) + b);
-            mine.x += v.x;
-            mine.y += v.y;
+            const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(h, r) + b);
+            mine[0] += v.x;
+            mine[1] += v.y;
+            mine[2] += v.z;
+            mine[3] += v.w;
         }
         uint2 all;
-        const uint32_t above = ev_scan(make_uint2(mine.x + mine.y, 0u), warp_sums, warp, lane, all).x;
-        if (above < need && above + mine.x + mine.y >= need) {
-            const bool upper = above + mine.y >= need;
-            pick[0] = upper ? b + 1 : b;
-            pick[1] = need - above - (upper ? 0u : mine.y);
+        uint32_t above = ev_scan(make_uint2(mine[0] + mine[1] + mine[2] + mine[3], 0u), warp_sums, warp, lane, all).x;
+#pragma unroll
+        for (int q = 3; q >= 0; --q) {
+            if (above < need && above + mine[q] >= need) {
+                pick[0] = b + q;
+                pick[1] = need - above;
+                pick[2] = mine[q];
+            }
+            above += mine[q];
         }
         __syncthreads();
         prefix |= pick[0] << shift;
@@ -984,49 +991,92 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
     // the warp's words of the CTA's
     const uint32_t cw = (e1 - e0 + 31) / 32, per = (cw + kEvWarps - 1) / kEvWarps, w0 = min(cw, warp * per), w1 = min(cw, w0 + per);
     const uint32_t low = (1u << lane) - 1u;
-    uint32_t equal = 0;
-    for (uint32_t w = w0; w < w1; ++w) {
-        const uint32_t e = e0 + w * 32 + lane;
-        equal += __popc(__ballot_sync(0xffffffffu, e < e1 && key_of(e) == prefix));
-    }
     uint2 all;
-    uint32_t eq0 = ev_scan(make_uint2(lane == 0 ? equal : 0u, 0u), warp_sums, warp, lane, all).x;
-    eq0 = __shfl_sync(0xffffffffu, eq0, 0);
-    if (tid == 0) counts[0] = all;
-    cluster.sync();
-    for (uint32_t r = 0; r < rank; ++r) eq0 += cluster.map_shared_rank(counts, r)[0].x;
-    uint2 first = make_uint2(0u, 0u);            // free and far entries before this warp's
-    uint32_t moves = 0;
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {       // counts, then lists
-        uint32_t eq = eq0, nfree = 0, nfar = 0;
+    uint32_t eq0 = 0;                            // entries with the key before this warp's
+    const bool some = pick[2] > need;            // not all entries with the key stay
+    if (some) {
+        uint32_t equal = 0;
         for (uint32_t w = w0; w < w1; ++w) {
-            const uint32_t e = e0 + w * 32 + lane, k = e < e1 ? key_of(e) : 0u;
-            const uint32_t eqs = __ballot_sync(0xffffffffu, e < e1 && k == prefix);
-            const bool stays = e < e1 && (k > prefix || (k == prefix && eq + __popc(eqs & low) < need));
-            eq += __popc(eqs);
-            const bool is_free = e < e1 && e < p.keep && !stays, is_far = stays && e >= p.keep;
-            const uint32_t frees = __ballot_sync(0xffffffffu, is_free), fars = __ballot_sync(0xffffffffu, is_far);
-            if (pass) {
-                const uint32_t i = first.x + nfree + __popc(frees & low), j = first.y + nfar + __popc(fars & low);
-                if (is_free && i < p.cap) to_list[i] = e;
-                if (is_far && j < p.cap) from_list[j] = e;
-            }
-            nfree += __popc(frees);
-            nfar += __popc(fars);
+            const uint32_t e = e0 + w * 32 + lane;
+            equal += __popc(__ballot_sync(0xffffffffu, e < e1 && key_of(e) == prefix));
         }
-        if (pass == 0) {
-            first = ev_scan(lane == 0 ? make_uint2(nfree, nfar) : make_uint2(0u, 0u), warp_sums, warp, lane, all);
-            first.x = __shfl_sync(0xffffffffu, first.x, 0);
-            first.y = __shfl_sync(0xffffffffu, first.y, 0);
-            if (tid == 0) counts[1] = all;
-            cluster.sync();
-            for (uint32_t r = 0; r < ctas; ++r) {
-                const uint2 v = cluster.map_shared_rank(counts, r)[1];
-                if (r < rank) first.x += v.x, first.y += v.y;
-                moves += v.y;
+        eq0 = __shfl_sync(0xffffffffu, ev_scan(make_uint2(lane == 0 ? equal : 0u, 0u), warp_sums, warp, lane, all).x, 0);
+        if (tid == 0) counts[0] = all;
+        cluster.sync();
+        for (uint32_t r = 0; r < rank; ++r) eq0 += cluster.map_shared_rank(counts, r)[0].x;
+    }
+    // masks of the words wb, wb + 1, .. that stay: lane i's of word wb + i
+    uint32_t eq = eq0;
+    auto masks = [&](uint32_t wb) -> uint32_t {
+        uint32_t mine = 0;
+        for (uint32_t i = 0; i < 32 && wb + i < w1; ++i) {
+            const uint32_t e = e0 + (wb + i) * 32 + lane, k = e < e1 ? key_of(e) : 0u;
+            uint32_t m = __ballot_sync(0xffffffffu, e < e1 && k >= prefix);
+            if (some) {
+                const uint32_t eqs = __ballot_sync(0xffffffffu, e < e1 && k == prefix);
+                m = __ballot_sync(0xffffffffu, (m >> lane & 1u) && (k > prefix || eq + __popc(eqs & low) < need));
+                eq += __popc(eqs);
             }
-            moves = min(moves, p.cap);
+            if (lane == i) mine = m;
+        }
+        return mine;
+    };
+    auto upto = [](uint32_t e, uint32_t end) -> uint32_t {       // bits of the entries e .. e + 31 that lie below `end`
+        return e >= end ? 0u : end - e >= 32 ? 0xffffffffu : (1u << (end - e)) - 1u;
+    };
+    // this lane's word: its free entries below `keep` (x), its kept ones past it (y)
+    auto split = [&](uint32_t wb, uint32_t m) -> uint2 {
+        if (wb + lane >= w1) return make_uint2(0u, 0u);
+        const uint32_t e = e0 + (wb + lane) * 32, k = upto(e, p.keep);
+        return make_uint2(~m & k & upto(e, e1), m & ~k);
+    };
+    uint32_t kept = 0;
+    uint2 mine = make_uint2(0u, 0u);
+    for (uint32_t wb = w0; wb < w1; wb += 32) {
+        kept = masks(wb);
+        const uint2 f = split(wb, kept);
+        mine.x += __popc(f.x);
+        mine.y += __popc(f.y);
+    }
+    uint2 first = ev_scan(mine, warp_sums, warp, lane, all);     // before this lane's words (if they are one)
+    if (tid == 0) counts[1] = all;
+    cluster.sync();
+    uint32_t moves = 0;
+    for (uint32_t r = 0; r < ctas; ++r) {
+        const uint2 v = cluster.map_shared_rank(counts, r)[1];
+        if (r < rank) first.x += v.x, first.y += v.y;
+        moves += v.y;
+    }
+    moves = min(moves, p.cap);
+    const bool once = w1 - w0 <= 32;
+    if (!once) {                                 // several words a lane: from the warp's first entry on
+        first.x = __shfl_sync(0xffffffffu, first.x, 0);
+        first.y = __shfl_sync(0xffffffffu, first.y, 0);
+        eq = eq0;
+    }
+    for (uint32_t wb = w0; wb < w1; wb += 32) {
+        if (!once) kept = masks(wb);
+        const uint2 f = split(wb, kept);
+        uint2 at = first;
+        if (!once) {
+            uint2 incl = make_uint2(__popc(f.x), __popc(f.y));
+            const uint2 v = incl;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+                if (lane >= uint32_t(o)) incl.x += x, incl.y += y;
+            }
+            at.x += incl.x - v.x;
+            at.y += incl.y - v.y;
+            first.x += __shfl_sync(0xffffffffu, incl.x, 31);
+            first.y += __shfl_sync(0xffffffffu, incl.y, 31);
+        }
+        for (uint32_t i = 0; i < 32 && wb + i < w1; ++i) {
+            const uint32_t fx = __shfl_sync(0xffffffffu, f.x, i), fy = __shfl_sync(0xffffffffu, f.y, i);
+            const uint32_t ax = __shfl_sync(0xffffffffu, at.x, i) + __popc(fx & low), ay = __shfl_sync(0xffffffffu, at.y, i) + __popc(fy & low);
+            const uint32_t e = e0 + (wb + i) * 32 + lane;
+            if ((fx >> lane & 1u) && ax < p.cap) to_list[ax] = e;
+            if ((fy >> lane & 1u) && ay < p.cap) from_list[ay] = e;
         }
     }
     cluster.sync();                              // the lists are written (and no CTA reads another's memory after this)
