@@ -16,7 +16,9 @@ struct CtxView {
     cudaStream_t stream;
     uint32_t* err;                       // device error word
     std::atomic<uint64_t>* dispatches;
+    void* packed;                        // packed attention: plan and parts of cut tile pairs (packed_scratch_bytes)
 };
+size_t packed_scratch_bytes(int num_sms);                // smoe_serve.cu
 CtxView ctx_view(SmoeCudaCtx* c);                        // smoe_cuda.cu
 int ctx_fail(int code, const char* msg, long v);         // sets the message of the failure, returns code
 

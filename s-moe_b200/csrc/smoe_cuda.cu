@@ -86,6 +86,7 @@ struct SmoeCudaCtx {
     uint2* g_htab = nullptr;         // [max_batch * 16][max_d_ff / 16][8]
     float2* g_hgs = nullptr;         // [max_batch * 16][max_d_ff / 64]
     float* g_ys = nullptr;           // [max_batch * 16][max_d_model]
+    void* packed = nullptr;          // packed attention: plan and parts (smoe_serve.cu)
     // expert parallel: this rank's exchange window (IPC-exported) and rank 0's, mapped
     uint8_t* ep_win = nullptr;
     size_t ep_win_bytes = 0;
@@ -503,6 +504,7 @@ SmoeCudaCtx* smoe_cuda_init_ex(const SmoeCudaInitArgs* args) {
     if ((e = cudaMalloc(&c->g_htab, slots * a.max_d_ff * 4)) != cudaSuccess) return fail(e);
     if ((e = cudaMalloc(&c->g_hgs, slots * (a.max_d_ff / 64) * 8)) != cudaSuccess) return fail(e);
     if ((e = cudaMalloc(&c->g_ys, slots * a.max_d_model * 4)) != cudaSuccess) return fail(e);
+    if ((e = cudaMalloc(&c->packed, smoe::packed_scratch_bytes(c->num_sms))) != cudaSuccess) return fail(e);
     cudaMemsetAsync(c->lstate, 0, sizeof(smoe::LayerState), c->stream);
     cudaMemsetAsync(c->lpair, 0, size_t(smoe::kLMaxTok) * 128 * 8, c->stream);
     cudaMemsetAsync(c->attn_cnt, 0, size_t(smoe::kAttnMaxHeads) * 4, c->stream);
@@ -544,7 +546,7 @@ void smoe_cuda_destroy(SmoeCudaCtx* c) {
     if (c->ep_win) cudaFree(c->ep_win);
     for (auto& ev : c->events)
         if (ev) cudaEventDestroy(ev);
-    void* bufs[] = {c->g_list, c->g_count, c->g_xtab, c->g_xgs, c->g_htab, c->g_hgs, c->g_ys, c->lstate, c->lpair, c->lpart, c->attn_part, c->attn_cnt, c->hidden, c->slot_out, c->in_stage, c->batch_out, c->logits, c->ids,
+    void* bufs[] = {c->packed, c->g_list, c->g_count, c->g_xtab, c->g_xgs, c->g_htab, c->g_hgs, c->g_ys, c->lstate, c->lpair, c->lpart, c->attn_part, c->attn_cnt, c->hidden, c->slot_out, c->in_stage, c->batch_out, c->logits, c->ids,
                     c->wts, c->ticket, c->err, c->gemv_out, c->gemv_in, c->blas_ws, c->xsplit};
     for (void* b : bufs)
         if (b) cudaFree(b);
@@ -575,7 +577,7 @@ uint64_t smoe_cuda_kernel_dispatches(const SmoeCudaCtx* c) { return c ? c->dispa
 }  // extern "C"
 
 namespace smoe {
-CtxView ctx_view(SmoeCudaCtx* c) { return {c->device, c->num_sms, c->smem_optin, c->stream, c->err, &c->dispatches}; }
+CtxView ctx_view(SmoeCudaCtx* c) { return {c->device, c->num_sms, c->smem_optin, c->stream, c->err, &c->dispatches, c->packed}; }
 int ctx_fail(int code, const char* msg, long v) {
     std::snprintf(g_err, sizeof(g_err), "%s (%ld)", msg, v);
     return code;

@@ -109,6 +109,20 @@ int check_rows(const SmoeKv4Rows* r, const char* what) {
     return SMOE_OK;
 }
 
+// Offsets in the context's scratch for packed attention.
+struct PackedScratch {
+    size_t cost, place, list, part, stat, bytes;
+    explicit PackedScratch(int num_sms) {
+        const size_t rows = size_t(2) * num_sms * 256;
+        cost = 65536;                            // (the plan: 16 bytes a CTA and one more)
+        place = cost + size_t(smoe::kPaMaxPairs) * 4;
+        list = place + size_t(smoe::kPaMaxPairs) * 8;
+        part = list + size_t(smoe::kPaMaxPairs) * 8;
+        stat = part + rows * 128 * 4;
+        bytes = stat + rows * 8;
+    }
+};
+
 // A 4-bit attention call's launch and workspace, from its arguments alone
 // (the workspace is asked for without a context).
 struct AttnPlan {
@@ -131,6 +145,8 @@ struct AttnPlan {
 
 }  // namespace
 
+size_t smoe::packed_scratch_bytes(int num_sms) { return PackedScratch(num_sms).bytes; }
+
 extern "C" {
 
 int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a) {
@@ -149,7 +165,11 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
         return ctx_fail(SMOE_ERR_ARG, "packed attention needs 16-byte aligned bases and strides that are multiples of 8", 0);
     if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return ctx_fail(SMOE_ERR_ARG, "packed attention needs a finite scale >= 0", 0);
     const CtxView c = smoe::ctx_view(ctx);
-    smoe::PackedArgs p{*a, a->num_heads / a->num_kv_heads, 0, std::max(a->scale * 1.4426950408889634f, 1e-35f), c.err};
+    smoe::PackedArgs p{};
+    p.a = *a;
+    p.group = a->num_heads / a->num_kv_heads;
+    p.scale_log2 = std::max(a->scale * 1.4426950408889634f, 1e-35f);
+    p.err = c.err;
     // (a scale of 0 must still keep the masked scores' -inf: 1e-35 times any finite score is 0 to the exponential)
     p.tokens = smoe::kPaRows / p.group;
     CUtensorMap mq, mk, mv;
@@ -162,15 +182,38 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
     } else {
         mk = mv = mq;                            // no row has a key: never read
     }
-    // at most one partial tile pair a sequence; the kernel counts them
-    const uint64_t ctas = (uint64_t(a->total_q) / (2 * p.tokens) + std::min(a->n_seqs, a->total_q)) * a->num_kv_heads;
-    if (ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_ARG, "packed attention: too many rows", long(a->total_q));
-    auto run = [&](auto kern, size_t smem) -> int {
-        const int r = smem_limit(c, kern, smem);
-        return r ? r : launch(c, kern, dim3(uint32_t(ctas)), dim3(smoe::kPaThreads), smem, mq, mk, mv, p);
+    // at most one partial tile pair a sequence; the kernels count them
+    const uint64_t pairs = uint64_t(a->total_q) / (2 * p.tokens) + std::min(a->n_seqs, a->total_q), ctas = pairs * a->num_kv_heads;
+    const uint64_t most = pairs * (uint64_t(a->total_k) / smoe::kPaKeys + 2);
+    // A CTA per pair when all of them fit the GPU at once and none is long: the plan and the joining of cut pairs cost
+    // some 6 us. (Above 65,536 pairs, or 2^31 blocks, too.)
+    const bool direct = (ctas <= uint64_t(c.num_sms) && a->total_k <= 8 * smoe::kPaKeys) || pairs > smoe::kPaMaxPairs || most >= (uint64_t(1) << 31);
+    const bool sorted = !direct && ctas >= uint64_t(4) * c.num_sms;
+    const PackedScratch sc(c.num_sms);
+    uint8_t* ws = static_cast<uint8_t*>(c.packed);
+    const uint32_t grid = direct ? uint32_t(ctas) : uint32_t(c.num_sms);
+    if (!direct) {
+        smoe::PaPlace* plan = nullptr;
+        uint2* list = nullptr;
+        if (sorted) {
+            p.list = list = reinterpret_cast<uint2*>(ws + sc.list);
+            p.taken = reinterpret_cast<uint32_t*>(ws);
+        } else {
+            p.plan = plan = reinterpret_cast<smoe::PaPlace*>(ws);
+            p.part = reinterpret_cast<float*>(ws + sc.part);
+            p.stat = reinterpret_cast<float2*>(ws + sc.stat);
+        }
+        if ((rc = launch(c, smoe::k_packed_plan, dim3(1), dim3(smoe::kPlThreads), 0, p, plan, grid,
+                         reinterpret_cast<uint32_t*>(ws + sc.cost), reinterpret_cast<uint2*>(ws + sc.place), list)))
+            return rc;
+    }
+    auto run = [&](auto kern, size_t smem, auto join) -> int {
+        int r = smem_limit(c, kern, smem);
+        if (r || (r = launch(c, kern, dim3(grid), dim3(smoe::kPaThreads), smem, mq, mk, mv, p)) || !p.plan) return r;
+        return launch(c, join, dim3(grid, 8), dim3(256), 0, p);
     };
-    return a->head_dim <= 64 ? run(smoe::k_attention_packed<64>, smoe::PackedSmem<64>::bytes())
-                             : run(smoe::k_attention_packed<128>, smoe::PackedSmem<128>::bytes());
+    return a->head_dim <= 64 ? run(smoe::k_attention_packed<64>, smoe::PackedSmem<64>::bytes(), smoe::k_packed_join<64>)
+                             : run(smoe::k_attention_packed<128>, smoe::PackedSmem<128>::bytes(), smoe::k_packed_join<128>);
 }
 
 uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim) {
