@@ -314,6 +314,23 @@ SMOE_DEVINL float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 operations in one instruction.
+SMOE_DEVINL uint64_t pack2(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+SMOE_DEVINL void unpack2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+SMOE_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+SMOE_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 SMOE_DEVINL uint32_t cvt_bf16x2(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -640,9 +657,16 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         }
                         odd = any(both, __hisnan(acc.x) || __hisnan(acc.y));
                     }
-                    float mx = m;
+                    float mq[8];                 // eight chains: the maximum's latency is the softmax warps' to wait for
 #pragma unroll
-                    for (int j = 0; j < 128; ++j) mx = fmaxf(mx, s[j]);
+                    for (int j = 0; j < 8; ++j) mq[j] = fmaxf(s[2 * j], s[2 * j + 1]);
+#pragma unroll
+                    for (int j = 16; j < 128; j += 2) mq[j / 2 % 8] = fmaxf(fmaxf(mq[j / 2 % 8], s[j]), s[j + 1]);
+#pragma unroll
+                    for (int w = 4; w; w >>= 1)
+#pragma unroll
+                        for (int j = 0; j < w; ++j) mq[j] = fmaxf(mq[j], mq[j + w]);
+                    const float mx = fmaxf(m, mq[0]);
                     // (each row for itself - a factor of 1 leaves the others of the
                     // warp as they are - so a row's bits do not depend on its neighbours)
                     const bool move = live && ((mx - m) * sl > 8.0f || (mx > m && m == -INFINITY));
@@ -666,14 +690,18 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         if (move) m = mx;
                     }
                     const float ml = m == -INFINITY ? 0.0f : m * sl;
-                    float sum = 0.0f;
+                    const uint64_t sl2 = pack2(sl, sl), ml2 = pack2(-ml, -ml);
+                    uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t w[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const float x = ex2(fmaf(s[c * 32 + 2 * k], sl, -ml)), y = ex2(fmaf(s[c * 32 + 2 * k + 1], sl, -ml));
-                            sum += x + y;
+                            float x, y;
+                            unpack2(fma2(pack2(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]), sl2, ml2), x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                            sums[k % 2] = add2(sums[k % 2], pack2(x, y));
                             w[k] = cvt_bf16x2(x, y);
                         }
                         tmem_st16(ts + c * 16, w);
@@ -735,7 +763,9 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         fence_proxy_async();     // the tensor core reads what these threads wrote
                         any(both, false);
                     }
-                    l += sum;
+                    float sum_x, sum_y;
+                    unpack2(add2(sums[0], sums[1]), sum_x, sum_y);
+                    l += sum_x + sum_y;
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
