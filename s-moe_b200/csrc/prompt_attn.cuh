@@ -23,7 +23,8 @@ namespace smoe {
 //  - few pairs: each CTA takes an equal share of the line of all pairs' key
 //    blocks, and the parts of a pair that is cut are joined by k_packed_join.
 constexpr uint32_t kPaRows = 128, kPaKeys = 128;
-constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA warp, MMA warp, the items' warp and an idle one (a register split goes by four)
+constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA, MMA, items and checks, a warp each (a register split goes by four warps)
+constexpr int kPaPoly = 4;                        // every 4th pair of exponentials is a polynomial
 constexpr int kPaItems = 2;                       // items that a CTA has at hand: the one in work and the next
 constexpr uint32_t kPaMaxPairs = 65536;          // tile pairs of a planned call (per KV head)
 
@@ -49,14 +50,17 @@ struct PackedArgs {
 template <int HP>                                // head_dim rounded up to 64 or 128
 struct PackedSmem {
     static constexpr uint32_t TILE = HP / 64 * 16384;            // 128 rows, 64-column halves of 128-byte rows
-    static constexpr int STAGES = HP == 128 ? 5 : 8;
-    static constexpr uint32_t Q = 0, KV = 2 * TILE, BAR = KV + STAGES * TILE, ITEMS = BAR + 384, END = ITEMS + kPaItems * 64;
+    static constexpr int STAGES = HP == 128 ? 4 : 8;             // even: keys in the even ones, values in the odd
+    static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + STAGES * TILE;        // OUT: 4 KB a softmax warp, rows on their way out
+    static constexpr uint32_t BAR = OUT + 8 * 4096, ITEMS = BAR + 384, END = ITEMS + kPaItems * 64;
     static constexpr uint32_t bytes() { return END + 1024; }     // the base is rounded up to 1024
 };
 
 // Keys [lo, hi) of a token at index i of its sequence.
 struct PackedSeq {
-    uint32_t q0, k0, len_q, len_k, causal, window;
+    uint32_t q0, k0, len_q, len_k;
+    uint16_t causal, bad;                        // bad: its rows are not in the buffers (len_q 0 then)
+    uint32_t window;
     SMOE_DEVINL uint32_t hi(uint32_t i) const {
         if (!causal) return len_k;
         const int64_t h = int64_t(i) + 1 + int64_t(len_k) - int64_t(len_q);
@@ -81,7 +85,7 @@ SMOE_DEVINL PackedSeq packed_seq(const SmoeCudaPackedAttnArgs& a, uint32_t s) {
     const uint32_t* ck = a.cu_k ? a.cu_k : a.cu_q;
     const uint32_t q0 = ld_plain(a.cu_q + s), q1 = ld_plain(a.cu_q + s + 1), k0 = ld_plain(ck + s), k1 = ld_plain(ck + s + 1);
     const bool ok = q0 <= q1 && q1 <= a.total_q && k0 <= k1 && k1 <= a.total_k;
-    return {q0, k0, ok ? q1 - q0 : 0u, ok ? k1 - k0 : 0u, a.causal, a.window};
+    return {q0, k0, ok ? q1 - q0 : 0u, ok ? k1 - k0 : 0u, uint16_t(a.causal != 0), uint16_t(!ok), a.window};
 }
 
 // What a CTA does next: some blocks of a tile pair. Worked out by a warp of
@@ -96,11 +100,17 @@ struct alignas(16) PaItem {
     uint16_t more, pad;                          // 0: there was no further item
 };
 static_assert(sizeof(PaItem) == 64, "an item's place in shared memory");
+// Whether some row of the pair may not see some key of the item's block i.
+SMOE_DEVINL bool pa_masked(const PaItem& it, uint32_t i) {
+    const uint32_t key0 = it.key0 + i * kPaKeys;
+    return key0 + kPaKeys > it.inner_hi || key0 < it.inner_lo;
+}
 struct PaWalk {
     PaPlace at, end;
     bool single;                                 // just the pair at `at`
     // the next item, false when there is none; afterwards `at` is behind it
     SMOE_DEVINL bool next(const PackedArgs& p, PaItem& it) {
+#pragma unroll 1
         for (;;) {
             if (at.kvh > end.kvh || (at.kvh == end.kvh && (at.seq > end.seq || (at.seq == end.seq && at.tok > end.tok)))) return false;
             const bool last = at.kvh == end.kvh && at.seq == end.seq && at.tok == end.tok;
@@ -169,25 +179,28 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
     pdl_acquire();
     const uint32_t tid = threadIdx.x, span = 2 * p.tokens;
     uint32_t pairs = 0, all;
+#pragma unroll 1
     for (uint32_t b = 0; b < p.a.n_seqs; b += kPlThreads) {      // the pairs' places, a thread a sequence
         const uint32_t s = b + tid;
         uint32_t n = 0;
         PackedSeq S{};
         if (s < p.a.n_seqs) {
             S = packed_seq(p.a, s);
-            const uint32_t* ck = p.a.cu_k ? p.a.cu_k : p.a.cu_q;
-            if (S.len_q != ld_plain(p.a.cu_q + s + 1) - S.q0 || S.len_k != ld_plain(ck + s + 1) - S.k0) serve_err(p.err, SMOE_DEVERR_BAD_RANGE);
+            if (S.bad) serve_err(p.err, SMOE_DEVERR_BAD_RANGE);
             n = (S.len_q + span - 1) / span;
         }
         const uint32_t first = pairs + pl_scan(n, sums, all);
         // (one long sequence: its places are written by all threads below)
+#pragma unroll 1
         for (uint32_t i = 0; i < min(n, 8u); ++i)
             if (first + i < kPaMaxPairs) place[first + i] = make_uint2(s, i * span);
         uint32_t more = __ballot_sync(0xffffffffu, n > 8);
+#pragma unroll 1
         while (more) {
             const int l = __ffs(more) - 1;
             more &= more - 1;
             const uint32_t nn = __shfl_sync(0xffffffffu, n, l), ff = __shfl_sync(0xffffffffu, first, l), ss = __shfl_sync(0xffffffffu, s, l);
+#pragma unroll 1
             for (uint32_t i = 8 + (tid & 31); i < nn; i += 32)
                 if (ff + i < kPaMaxPairs) place[ff + i] = make_uint2(ss, i * span);
         }
@@ -198,6 +211,7 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
     if (list) {
         bins[tid] = 0;
         __syncthreads();
+#pragma unroll 1
         for (uint32_t i = tid; i < pairs; i += kPlThreads) {
             const uint2 at = place[i];
             const PackedSeq S = packed_seq(p.a, at.x);
@@ -209,6 +223,7 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
         const uint32_t before = pl_scan(bins[tid], sums, all);
         bins[tid] = before;
         __syncthreads();
+#pragma unroll 1
         for (uint32_t i = tid; i < pairs; i += kPlThreads) list[atomicAdd(&bins[kPlThreads - 1 - cost[i]], 1u)] = place[i];
         if (tid == 0) {
             p.taken[0] = 0;
@@ -217,6 +232,7 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
         return;
     }
     uint32_t total = 0;                          // (below 2^31: the host bounds it)
+#pragma unroll 1
     for (uint32_t b = 0; b < pairs; b += kPlThreads) {
         const uint32_t i = b + tid;
         uint32_t n = 0;
@@ -230,11 +246,13 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
         total += all;
     }
     __syncthreads();
+#pragma unroll 1
     for (uint32_t c = tid; c <= ctas; c += kPlThreads) {
         PaPlace at{p.a.num_kv_heads, 0u, 0u, 0u};
         const uint64_t x = uint64_t(total) * p.a.num_kv_heads * c / ctas;
         if (c < ctas && pairs) {
             uint32_t kvh = uint32_t(x / total), y = uint32_t(x % total), lo = 0, hi = pairs - 1;
+#pragma unroll 1
             while (lo < hi) {                    // the last pair whose cost starts at or before y
                 const uint32_t mid = (lo + hi + 1) / 2;
                 if (cost[mid] <= y) lo = mid;
@@ -331,32 +349,57 @@ SMOE_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+SMOE_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// 2^x of two numbers without the exponential unit (16 results a cycle and SM,
+// half of what the tensor cores would need): x = n + f with n a whole number
+// and f in [-1/2, 1/2] (Cody and Waite), a polynomial of degree 4 in f fitted
+// for the smallest largest relative error (2.6e-6), times 2^n. Below -127 it is 0 (masked scores), a
+// NaN stays one.
+SMOE_DEVINL uint64_t ex2_poly(uint64_t x) {
+    float a, b;
+    unpack2(x, a, b);
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+    x = pack2(a, b);
+    const float magic = 12582912.0f;             // 1.5 x 2^23: adding it rounds to a whole number, in the low bits
+    const uint64_t r = add2(x, pack2(magic, magic)), f = add2(x, mul2(add2(r, pack2(-magic, -magic)), pack2(-1.0f, -1.0f)));
+    uint64_t y = fma2(pack2(0.009570101f, 0.009570101f), f, pack2(0.05591786f, 0.05591786f));
+    y = fma2(y, f, pack2(0.24024744f, 0.24024744f));
+    y = fma2(y, f, pack2(0.6931218f, 0.6931218f));
+    y = fma2(y, f, pack2(0.9999993f, 0.9999993f));
+    float ra, rb;
+    unpack2(r, ra, rb);
+    const float sa = __uint_as_float(__float_as_uint(ra) * 8388608u + 0x3F800000u), sb = __uint_as_float(__float_as_uint(rb) * 8388608u + 0x3F800000u);
+    return mul2(y, pack2(sa, sb));
+}
 SMOE_DEVINL uint32_t cvt_bf16x2(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-// (Inlined: a call would bring the calling convention's registers into the
-// softmax warps' budget.) A bounded wait: after one ran out, all others of the CTA return at once.
-// The roles then finish their loops on whatever the buffers hold (every
-// address stays in the CTA's own memory) and the error word is set.
-SMOE_DEVINL void pa_wait_slow(uint64_t* bar, uint32_t parity, volatile uint32_t* fail, uint32_t* err) {
-    const uint64_t end = gtimer() + SMOE_WAIT_NS_DEFAULT;
+// A bounded wait, small enough to be inlined at each place (a call would
+// bring the calling convention's registers into the softmax warps' budget):
+// some tenths of a second of polls. After one ran out, all others of the CTA
+// give up within 256; the roles then finish on whatever the buffers hold
+// (every address stays in the CTA's own memory) and the error word is set.
+constexpr uint32_t kPaPolls = 1u << 24;
+SMOE_DEVINL void pa_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* fail, uint32_t* err) {
 #pragma unroll 1
-    for (uint32_t i = 0; i < SMOE_SPIN_LIMIT; ++i) {
-        if (mbar_try_wait(bar, parity)) return;
-        if ((i & 15) == 15 && (*fail || gtimer() > end)) break;
-    }
-    *fail = 1u;
-    atomicCAS(err, 0u, uint32_t(SMOE_DEVERR_MBAR_TIMEOUT));
+    for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i)
+        if ((i & 255) == 255 && (*fail || i >= kPaPolls)) {
+            *fail = 1u;
+            atomicCAS(err, 0u, uint32_t(SMOE_DEVERR_MBAR_TIMEOUT));
+            break;
+        }
 }
-
 // The same regardless of earlier failures: for copies and products in flight.
 SMOE_DEVINL void pa_drain(uint64_t* bar, uint32_t parity) {
-    const uint64_t end = gtimer() + SMOE_WAIT_NS_DEFAULT;
 #pragma unroll 1
-    for (uint32_t i = 0; i < SMOE_SPIN_LIMIT; ++i)
-        if (mbar_try_wait(bar, parity) || ((i & 15) == 15 && gtimer() > end)) return;
+    for (uint32_t i = 0; i < kPaPolls && !mbar_try_wait(bar, parity); ++i) {}
 }
 
 template <int HP>
@@ -369,13 +412,12 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR);
-    uint64_t *qf = bars, *qe = bars + 2, *sf = bars + 4, *pr = bars + 6, *of = bars + 8, *itf = bars + 10, *ite = itf + kPaItems, *xb = ite + kPaItems, *kvf = xb + 3, *kve = kvf + ST;
+    uint64_t *qf = bars, *qe = bars + 2, *sf = bars + 4, *pr = bars + 6, *pl = bars + 8, *of = bars + 10, *vc = bars + 12, *itf = bars + 16, *ite = itf + kPaItems, *xb = ite + kPaItems, *kvf = xb + 3, *kve = kvf + ST;
     uint32_t* words = reinterpret_cast<uint32_t*>(kve + ST);
     PaItem* items = reinterpret_cast<PaItem*>(smem + SM::ITEMS);
     volatile uint32_t *fail = words, *begun = words + 1;         // begun[t]: the accumulator holds something before block 0's P V
     uint32_t* tslot = words + 3;
-    volatile uint32_t* xflag = words + 6;                        // [3 meetings of softmax warps][3 turns] somebody said yes
-    uint32_t* where = words + 4;                                 // without a plan: the CTA's sequence and first token
+    volatile uint32_t* odds = words + 6;                         // [4] of the last masked blocks: its values hold an infinity or NaN
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const SmoeCudaPackedAttnArgs& a = p.a;
 
@@ -386,17 +428,18 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
             mbar_init(qe + i, 1);
             mbar_init(sf + i, 1);
             mbar_init(pr + i, 4);
+            mbar_init(pl + i, 4);
             mbar_init(of + i, 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(vc + i, 1);
         for (int i = 0; i < kPaItems; ++i) {
             mbar_init(itf + i, 1);
-            mbar_init(ite + i, 10);              // the TMA lane, the MMA lane, eight softmax warps
+            mbar_init(ite + i, 11);              // the TMA lane, the MMA lane, the checking warp, eight softmax warps
         }
         for (int i = 0; i < 3; ++i) mbar_init(xb + i, i < 2 ? 4 : 8);
-        for (int i = 0; i < 9; ++i) xflag[i] = 0u;
         for (int i = 0; i < ST; ++i) {
             mbar_init(kvf + i, 1);
-            mbar_init(kve + i, 1);
+            mbar_init(kve + i, 1 + i % 2);       // the MMA lane; of values (odd stages), the checking warp, too
         }
         *fail = begun[0] = begun[1] = 0u;
         fence_mbar_init();
@@ -404,60 +447,11 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     if (warp == 9) tmem_alloc(tslot, 512);
     pdl_acquire();
 
-    PaWalk walk;
-    walk.single = !p.plan;
-    if (p.list) {
-    } else if (p.plan) {
-        walk.at = p.plan[blockIdx.x];
-        walk.end = p.plan[blockIdx.x + 1];
-    } else {
-        // The CTA's tile pair, counted from the last one backwards: later
-        // tokens have more keys, so long tiles start first. One lane per sequence.
-        const uint32_t kvh = blockIdx.x % a.num_kv_heads, span = 2 * p.tokens;
-        if (warp == 0) {
-            uint32_t total = 0;
-            auto pairs = [&](uint32_t s) -> uint32_t {
-                if (s >= a.n_seqs) return 0u;
-                const PackedSeq S = packed_seq(a, s);
-                const uint32_t* ck = a.cu_k ? a.cu_k : a.cu_q;
-                if (blockIdx.x == 0 && (S.len_q != ld_plain(a.cu_q + s + 1) - S.q0 || S.len_k != ld_plain(ck + s + 1) - S.k0))
-                    serve_err(p.err, SMOE_DEVERR_BAD_RANGE);
-                return (S.len_q + span - 1) / span;
-            };
-            for (uint32_t b = 0; b < a.n_seqs; b += 32) total += __reduce_add_sync(0xffffffffu, pairs(b + lane));
-            const uint32_t me = blockIdx.x / a.num_kv_heads;
-            if (lane == 0) where[0] = a.n_seqs;
-            __syncwarp();
-            if (me < total) {
-                uint32_t want = total - 1 - me, before = 0;
-                for (uint32_t b = 0; b < a.n_seqs; b += 32) {
-                    const uint32_t n = pairs(b + lane);
-                    uint32_t incl = n;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-                        if (lane >= uint32_t(o)) incl += v;
-                    }
-                    const uint32_t first = before + incl - n;
-                    if (want >= first && want < first + n) {
-                        where[0] = b + lane;
-                        where[1] = (want - first) * span;
-                    }
-                    before += __shfl_sync(0xffffffffu, incl, 31);
-                    if (before > want) break;
-                }
-            }
-        }
-        __syncthreads();
-        walk.at = {kvh, where[0], where[1], 0u};
-        walk.end = walk.at;
-        if (where[0] >= a.n_seqs) walk.at.kvh = walk.end.kvh + 1;              // past the last pair
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tslot;
-    auto wait = [&](uint64_t* b, uint32_t ph) { if (!*fail && !mbar_try_wait(b, ph & 1)) pa_wait_slow(b, ph & 1, fail, p.err); };
+    auto wait = [&](uint64_t* b, uint32_t ph) { pa_wait(b, ph & 1, fail, p.err); };
     // item k, of a role; and done with it
     auto item = [&](uint32_t k) -> const PaItem& {
         wait(itf + k % kPaItems, k / kPaItems);
@@ -471,12 +465,14 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         // ---------------------------------------------------- loads (one lane)
         if (elect_one()) {
             uint32_t j = 0, nq[2] = {0u, 0u};    // units sent for, Q tiles sent for
+#pragma unroll 1
             for (uint32_t k = 0; !*fail; ++k) {
                 const PaItem& it = item(k);
                 if (!it.more) break;
                 const uint32_t m = max(it.cnt[0], it.cnt[1]), kvh = it.kvh, row_q = it.S.q0 + it.tok, row_k = it.S.k0 + it.key0;
                 const uint32_t cnt[2] = {it.cnt[0], it.cnt[1]};
                 item_done(k);
+#pragma unroll 1
                 for (uint32_t i = 0; i < 2 * m; ++i, ++j) {      // K0 V0 K1 V1 .., the Q tiles around K0
                     if (i < 2 && (i ? cnt[1] : cnt[0])) {
                         const uint32_t q = i ? nq[1]++ : nq[0]++;
@@ -494,6 +490,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
             }
             // nothing may be in flight when the CTA ends (the MMA warp has
             // waited for all of it unless a wait ran out)
+#pragma unroll 1
             for (uint32_t k = j > ST ? j - ST : 0; k < j; ++k) pa_drain(kvf + k % ST, (k / ST) & 1);
             for (int t = 0; t < 2; ++t)
                 if (nq[t]) pa_drain(qf + t, (nq[t] - 1) & 1);
@@ -514,13 +511,19 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 tc_commit(sf + t);
                 if (last) tc_commit(qe + t);     // the tile's Q has been read
             };
-            auto pv = [&](uint32_t t, uint32_t st, bool more) {
+            auto pv = [&](uint32_t t, uint32_t st, bool more, uint32_t block) {
                 const uint64_t vd = tc_desc_sw128(skv + st * SM::TILE, 16384);
 #pragma unroll
-                for (int s = 0; s < kPaKeys / 16; ++s)
+                for (int s = 0; s < kPaKeys / 16; ++s) {
+                    if (s == kPaKeys / 16 * 3 / 4) {             // the last quarter of P
+                        wait(pl + t, block);
+                        tc_fence_after();
+                    }
                     tc_mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + s * 8, vd + ((s * 2048) >> 4), IPV, more || s > 0);
+                }
                 tc_commit(of + t);
             };
+#pragma unroll 1
             for (uint32_t k = 0; !*fail; ++k) {
                 const PaItem& it = item(k);
                 if (!it.more) break;
@@ -537,6 +540,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         }
                     tc_commit(kve + j0 % ST);
                 }
+#pragma unroll 1
                 for (uint32_t i = 0; i < m; ++i) {
                     const uint32_t jv = j0 + 2 * i + 1, jk = jv + 1, sv = jv % ST, sk = jk % ST;
                     wait(kvf + sv, jv / ST);
@@ -547,9 +551,9 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         if (i < nt) {
                             // (of an item's first block this also says that the
                             // softmax warps have read the last item's sums)
-                            wait(pr + t, nb[t]++);
+                            wait(pr + t, nb[t]);
                             tc_fence_after();
-                            pv(t, sv, i > 0 || begun[t]);
+                            pv(t, sv, i > 0 || begun[t], nb[t]++);
                         }
                         if (i + 1 < nt) qk(t, sk, i + 2 == nt);
                     }
@@ -562,28 +566,111 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         }
     } else if (warp == 10) {
         // ------------------------------------------------------------- items
+        PaWalk walk;
+        walk.single = !p.plan;
+        uint32_t pairs = 0;
+        if (p.list) {
+            pairs = ld_plain(p.taken + 1);
+        } else if (p.plan) {
+            walk.at = p.plan[blockIdx.x];
+            walk.end = p.plan[blockIdx.x + 1];
+        } else {
+            // The CTA's tile pair, counted from the last one backwards: later
+            // tokens have more keys, so long tiles start first. One lane a sequence.
+            const uint32_t kvh = blockIdx.x % a.num_kv_heads, me = blockIdx.x / a.num_kv_heads, span = 2 * p.tokens;
+            auto count = [&](uint32_t s) -> uint32_t {
+                if (s >= a.n_seqs) return 0u;
+                const PackedSeq S = packed_seq(a, s);
+                if (S.bad && blockIdx.x == 0) serve_err(p.err, SMOE_DEVERR_BAD_RANGE);
+                return (S.len_q + span - 1) / span;
+            };
+            uint32_t total = 0, seq = a.n_seqs, tok = 0, n = 0, before = 0;
+#pragma unroll 1
+            for (uint32_t b = 0; b < a.n_seqs; b += 32) total += __reduce_add_sync(0xffffffffu, n = count(b + lane));
+            const uint32_t want = total - 1 - me;
+#pragma unroll 1
+            for (uint32_t b = 0; b < a.n_seqs && me < total && before <= want; b += 32) {
+                if (a.n_seqs > 32) n = count(b + lane);          // (else they are still at hand)
+                uint32_t incl = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= uint32_t(o)) incl += v;
+                }
+                const uint32_t first = before + incl - n, hit = __ballot_sync(0xffffffffu, want >= first && want < first + n);
+                if (hit) {
+                    seq = b + __ffs(hit) - 1;
+                    tok = __shfl_sync(0xffffffffu, (want - first) * span, __ffs(hit) - 1);
+                }
+                before += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            walk.at = {kvh, seq, tok, 0u};
+            walk.end = walk.at;
+            if (seq >= a.n_seqs) walk.at.kvh = kvh + 1;          // past the last pair
+        }
         if (elect_one()) {
             bool more = true;
-            const uint32_t pairs = p.list ? ld_plain(p.taken + 1) : 0u;
+#pragma unroll 1
             for (uint32_t k = 0; more && !*fail; ++k) {
                 PaItem it{};
                 if (k >= kPaItems) wait(ite + k % kPaItems, k / kPaItems - 1);
                 if (p.list) {
                     const uint32_t i = atomicAdd(p.taken, 1u), pair = i / a.num_kv_heads;
-                    more = pair < pairs;
-                    if (more) {
-                        const uint2 q = ld_plain(p.list + pair);
-                        walk.at = {i % a.num_kv_heads, q.x, q.y, 0u};
-                        walk.end = walk.at;
-                        walk.next(p, it);
-                    }
-                } else {
-                    more = walk.next(p, it);
+                    const uint2 q = pair < pairs ? ld_plain(p.list + pair) : make_uint2(0u, 0u);
+                    walk.at = {i % a.num_kv_heads, q.x, q.y, 0u};
+                    walk.end = walk.at;
+                    if (pair >= pairs) walk.at.kvh = walk.end.kvh + 1;
                 }
+                more = walk.next(p, it);
                 it.more = more;
                 items[k % kPaItems] = it;
                 mbar_arrive(itf + k % kPaItems);
             }
+        }
+    } else {
+        // ------------------------------------------------- checks (one warp)
+        // Values of blocks that not every row may see all of: is there an
+        // infinity or NaN?
+        uint32_t j0 = 0, nm = 0;
+#pragma unroll 1
+        for (uint32_t k = 0;; ++k) {
+            const PaItem& it = item(k);
+            if (__any_sync(0xffffffffu, *fail || !it.more)) break;
+            const uint32_t m = max(it.cnt[0], it.cnt[1]);
+#pragma unroll 1
+            for (uint32_t i = 0; i < m; ++i) {
+                const uint32_t jv = j0 + 2 * i + 1;
+                wait(kvf + jv % ST, jv / ST);    // (all of them in turn: a phase skipped could be taken for another)
+                if (!pa_masked(it, i)) {
+                    if (lane == 0) mbar_arrive(kve + jv % ST);
+                    continue;
+                }
+                const uint4* v = reinterpret_cast<const uint4*>(smem + SM::KV + jv % ST * SM::TILE) + lane;
+                __nv_bfloat162 acc[4];
+                const __nv_bfloat162 zero = __float2bfloat162_rn(0.0f);
+                acc[0] = acc[1] = acc[2] = acc[3] = zero;
+#pragma unroll 8
+                for (uint32_t q = 0; q < SM::TILE / 16; q += 32) {               // 0 times one of those is a NaN
+                    const uint4 x = v[q];
+                    acc[0] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), zero, acc[0]);
+                    acc[1] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), zero, acc[1]);
+                    acc[2] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), zero, acc[2]);
+                    acc[3] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), zero, acc[3]);
+                }
+                const __nv_bfloat162 all = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
+                const bool odd = __any_sync(0xffffffffu, __hisnan(all.x) || __hisnan(all.y));
+                if (lane == 0) {
+                    // (At most four V tiles are in the ring, so of the masked block four
+                    // back all products are done: the softmax warps have read its flag.)
+                    odds[nm % 4] = odd;
+                    mbar_arrive(vc + nm % 4);
+                    mbar_arrive(kve + jv % ST);
+                }
+                ++nm;
+            }
+            j0 += 2 * m;
+            __syncwarp();
+            if (lane == 0) item_done(k);
         }
     }
     } else {
@@ -598,22 +685,18 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         const float sl = p.scale_log2;
         const uint32_t tk = r / p.group, hd = r % p.group;       // the row's token of the tile and head of the group
         uint32_t j0 = 0, nb = 0;                 // units and this tile's blocks so far
-        // A meeting of this tile's four warps, or of both tiles' eight: whether
-        // any thread came with yes. (An mbarrier and not a named one, so that
-        // the wait is bounded. A turn's flag is cleared a turn ahead: by then all have read its last use.)
+        uint32_t nm = 0;                         // masked blocks so far
+        // A meeting of this tile's four warps, or of both tiles' eight. (An
+        // mbarrier and not a named one, so that the wait is bounded.)
         uint32_t met[2] = {0u, 0u};
-        auto any = [&](bool all, bool yes) -> bool {
+        auto meet = [&](bool all) {
             const uint32_t x = all ? 2u : t, turn = all ? met[1]++ : met[0]++;
-            const bool mine = __any_sync(0xffffffffu, yes);
             __syncwarp();
-            if (lane == 0) {
-                xflag[x * 3 + (turn + 1) % 3] = 0u;
-                if (mine) xflag[x * 3 + turn % 3] = 1u;
-                mbar_arrive(xb + x);
-            }
+            if (lane == 0) mbar_arrive(xb + x);
             wait(xb + x, turn);
-            return __any_sync(0xffffffffu, xflag[x * 3 + turn % 3] != 0u);
+            __syncwarp();
         };
+#pragma unroll 1
         for (uint32_t k = 0;; ++k) {
             const PaItem& im = item(k);
             if (__any_sync(0xffffffffu, *fail || !im.more)) break;
@@ -627,7 +710,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll 1
                 for (uint32_t i = 0; i < nt; ++i) {
                     const uint32_t key0 = first_key + i * kPaKeys, jv = j0 + 2 * i + 1;
-                    const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;
+                    const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;   // (pa_masked)
                     float s[128];
                     wait(sf + t, nb + i);
                     tc_fence_after();
@@ -639,23 +722,18 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     uint4* const vt = reinterpret_cast<uint4*>(smem + SM::KV + jv % ST * SM::TILE);
                     if (masked) {
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
-                            if (uint32_t(j) < ja || uint32_t(j) >= jb) s[j] = -INFINITY;
+                        for (int c = 0; c < 4; ++c) {            // bits of the 32 columns in [ja, jb)
+                            auto below = [](uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+                            const uint32_t from = ja > c * 32u ? ja - c * 32u : 0u, to_ = jb > c * 32u ? jb - c * 32u : 0u, open = below(to_) & ~below(from);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(open >> j & 1u)) s[c * 32 + j] = -INFINITY;
+                        }
                         // A zero probability does not silence an infinity or NaN
                         // in the matrix product, and this block has keys that
-                        // not every row may see: look for one.
-                        wait(kvf + jv % ST, jv / ST);
-                        __nv_bfloat162 acc = __float2bfloat162_rn(0.0f);
-                        const __nv_bfloat162 zero = acc;
-#pragma unroll 4
-                        for (uint32_t k = r; k < SM::TILE / 16; k += 128) {
-                            const uint4 x = vt[k];
-                            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                acc = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&xs[q]), zero, acc);
-                        }
-                        odd = any(both, __hisnan(acc.x) || __hisnan(acc.y));
+                        // not every row may see: was there one?
+                        wait(vc + nm % 4, nm / 4);
+                        odd = __any_sync(0xffffffffu, odds[nm++ % 4]);
                     }
                     float mq[8];                 // eight chains: the maximum's latency is the softmax warps' to wait for
 #pragma unroll
@@ -692,21 +770,34 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     const float ml = m == -INFINITY ? 0.0f : m * sl;
                     const uint64_t sl2 = pack2(sl, sl), ml2 = pack2(-ml, -ml);
                     uint64_t sums[2] = {0ull, 0ull};
+                    if (i == 0 && r == 0) begun[t] = odd;        // the product then adds to what the rows put there
+                    auto give = [&](uint64_t* b) {               // what this warp has put into tensor memory, to the MMA warp
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b);
+                    };
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t w[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
+                            const uint64_t z = fma2(pack2(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]), sl2, ml2);
                             float x, y;
-                            unpack2(fma2(pack2(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]), sl2, ml2), x, y);
-                            x = ex2(x);
-                            y = ex2(y);
+                            if (k % kPaPoly == kPaPoly - 1) {
+                                unpack2(ex2_poly(z), x, y);
+                            } else {
+                                unpack2(z, x, y);
+                                x = ex2(x);
+                                y = ex2(y);
+                            }
                             sums[k % 2] = add2(sums[k % 2], pack2(x, y));
                             w[k] = cvt_bf16x2(x, y);
                         }
                         tmem_st16(ts + c * 16, w);
+                        // three quarters of the block's product can start
+                        if (c == 2 && !odd) give(pr + t);
                     }
-                    if (i == 0 && r == 0) begun[t] = odd;        // the product then adds to what the rows put there
                     if (odd) {
                         // Rare. Each row adds its own share of the infinities and
                         // NaN to its accumulator; then they are zeroed in the
@@ -748,7 +839,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                             for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k]);
                             tmem_st16(to + c, w);
                         }
-                        any(both, false);  // all rows of both tiles have read them
+                        meet(both);  // all rows of both tiles have read them
 #pragma unroll 1
                         for (uint32_t k = both ? tid : r; k < SM::TILE / 16; k += both ? 256 : 128) {
                             uint4 x = vt[k];
@@ -761,63 +852,77 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                             vt[k] = make_uint4(xs[0], xs[1], xs[2], xs[3]);
                         }
                         fence_proxy_async();     // the tensor core reads what these threads wrote
-                        any(both, false);
+                        meet(both);
                     }
                     float sum_x, sum_y;
                     unpack2(add2(sums[0], sums[1]), sum_x, sum_y);
                     l += sum_x + sum_y;
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(pr + t);
+                    if (odd) give(pr + t);
+                    give(pl + t);
                 }
                 nb += nt;
                 wait(of + t, nb - 1);
                 tc_fence_after();
             }
+            for (uint32_t i = nt; i < im.cnt[t ^ 1]; ++i) nm += pa_masked(im, i);
             j0 += 2 * max(im.cnt[0], im.cnt[1]);
             const uint32_t token = im.tok + t * p.tokens + tk, head = im.kvh * p.group + hd;
-            if (im.whole) {
-                const bool keys = live && im.S.hi(token) > im.S.lo(token);
+            // Rows go out through shared memory, 128 bytes of each at a time:
+            // eight lanes a row, four whole lines an instruction (a thread
+            // storing its own row touches 32 lines with each).
+            const bool whole = im.whole, keys = live && im.S.hi(token) > im.S.lo(token);
+            uint4* const out = reinterpret_cast<uint4*>(smem + SM::OUT) + warp * 256;
+            const uint32_t row = lane / 8, piece = lane % 8;
+            uint8_t* dst;
+            if (whole) {
                 const float inv = keys ? 1.0f / l : 0.0f;
-                uint16_t* dst = a.out + uint64_t(im.S.q0 + token) * a.out_row + uint64_t(head) * a.out_head;
-#pragma unroll 1
-                for (uint32_t c = 0; c < HP; c += 32) {
-                    float o[32];
-                    if (nt) {
-                        tmem_ld32(to + c, o);
-                        tmem_ld_wait();
-                    }
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                        if (live && c + h * 8 < a.head_dim) {
-                            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                            if (keys) {
-                                w.x = cvt_bf16x2(o[h * 8] * inv, o[h * 8 + 1] * inv);
-                                w.y = cvt_bf16x2(o[h * 8 + 2] * inv, o[h * 8 + 3] * inv);
-                                w.z = cvt_bf16x2(o[h * 8 + 4] * inv, o[h * 8 + 5] * inv);
-                                w.w = cvt_bf16x2(o[h * 8 + 6] * inv, o[h * 8 + 7] * inv);
-                            }
-                            *reinterpret_cast<uint4*>(dst + c + h * 8) = w;
-                        }
-                }
+                dst = live ? reinterpret_cast<uint8_t*>(a.out + uint64_t(im.S.q0 + token) * a.out_row + uint64_t(head) * a.out_head) : nullptr;
                 if (a.lse && live)
                     a.lse[uint64_t(im.S.q0 + token) * a.num_heads + head] = keys ? m * a.scale + logf(l) : -INFINITY;
+                l = inv;
             } else {
                 // a part: 2 * CTA when it continues a pair (or is the CTA's only one), 2 * CTA + 1 when it starts one
-                const uint64_t row = (uint64_t(2 * blockIdx.x + im.starts) * 2 + t) * 128 + r;
-                if (nt) {
-                    float4* dst = reinterpret_cast<float4*>(p.part + row * HP);
+                const uint64_t at = (uint64_t(2 * blockIdx.x + im.starts) * 2 + t) * 128 + r;
+                dst = nt ? reinterpret_cast<uint8_t*>(p.part + at * HP) : nullptr;
+                p.stat[at] = make_float2(m, nt ? l : 0.0f);
+            }
+            const uint32_t row_bytes = whole ? a.head_dim * 2 : HP * 4;
 #pragma unroll 1
-                    for (uint32_t c = 0; c < HP; c += 32) {
-                        float o[32];
-                        tmem_ld32(to + c, o);
-                        tmem_ld_wait();
+            for (uint32_t c = 0; c * 128 < row_bytes; ++c) {     // 64 columns of the result, or 32 of a part
+                uint4 w[8];
+                if (whole) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) dst[c / 4 + k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    for (int h = 0; h < 2; ++h) {
+                        float o[32];
+                        if (nt) {
+                            tmem_ld32(to + c * 64 + h * 32, o);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[h * 4 + k] = keys ? make_uint4(cvt_bf16x2(o[8 * k] * l, o[8 * k + 1] * l), cvt_bf16x2(o[8 * k + 2] * l, o[8 * k + 3] * l),
+                                                             cvt_bf16x2(o[8 * k + 4] * l, o[8 * k + 5] * l), cvt_bf16x2(o[8 * k + 6] * l, o[8 * k + 7] * l))
+                                                : make_uint4(0u, 0u, 0u, 0u);
                     }
+                } else if (nt) {
+                    float o[32];
+                    tmem_ld32(to + c * 32, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        w[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
                 }
-                p.stat[row] = make_float2(m, nt ? l : 0.0f);
+                __syncwarp();                    // (the last round's have been read)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) out[lane * 8 + (k ^ (lane & 7))] = w[k];
+                __syncwarp();
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const uint32_t from = g * 4 + row;
+                    uint8_t* at = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
+                    const uint32_t byte = c * 128 + piece * 16;
+                    if (at && byte < row_bytes) *reinterpret_cast<uint4*>(at + byte) = out[from * 8 + (piece ^ (from & 7))];
+                }
             }
             tc_fence_before();                   // (the sums have been read: the next pr says so)
             __syncwarp();
@@ -831,58 +936,70 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
 }
 
 // The parts of the cut pairs. grid (CTAs of the attention, 8): block (c, y)
-// does 32 of the 256 rows of the pair that CTA c is the first to continue,
-// a warp four rows: CTA c - 1 has its first part, c, c + 1, .. the others.
+// does 32 of the 256 rows of the pair that CTA c is the first to continue:
+// CTA c - 1 has its first part, c, c + 1, .. the others. A warp does four rows
+// side by side, eight lanes a row.
 template <int HP>
 __global__ void __launch_bounds__(256) k_packed_join(const PackedArgs p) {
+    __shared__ uint32_t list[1024];              // the parts' numbers (more CTAs than that no GPU has SMs for)
+    __shared__ uint32_t parts;
     pdl_release();
     pdl_acquire();
     const SmoeCudaPackedAttnArgs& a = p.a;
-    const uint32_t c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const PaPlace at = p.plan[c];
-    if (c == 0 || at.blk == 0) return;
+    const uint32_t c = blockIdx.x, tid = threadIdx.x;
+    const PaPlace at = p.plan[c], before = p.plan[c ? c - 1 : 0];
     auto same = [&](const PaPlace& x) { return x.kvh == at.kvh && x.seq == at.seq && x.tok == at.tok; };
-    const PaPlace before = p.plan[c - 1];
-    if (same(before) && before.blk) return;      // an earlier CTA continues this pair, too
-    uint32_t end = c + 1;                        // parts of CTAs c - 1 (its start) and c .. end - 1
-    while (end < gridDim.x) {
-        const PaPlace x = p.plan[end];
-        if (!same(x)) break;
-        ++end;
-    }
-    const PackedSeq S = packed_seq(a, at.seq);
-    constexpr int V = HP / 32;                   // columns of a lane
-    for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t row = blockIdx.y * 32 + warp * 4 + k, t = row / 128, r = row % 128;
-        const uint32_t token = at.tok + t * p.tokens + r / p.group, head = at.kvh * p.group + r % p.group;
-        if (r >= p.group * p.tokens || token >= S.len_q) continue;
-        const uint64_t row0 = (uint64_t(2 * (c - 1) + 1) * 2 + t) * 128 + r;   // of CTA c - 1; those after: 2 (c + i)
-        auto part = [&](uint32_t i) { return i == 0 ? row0 : (uint64_t(2 * (c + i - 1)) * 2 + t) * 128 + r; };
-        const uint32_t parts = end - c + 1;
-        // (a CTA whose share is empty has written nothing)
-        auto idle = [&](uint32_t i) { return i && same(p.plan[c + i]) && p.plan[c + i].blk == p.plan[c + i - 1].blk; };
-        float mx = -INFINITY, l = 0.0f, o[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = 0.0f;
-        for (uint32_t i = 0; i < parts; ++i)
-            if (!idle(i)) mx = fmaxf(mx, p.stat[part(i)].x);
-        for (uint32_t i = 0; i < parts; ++i) {
-            if (idle(i)) continue;
-            const float2 st = p.stat[part(i)];
-            if (st.x == -INFINITY && st.y == 0.0f) continue;     // no key in this part (its sums may not be written)
-            const float f = st.x == -INFINITY ? 1.0f : ex2((st.x - mx) * p.scale_log2);         // (-inf scores alone: NaN stays)
-            l = fmaf(st.y, f, l);
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] = fmaf(p.part[part(i) * HP + v * 32 + lane], f, o[v]);
+    if (c == 0 || at.blk == 0 || (same(before) && before.blk)) return;         // (an earlier CTA continues it, too)
+    if (tid == 0) {
+        uint32_t n = 0;
+        list[n++] = 2 * (c - 1) + 1;
+        PaPlace x = at;
+#pragma unroll 1
+        for (uint32_t e = c; e < gridDim.x && same(x) && n < 1024; ++e) {
+            const PaPlace y = p.plan[e + 1];
+            if (!(same(y) && y.blk == x.blk)) list[n++] = 2 * e;               // (a CTA whose share is empty has written nothing)
+            x = y;
         }
-        const bool keys = S.hi(token) > S.lo(token);
-        const float inv = keys ? 1.0f / l : 0.0f;
-        uint16_t* dst = a.out + uint64_t(S.q0 + token) * a.out_row + uint64_t(head) * a.out_head;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (v * 32 + lane < a.head_dim) dst[v * 32 + lane] = __bfloat16_as_ushort(__float2bfloat16_rn(keys ? o[v] * inv : 0.0f));
-        if (a.lse && lane == 0) a.lse[uint64_t(S.q0 + token) * a.num_heads + head] = keys ? mx * a.scale + logf(l) : -INFINITY;
+        parts = n;
     }
+    __syncthreads();
+    const PackedSeq S = packed_seq(a, at.seq);
+    const uint32_t row = blockIdx.y * 32 + tid / 8, t = row / 128, r = row % 128, q = tid % 8, n = parts;
+    const uint32_t token = at.tok + t * p.tokens + r / p.group, head = at.kvh * p.group + r % p.group;
+    if (r >= p.group * p.tokens || token >= S.len_q) return;
+    constexpr int V = HP / 32;                   // four columns a lane, V times
+    float mx = -INFINITY, l = 0.0f;
+    float4 o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; ++i) mx = fmaxf(mx, p.stat[(uint64_t(list[i]) * 2 + t) * 128 + r].x);
+#pragma unroll 2
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint64_t src = (uint64_t(list[i]) * 2 + t) * 128 + r;
+        const float2 st = p.stat[src];
+        const bool none = st.x == -INFINITY && st.y == 0.0f;     // no key in this part (its sums may not be written)
+        const float f = none ? 0.0f : st.x == -INFINITY ? 1.0f : ex2((st.x - mx) * p.scale_log2);     // (-inf scores alone: NaN stays)
+        l = fmaf(st.y, f, l);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (none) continue;
+            const float4 x = *reinterpret_cast<const float4*>(p.part + src * HP + v * 32 + q * 4);
+            o[v].x = fmaf(x.x, f, o[v].x);
+            o[v].y = fmaf(x.y, f, o[v].y);
+            o[v].z = fmaf(x.z, f, o[v].z);
+            o[v].w = fmaf(x.w, f, o[v].w);
+        }
+    }
+    const bool keys = S.hi(token) > S.lo(token);
+    const float inv = keys ? 1.0f / l : 0.0f;
+    uint16_t* dst = a.out + uint64_t(S.q0 + token) * a.out_row + uint64_t(head) * a.out_head;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (v * 32 + q * 4 < a.head_dim)         // (head_dim is a multiple of 8)
+            *reinterpret_cast<uint2*>(dst + v * 32 + q * 4) = keys ? make_uint2(cvt_bf16x2(o[v].x * inv, o[v].y * inv), cvt_bf16x2(o[v].z * inv, o[v].w * inv))
+                                                                   : make_uint2(0u, 0u);
+    if (a.lse && q == 0) a.lse[uint64_t(S.q0 + token) * a.num_heads + head] = keys ? mx * a.scale + logf(l) : -INFINITY;
 }
 
 }  // namespace smoe

@@ -46,13 +46,14 @@ SMOE_DEVINL bool elect_one() {
     return p != 0;
 }
 
-SMOE_DEVINL void serve_err(uint32_t* err, uint32_t code) { atomicCAS(err, 0u, code); }
+static __device__ __noinline__ void serve_err(uint32_t* err, uint32_t code) { atomicCAS(err, 0u, code); }
 
 // The sequence s with cu[s] <= row < cu[s + 1] (cu ascending, cu[0] = 0), by
 // one warp together: each step looks at 32 bounds, so 1024 sequences take
 // two dependent loads. n when there is none.
 SMOE_DEVINL uint32_t seq_of_row(const uint32_t* cu, uint32_t n, uint32_t row, uint32_t lane) {
     uint32_t lo = 0, span = n;           // the answer is in [lo, lo + span)
+#pragma unroll 1
     while (span > 1) {
         const uint32_t step = (span + 31) / 32, at = lo + min((lane + 1) * step, span);
         const uint32_t past = __ballot_sync(0xffffffffu, ld_plain(cu + at) <= row);   // bounds at or below the row
