@@ -23,8 +23,7 @@ namespace smoe {
 //  - few pairs: each CTA takes an equal share of the line of all pairs' key
 //    blocks, and the parts of a pair that is cut are joined by k_packed_join.
 constexpr uint32_t kPaRows = 128, kPaKeys = 128;
-constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA, MMA, items and checks, a warp each (a register split goes by four warps)
-constexpr int kPaPoly = 4;                        // every 4th pair of exponentials is a polynomial
+constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA, MMA, items and checks, a warp each
 constexpr int kPaItems = 2;                       // items that a CTA has at hand: the one in work and the next
 constexpr uint32_t kPaMaxPairs = 65536;          // tile pairs of a planned call (per KV head)
 
@@ -321,12 +320,6 @@ SMOE_DEVINL float tmem_ld1(uint32_t taddr) {
     return __uint_as_float(r);
 }
 SMOE_DEVINL void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// No multicast; x (element coordinate) a multiple of 64.
-SMOE_DEVINL void tma_load3(void* dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        :: "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
-}
 SMOE_DEVINL float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -349,57 +342,66 @@ SMOE_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-SMOE_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-// 2^x of two numbers without the exponential unit (16 results a cycle and SM,
-// half of what the tensor cores would need): x = n + f with n a whole number
-// and f in [-1/2, 1/2] (Cody and Waite), a polynomial of degree 4 in f fitted
-// for the smallest largest relative error (2.6e-6), times 2^n. Below -127 it is 0 (masked scores), a
-// NaN stays one.
-SMOE_DEVINL uint64_t ex2_poly(uint64_t x) {
-    float a, b;
-    unpack2(x, a, b);
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
-    x = pack2(a, b);
-    const float magic = 12582912.0f;             // 1.5 x 2^23: adding it rounds to a whole number, in the low bits
-    const uint64_t r = add2(x, pack2(magic, magic)), f = add2(x, mul2(add2(r, pack2(-magic, -magic)), pack2(-1.0f, -1.0f)));
-    uint64_t y = fma2(pack2(0.009570101f, 0.009570101f), f, pack2(0.05591786f, 0.05591786f));
-    y = fma2(y, f, pack2(0.24024744f, 0.24024744f));
-    y = fma2(y, f, pack2(0.6931218f, 0.6931218f));
-    y = fma2(y, f, pack2(0.9999993f, 0.9999993f));
-    float ra, rb;
-    unpack2(r, ra, rb);
-    const float sa = __uint_as_float(__float_as_uint(ra) * 8388608u + 0x3F800000u), sb = __uint_as_float(__float_as_uint(rb) * 8388608u + 0x3F800000u);
-    return mul2(y, pack2(sa, sb));
-}
 SMOE_DEVINL uint32_t cvt_bf16x2(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
+// Barriers and words in shared memory by their 32-bit addresses: the softmax
+// warps have no register to spare for generic pointers.
+struct Bar {
+    uint32_t a;
+    SMOE_DEVINL Bar operator+(uint32_t i) const { return {a + 8 * i}; }
+    SMOE_DEVINL void init(uint32_t count) const { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(a), "r"(count)); }
+    SMOE_DEVINL void arrive() const { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(a) : "memory"); }
+    SMOE_DEVINL void expect(uint32_t bytes) const {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(a), "r"(bytes) : "memory");
+    }
+    SMOE_DEVINL void commit() const {            // arrives when all products issued so far are done
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(a) : "memory");
+    }
+    SMOE_DEVINL bool try_wait(uint32_t parity) const {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+        return ok != 0;
+    }
+};
+struct Word {
+    uint32_t a;
+    SMOE_DEVINL Word operator+(uint32_t i) const { return {a + 4 * i}; }
+    SMOE_DEVINL uint32_t get() const {
+        uint32_t v;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+        return v;
+    }
+    SMOE_DEVINL void set(uint32_t v) const { asm volatile("st.volatile.shared.u32 [%0], %1;" :: "r"(a), "r"(v) : "memory"); }
+};
 // A bounded wait, small enough to be inlined at each place (a call would
 // bring the calling convention's registers into the softmax warps' budget):
 // some tenths of a second of polls. After one ran out, all others of the CTA
 // give up within 256; the roles then finish on whatever the buffers hold
 // (every address stays in the CTA's own memory) and the error word is set.
 constexpr uint32_t kPaPolls = 1u << 24;
-SMOE_DEVINL void pa_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* fail, uint32_t* err) {
+SMOE_DEVINL void pa_wait(Bar bar, uint32_t parity, Word fail, uint32_t* err) {
 #pragma unroll 1
-    for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i)
-        if ((i & 255) == 255 && (*fail || i >= kPaPolls)) {
-            *fail = 1u;
+    for (uint32_t i = 0; !bar.try_wait(parity); ++i)
+        if ((i & 255) == 255 && (fail.get() || i >= kPaPolls)) {
+            fail.set(1u);
             atomicCAS(err, 0u, uint32_t(SMOE_DEVERR_MBAR_TIMEOUT));
             break;
         }
 }
 // The same regardless of earlier failures: for copies and products in flight.
-SMOE_DEVINL void pa_drain(uint64_t* bar, uint32_t parity) {
+SMOE_DEVINL void pa_drain(Bar bar, uint32_t parity) {
 #pragma unroll 1
-    for (uint32_t i = 0; i < kPaPolls && !mbar_try_wait(bar, parity); ++i) {}
+    for (uint32_t i = 0; i < kPaPolls && !bar.try_wait(parity); ++i) {}
+}
+// No multicast; x (element coordinate) a multiple of 64.
+SMOE_DEVINL void tma_load3(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, Bar bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar.a) : "memory");
 }
 
 template <int HP>
@@ -411,37 +413,38 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     constexpr uint32_t TMEM_O = 256;             // columns: S of tile 0, S of tile 1, O of tile 0, O of tile 1
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR);
-    uint64_t *qf = bars, *qe = bars + 2, *sf = bars + 4, *pr = bars + 6, *pl = bars + 8, *of = bars + 10, *vc = bars + 12, *itf = bars + 16, *ite = itf + kPaItems, *xb = ite + kPaItems, *kvf = xb + 3, *kve = kvf + ST;
-    uint32_t* words = reinterpret_cast<uint32_t*>(kve + ST);
-    PaItem* items = reinterpret_cast<PaItem*>(smem + SM::ITEMS);
-    volatile uint32_t *fail = words, *begun = words + 1;         // begun[t]: the accumulator holds something before block 0's P V
-    uint32_t* tslot = words + 3;
-    volatile uint32_t* odds = words + 6;                         // [4] of the last masked blocks: its values hold an infinity or NaN
+    const uint32_t base = smem_u32(smem);
+    const Bar qf{base + SM::BAR}, qe = qf + 2, sf = qf + 4, pr = qf + 6, pl = qf + 8, of = qf + 10, vc = qf + 12, itf = qf + 16, ite = itf + kPaItems,
+              xb = ite + kPaItems, kvf = xb + 3, kve = kvf + ST;
+    const Word fail{(kve + ST).a}, begun = fail + 1, odds = fail + 4;          // begun[t]: the accumulator holds something before block 0's P V
+    uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + SM::BAR + ((kve + ST).a - qf.a)) + 3;  // odds[4]: of the last masked blocks: its values hold an infinity or NaN
+    PaItem* const items = reinterpret_cast<PaItem*>(smem + SM::ITEMS);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const SmoeCudaPackedAttnArgs& a = p.a;
 
     pdl_release();
     if (warp == 8 && lane == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(qf + i, 1);
-            mbar_init(qe + i, 1);
-            mbar_init(sf + i, 1);
-            mbar_init(pr + i, 4);
-            mbar_init(pl + i, 4);
-            mbar_init(of + i, 1);
+            (qf + i).init(1);
+            (qe + i).init(1);
+            (sf + i).init(1);
+            (pr + i).init(4);
+            (pl + i).init(4);
+            (of + i).init(1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(vc + i, 1);
+        for (int i = 0; i < 4; ++i) (vc + i).init(1);
         for (int i = 0; i < kPaItems; ++i) {
-            mbar_init(itf + i, 1);
-            mbar_init(ite + i, 11);              // the TMA lane, the MMA lane, the checking warp, eight softmax warps
+            (itf + i).init(1);
+            (ite + i).init(11);              // the TMA lane, the MMA lane, the checking warp, eight softmax warps
         }
-        for (int i = 0; i < 3; ++i) mbar_init(xb + i, i < 2 ? 4 : 8);
+        for (int i = 0; i < 3; ++i) (xb + i).init(i < 2 ? 4 : 8);
         for (int i = 0; i < ST; ++i) {
-            mbar_init(kvf + i, 1);
-            mbar_init(kve + i, 1 + i % 2);       // the MMA lane; of values (odd stages), the checking warp, too
+            (kvf + i).init(1);
+            (kve + i).init(1 + i % 2);       // the MMA lane; of values (odd stages), the checking warp, too
         }
-        *fail = begun[0] = begun[1] = 0u;
+        fail.set(0u);
+        begun.set(0u);
+        (begun + 1).set(0u);
         fence_mbar_init();
     }
     if (warp == 9) tmem_alloc(tslot, 512);
@@ -451,22 +454,19 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tslot;
-    auto wait = [&](uint64_t* b, uint32_t ph) { pa_wait(b, ph & 1, fail, p.err); };
+    auto wait = [&](Bar b, uint32_t ph) { pa_wait(b, ph & 1, fail, p.err); };
     // item k, of a role; and done with it
     auto item = [&](uint32_t k) -> const PaItem& {
         wait(itf + k % kPaItems, k / kPaItems);
         return items[k % kPaItems];
     };
-    auto item_done = [&](uint32_t k) { mbar_arrive(ite + k % kPaItems); };
-    // 384 threads start with 168 registers: 256 x 208 + 128 x 80 of them
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    auto item_done = [&](uint32_t k) { (ite + k % kPaItems).arrive(); };
     if (warp == 8) {
         // ---------------------------------------------------- loads (one lane)
         if (elect_one()) {
             uint32_t j = 0, nq[2] = {0u, 0u};    // units sent for, Q tiles sent for
 #pragma unroll 1
-            for (uint32_t k = 0; !*fail; ++k) {
+            for (uint32_t k = 0; !fail.get(); ++k) {
                 const PaItem& it = item(k);
                 if (!it.more) break;
                 const uint32_t m = max(it.cnt[0], it.cnt[1]), kvh = it.kvh, row_q = it.S.q0 + it.tok, row_k = it.S.k0 + it.key0;
@@ -477,15 +477,15 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     if (i < 2 && (i ? cnt[1] : cnt[0])) {
                         const uint32_t q = i ? nq[1]++ : nq[0]++;
                         if (q) wait(qe + i, q - 1);
-                        mbar_arrive_expect_tx(qf + i, p.group * p.tokens * 128 * NH);
+                        (qf + i).expect(p.group * p.tokens * 128 * NH);
                         for (int h = 0; h < NH; ++h)
-                            tma_load3(smem + SM::Q + i * SM::TILE + h * 16384, &mq, h * 64, kvh * p.group, row_q + i * p.tokens, qf + i);
+                            tma_load3(base + SM::Q + i * SM::TILE + h * 16384, &mq, h * 64, kvh * p.group, row_q + i * p.tokens, qf + i);
                     }
                     const uint32_t st = j % ST, round = j / ST;
                     if (round) wait(kve + st, round - 1);
-                    mbar_arrive_expect_tx(kvf + st, SM::TILE);
+                    (kvf + st).expect(SM::TILE);
                     for (int h = 0; h < NH; ++h)
-                        tma_load3(smem + SM::KV + st * SM::TILE + h * 16384, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
+                        tma_load3(base + SM::KV + st * SM::TILE + h * 16384, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
                 }
             }
             // nothing may be in flight when the CTA ends (the MMA warp has
@@ -499,7 +499,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         // ------------------------------------------------------ MMA (one lane)
         if (elect_one()) {
             constexpr uint32_t IQK = tc_idesc_bf16(128, 128, 0), IPV = tc_idesc_bf16(128, HP, 1);
-            const uint32_t sq = smem_u32(smem + SM::Q), skv = smem_u32(smem + SM::KV);
+            const uint32_t sq = base + SM::Q, skv = base + SM::KV;
             uint32_t j0 = 0, nq[2] = {0u, 0u}, nb[2] = {0u, 0u}; // units, Q tiles, blocks of each tile so far
             auto qk = [&](uint32_t t, uint32_t st, bool last) {
                 const uint64_t qd = tc_desc_sw128(sq + t * SM::TILE, 16), kd = tc_desc_sw128(skv + st * SM::TILE, 16);
@@ -508,8 +508,8 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     const uint32_t o = (s / 4 * 16384 + s % 4 * 32) >> 4;
                     tc_mma_f16(tmem + t * 128, qd + o, kd + o, IQK, s > 0);
                 }
-                tc_commit(sf + t);
-                if (last) tc_commit(qe + t);     // the tile's Q has been read
+                (sf + t).commit();
+                if (last) (qe + t).commit();     // the tile's Q has been read
             };
             auto pv = [&](uint32_t t, uint32_t st, bool more, uint32_t block) {
                 const uint64_t vd = tc_desc_sw128(skv + st * SM::TILE, 16384);
@@ -521,10 +521,10 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     }
                     tc_mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + s * 8, vd + ((s * 2048) >> 4), IPV, more || s > 0);
                 }
-                tc_commit(of + t);
+                (of + t).commit();
             };
 #pragma unroll 1
-            for (uint32_t k = 0; !*fail; ++k) {
+            for (uint32_t k = 0; !fail.get(); ++k) {
                 const PaItem& it = item(k);
                 if (!it.more) break;
                 const uint32_t c0 = it.cnt[0], c1 = it.cnt[1], m = max(c0, c1);
@@ -538,7 +538,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                             tc_fence_after();
                             qk(t, j0 % ST, (t ? c1 : c0) == 1);
                         }
-                    tc_commit(kve + j0 % ST);
+                    (kve + j0 % ST).commit();
                 }
 #pragma unroll 1
                 for (uint32_t i = 0; i < m; ++i) {
@@ -553,12 +553,12 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                             // softmax warps have read the last item's sums)
                             wait(pr + t, nb[t]);
                             tc_fence_after();
-                            pv(t, sv, i > 0 || begun[t], nb[t]++);
+                            pv(t, sv, i > 0 || (begun + t).get(), nb[t]++);
                         }
                         if (i + 1 < nt) qk(t, sk, i + 2 == nt);
                     }
-                    tc_commit(kve + sv);
-                    if (i + 1 < m) tc_commit(kve + sk);
+                    (kve + sv).commit();
+                    if (i + 1 < m) (kve + sk).commit();
                 }
                 j0 += 2 * m;
             }
@@ -611,7 +611,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (elect_one()) {
             bool more = true;
 #pragma unroll 1
-            for (uint32_t k = 0; more && !*fail; ++k) {
+            for (uint32_t k = 0; more && !fail.get(); ++k) {
                 PaItem it{};
                 if (k >= kPaItems) wait(ite + k % kPaItems, k / kPaItems - 1);
                 if (p.list) {
@@ -624,10 +624,10 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 more = walk.next(p, it);
                 it.more = more;
                 items[k % kPaItems] = it;
-                mbar_arrive(itf + k % kPaItems);
+                (itf + k % kPaItems).arrive();
             }
         }
-    } else {
+    } else if (warp == 11) {
         // ------------------------------------------------- checks (one warp)
         // Values of blocks that not every row may see all of: is there an
         // infinity or NaN?
@@ -635,14 +635,14 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll 1
         for (uint32_t k = 0;; ++k) {
             const PaItem& it = item(k);
-            if (__any_sync(0xffffffffu, *fail || !it.more)) break;
+            if (__any_sync(0xffffffffu, fail.get() || !it.more)) break;
             const uint32_t m = max(it.cnt[0], it.cnt[1]);
 #pragma unroll 1
             for (uint32_t i = 0; i < m; ++i) {
                 const uint32_t jv = j0 + 2 * i + 1;
                 wait(kvf + jv % ST, jv / ST);    // (all of them in turn: a phase skipped could be taken for another)
                 if (!pa_masked(it, i)) {
-                    if (lane == 0) mbar_arrive(kve + jv % ST);
+                    if (lane == 0) (kve + jv % ST).arrive();
                     continue;
                 }
                 const uint4* v = reinterpret_cast<const uint4*>(smem + SM::KV + jv % ST * SM::TILE) + lane;
@@ -662,9 +662,9 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 if (lane == 0) {
                     // (At most four V tiles are in the ring, so of the masked block four
                     // back all products are done: the softmax warps have read its flag.)
-                    odds[nm % 4] = odd;
-                    mbar_arrive(vc + nm % 4);
-                    mbar_arrive(kve + jv % ST);
+                    (odds + nm % 4).set(odd);
+                    (vc + nm % 4).arrive();
+                    (kve + jv % ST).arrive();
                 }
                 ++nm;
             }
@@ -672,12 +672,11 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
             __syncwarp();
             if (lane == 0) item_done(k);
         }
-    }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ----------------------------------------------------------- softmax
-        // One thread a row: the scores of a block come from tensor memory
-        // as 128 registers. The reference maximum is only moved when the
+        // One thread a row, which reads its scores twice, 32 at a time with the
+        // next 32 on their way: for the maximum and for the exponentials. (All
+        // 128 at once left the loop without registers.) The reference maximum is only moved when the
         // running one is more than 8 (in log2) above it, so the
         // accumulator is rarely rescaled; probabilities stay below 2^8.
         const uint32_t t = warp >> 2, r = tid & 127;
@@ -692,14 +691,14 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         auto meet = [&](bool all) {
             const uint32_t x = all ? 2u : t, turn = all ? met[1]++ : met[0]++;
             __syncwarp();
-            if (lane == 0) mbar_arrive(xb + x);
+            if (lane == 0) (xb + x).arrive();
             wait(xb + x, turn);
             __syncwarp();
         };
 #pragma unroll 1
         for (uint32_t k = 0;; ++k) {
             const PaItem& im = item(k);
-            if (__any_sync(0xffffffffu, *fail || !im.more)) break;
+            if (__any_sync(0xffffffffu, fail.get() || !im.more)) break;
             const uint32_t nt = im.cnt[t];
             const bool live = r < p.group * p.tokens && im.tok + t * p.tokens + tk < im.S.len_q;
             float m = -INFINITY, l = 0.0f;
@@ -711,35 +710,32 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 for (uint32_t i = 0; i < nt; ++i) {
                     const uint32_t key0 = first_key + i * kPaKeys, jv = j0 + 2 * i + 1;
                     const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;   // (pa_masked)
-                    float s[128];
-                    wait(sf + t, nb + i);
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
-                    tmem_ld_wait();
-                    bool odd = false;            // this block's values hold an infinity or NaN
                     const uint32_t ja = lo > key0 ? lo - key0 : 0u, jb = hi > key0 ? hi - key0 : 0u;       // columns [ja, jb)
                     uint4* const vt = reinterpret_cast<uint4*>(smem + SM::KV + jv % ST * SM::TILE);
-                    if (masked) {
+                    float x[2][32];              // 32 scores at hand, the next 32 on their way
+                    auto hide = [&](float* y, int c) {           // those of columns 32 c .. that the row may not see
+                        auto below = [](uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+                        const uint32_t from = ja > c * 32u ? ja - c * 32u : 0u, to_ = jb > c * 32u ? jb - c * 32u : 0u, open = below(to_) & ~below(from);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {            // bits of the 32 columns in [ja, jb)
-                            auto below = [](uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-                            const uint32_t from = ja > c * 32u ? ja - c * 32u : 0u, to_ = jb > c * 32u ? jb - c * 32u : 0u, open = below(to_) & ~below(from);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!(open >> j & 1u)) s[c * 32 + j] = -INFINITY;
-                        }
-                        // A zero probability does not silence an infinity or NaN
-                        // in the matrix product, and this block has keys that
-                        // not every row may see: was there one?
-                        wait(vc + nm % 4, nm / 4);
-                        odd = __any_sync(0xffffffffu, odds[nm++ % 4]);
-                    }
+                        for (int j = 0; j < 32; ++j)
+                            if (!(open >> j & 1u)) y[j] = -INFINITY;
+                    };
+                    wait(sf + t, nb + i);
+                    tc_fence_after();
+                    tmem_ld32(ts, x[0]);
+                    tmem_ld_wait();
                     float mq[8];                 // eight chains: the maximum's latency is the softmax warps' to wait for
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mq[j] = fmaxf(s[2 * j], s[2 * j + 1]);
+                    for (int j = 0; j < 8; ++j) mq[j] = -INFINITY;
 #pragma unroll
-                    for (int j = 16; j < 128; j += 2) mq[j / 2 % 8] = fmaxf(fmaxf(mq[j / 2 % 8], s[j]), s[j + 1]);
+                    for (int c = 0; c < 4; ++c) {
+                        float* y = x[c & 1];
+                        tmem_ld32(ts + (c + 1) % 4 * 32, x[(c + 1) & 1]);        // (after the last the first again, for the exponentials)
+                        if (masked) hide(y, c);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) mq[j / 2 % 8] = fmaxf(fmaxf(mq[j / 2 % 8], y[j]), y[j + 1]);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
                     for (int w = 4; w; w >>= 1)
 #pragma unroll
@@ -767,36 +763,42 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         l *= f;
                         if (move) m = mx;
                     }
+                    // A zero probability does not silence an infinity or NaN
+                    // among the values in the matrix product, and a masked block
+                    // has keys that not every row may see: was there one?
+                    bool odd = false;
+                    if (masked) {
+                        wait(vc + nm % 4, nm / 4);
+                        odd = __any_sync(0xffffffffu, (odds + nm++ % 4).get());
+                    }
                     const float ml = m == -INFINITY ? 0.0f : m * sl;
                     const uint64_t sl2 = pack2(sl, sl), ml2 = pack2(-ml, -ml);
                     uint64_t sums[2] = {0ull, 0ull};
-                    if (i == 0 && r == 0) begun[t] = odd;        // the product then adds to what the rows put there
-                    auto give = [&](uint64_t* b) {               // what this warp has put into tensor memory, to the MMA warp
+                    if (i == 0 && r == 0) (begun + t).set(odd);        // the product then adds to what the rows put there
+                    auto give = [&](Bar b) {               // what this warp has put into tensor memory, to the MMA warp
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(b);
+                        if (lane == 0) b.arrive();
                     };
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        float* y = x[c & 1];
+                        if (c < 3) tmem_ld32(ts + (c + 1) * 32, x[(c + 1) & 1]);
+                        if (masked) hide(y, c);
                         uint32_t w[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const uint64_t z = fma2(pack2(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1]), sl2, ml2);
-                            float x, y;
-                            if (k % kPaPoly == kPaPoly - 1) {
-                                unpack2(ex2_poly(z), x, y);
-                            } else {
-                                unpack2(z, x, y);
-                                x = ex2(x);
-                                y = ex2(y);
-                            }
-                            sums[k % 2] = add2(sums[k % 2], pack2(x, y));
-                            w[k] = cvt_bf16x2(x, y);
+                            float u, v;
+                            unpack2(fma2(pack2(y[2 * k], y[2 * k + 1]), sl2, ml2), u, v);
+                            u = ex2(u);
+                            v = ex2(v);
+                            sums[k % 2] = add2(sums[k % 2], pack2(u, v));
+                            w[k] = cvt_bf16x2(u, v);
                         }
-                        tmem_st16(ts + c * 16, w);
-                        // three quarters of the block's product can start
-                        if (c == 2 && !odd) give(pr + t);
+                        if (c < 3) tmem_ld_wait();
+                        tmem_st16(ts + c * 16, w);               // (over scores that have been read)
+                        if (c == 2 && !odd) give(pr + t);        // three quarters of the block's product can start
                     }
                     if (odd) {
                         // Rare. Each row adds its own share of the infinities and
