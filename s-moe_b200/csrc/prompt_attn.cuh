@@ -863,15 +863,13 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     give(pl + t);
                 }
                 nb += nt;
-                wait(of + t, nb - 1);
-                tc_fence_after();
             }
             for (uint32_t i = nt; i < im.cnt[t ^ 1]; ++i) nm += pa_masked(im, i);
             j0 += 2 * max(im.cnt[0], im.cnt[1]);
-            const uint32_t token = im.tok + t * p.tokens + tk, head = im.kvh * p.group + hd;
             // Rows go out through shared memory, 128 bytes of each at a time:
             // eight lanes a row, four whole lines an instruction (a thread
             // storing its own row touches 32 lines with each).
+            const uint32_t token = im.tok + t * p.tokens + tk, head = im.kvh * p.group + hd;
             const bool whole = im.whole, keys = live && im.S.hi(token) > im.S.lo(token);
             uint4* const out = reinterpret_cast<uint4*>(smem + SM::OUT) + warp * 256;
             const uint32_t row = lane / 8, piece = lane % 8;
@@ -887,6 +885,10 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 const uint64_t at = (uint64_t(2 * blockIdx.x + im.starts) * 2 + t) * 128 + r;
                 dst = nt ? reinterpret_cast<uint8_t*>(p.part + at * HP) : nullptr;
                 p.stat[at] = make_float2(m, nt ? l : 0.0f);
+            }
+            if (nt) {
+                wait(of + t, nb - 1);
+                tc_fence_after();
             }
             const uint32_t row_bytes = whole ? a.head_dim * 2 : HP * 4;
 #pragma unroll 1
@@ -918,13 +920,17 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll
                 for (int k = 0; k < 8; ++k) out[lane * 8 + (k ^ (lane & 7))] = w[k];
                 __syncwarp();
+                uint8_t* at[8];
+                const uint32_t byte = c * 128 + piece * 16;
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     const uint32_t from = g * 4 + row;
-                    uint8_t* at = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
-                    const uint32_t byte = c * 128 + piece * 16;
-                    if (at && byte < row_bytes) *reinterpret_cast<uint4*>(at + byte) = out[from * 8 + (piece ^ (from & 7))];
+                    at[g] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
+                    w[g] = out[from * 8 + (piece ^ (from & 7))];
                 }
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                    if (at[g] && byte < row_bytes) *reinterpret_cast<uint4*>(at[g] + byte) = w[g];
             }
             tc_fence_before();                   // (the sums have been read: the next pr says so)
             __syncwarp();
