@@ -39,95 +39,224 @@ SMOE_DEVINL uint32_t kv4_page(const SmoeKv4Cache& c, uint32_t s, uint64_t e, uin
 }
 
 // ------------------------------------------------------------ append and read
-// One half-warp per (row, KV head, K or V, group of 64): 4 values a lane, the
-// group's minimum and maximum by four shuffles, 4 codes (2 bytes) a lane, so a
-// group's loads (128 or 256 bytes) and stores (32) are whole sectors. A warp
-// takes two units of one row; the rows of a CTA are consecutive.
-SMOE_DEVINL float4 kv4_load4(const void* p, size_t at, int dtype) {
-    if (dtype == SMOE_DTYPE_F32) return *(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
-    const uint2 u = *(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                       __uint_as_float(u.y & 0xffff0000u));
+// A CTA takes 8 rows: a warp finds each one's entry (sequence, page, slot), and
+// four lanes do a unit - a group of 64 values of a row, KV head and side - 16
+// values a lane: the group's 32 bytes of codes are 8 a lane, its minimum and
+// maximum two shuffles. Values are fetched before the entries are known, and
+// two units a lane are in flight. Bound by the chain of look-ups (bounds,
+// length, page table) for a step's rows and by the bytes for a prompt's.
+constexpr int kKwRows = 8, kKwThreads = 256;
+
+struct Kv4RowPlace {
+    uint32_t page, slot, pos;                    // page ~0: nowhere
+};
+// The places of the CTA's rows, a warp a row; entry = base[s] + index in the sequence.
+SMOE_DEVINL void kv4_places(const Kv4Args& a, const SmoeKv4Rows& r, const uint32_t* base, Kv4RowPlace* places) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kKwRows + warp, ns = a.c.n_seqs;
+    Kv4RowPlace p{~0u, 0u, 0u};
+    if (row < r.total) {
+        // (a decode step has a row a sequence: look there first)
+        uint32_t s = ns;
+        if (row < ns && ld_plain(r.cu + row) <= row && row < ld_plain(r.cu + row + 1)) s = row;
+        else s = seq_of_row(r.cu, ns, row, lane);
+        if (s < ns) {                            // (else: a row past the last sequence)
+            const uint32_t t = row - ld_plain(r.cu + s);
+            const uint64_t e = uint64_t(base ? ld_plain(base + s) : 0u) + t;
+            if (a.c.pos) p.pos = ld_plain((a.c.seen ? a.c.seen : a.c.len) + s) + t;
+            p.page = kv4_page(a.c, s, e, a.err);
+            p.slot = uint32_t(e % kKvPage);
+        }
+    }
+    if (lane == 0) places[warp] = p;
+    __syncthreads();
 }
 
-__global__ void __launch_bounds__(256) k_kv4_append(Kv4Args a, SmoeKv4Rows r) {
-    pdl_release();
-    pdl_acquire();
-    const Kv4Geom G(a.c.head_dim);
-    const uint32_t lane = threadIdx.x & 31, hl = lane & 15;
-    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= r.total) return;
-    const uint32_t s = seq_of_row(r.cu, a.c.n_seqs, row, lane);
-    if (s >= a.c.n_seqs) return;                 // rows past the last sequence
-    const uint32_t t = row - ld_plain(r.cu + s);
-    const uint64_t e = uint64_t(ld_plain(a.c.len + s)) + t;
-    const uint32_t page = kv4_page(a.c, s, e, a.err);
-    if (page == ~0u) return;
-    const uint32_t slot = uint32_t(e % kKvPage), units = a.c.num_kv_heads * 2 * G.ng;
-    for (uint32_t u = lane >> 4; u < units; u += 2) {
-        const uint32_t g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
-        const size_t at = kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head;
-        const float4 x = kv4_load4(kv ? r.v : r.k, at + g * 64 + hl * 4, r.dtype);
-        float lo = fminf(fminf(x.x, x.y), fminf(x.z, x.w)), hi = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-        const uint32_t m = lane < 16 ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-        for (int o = 8; o; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(m, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(m, hi, o));
-        }
-        const __nv_bfloat16 bb = __float2bfloat16_rn(lo);
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-        const float bias = __bfloat162float(bb), scale = __bfloat162float(sb);
-        const float xs[4] = {x.x, x.y, x.z, x.w};
-        uint32_t code = 0;
+// 16 values of a row, in pieces of 16 bytes, or of 8 where a bf16 row may start between two such.
+template <int DTYPE, bool WIDE>
+SMOE_DEVINL void kv4_load16(const void* p, size_t at, float* x) {
+    if (DTYPE == SMOE_DTYPE_F32) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float q = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(xs[i], bias), scale)) : 0.0f;
-            code |= uint32_t(fminf(fmaxf(q, 0.0f), 15.0f)) << (4 * i);
+            const float4 v = ld_plain(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at) + i);
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
         }
-        uint8_t* blk = a.c.blocks + (size_t(page) * a.c.num_kv_heads + h) * G.block;
-        *reinterpret_cast<uint16_t*>(blk + G.codes(kv, g) + slot * 32 + hl * 2) = uint16_t(code);
-        if (hl == 0) {
-            *reinterpret_cast<uint32_t*>(blk + G.sb(kv, g) + slot * 4) =
-                uint32_t(__bfloat16_as_ushort(sb)) | uint32_t(__bfloat16_as_ushort(bb)) << 16;
-            if (kv == 0 && g == 0) {
-                const size_t i = (size_t(page) * a.c.num_kv_heads + h) * kKvPage + slot;
-                if (a.c.pos) a.c.pos[i] = ld_plain((a.c.seen ? a.c.seen : a.c.len) + s) + t;
-                if (a.c.score) a.c.score[i] = 0.0f;
-            }
+        return;
+    }
+    uint32_t w[8];
+    if (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 v = ld_plain(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at) + i);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint2 v = ld_plain(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at) + i);
+            w[2 * i] = v.x;
+            w[2 * i + 1] = v.y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
 
-__global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* first, SmoeKv4Rows r) {
+// The code of one value by the definition.
+static __device__ __noinline__ uint32_t kv4_code(float x, float bias, float scale) {
+    const float q = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x, bias), scale)) : 0.0f;
+    return uint32_t(fminf(fmaxf(q, 0.0f), 15.0f));
+}
+// Those of 16 values, without dividing: with d = x - bias, the code nearest to
+// d / scale by way of the reciprocal is right or off by one. r scale (4 + 8
+// bits) and u = d - r scale are exact, so 2 |u| against scale says which, ties
+// included: fl(d / scale) is exactly half-way only where d is (2 r + 1) scale / 2
+// - neighbours of that number in fp32 are further from it than half a unit of
+// the quotient. (bf16 values hit ties often: some in every second warp.)
+SMOE_DEVINL void kv4_codes16(const float* y, float bias, float scale, uint32_t* code) {
+    code[0] = code[1] = 0u;
+    if (!(scale >= 1e-37f)) {                    // no finite reciprocal, or no positive scale
+        if (scale > 0.0f)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) code[k / 8] |= kv4_code(y[k], bias, scale) << (4 * (k % 8));
+        return;
+    }
+    const float inv = 1.0f / scale, magic = 12582912.0f;         // 1.5 x 2^23: adding it rounds to a whole number, in the low bits
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const float d = __fsub_rn(y[k], bias), t = fminf(fmaxf(d * inv, 0.0f), 15.0f) + magic;
+        const float u = fmaf(-(t - magic), scale, d), v = fabsf(u + u);
+        const uint32_t r = __float_as_uint(t) & 15u;
+        const bool off = v > scale || (v == scale && (r & 1u));
+        const int c = int(r) + (off ? (u > 0.0f ? 1 : -1) : 0);
+        code[k / 8] |= uint32_t(max(0, min(15, c))) << (4 * (k % 8));
+    }
+}
+
+template <int DTYPE, bool WIDE>
+__global__ void __launch_bounds__(kKwThreads, 4) k_kv4_append(Kv4Args a, SmoeKv4Rows r) {
+    __shared__ Kv4RowPlace places[kKwRows];
     pdl_release();
     pdl_acquire();
     const Kv4Geom G(a.c.head_dim);
-    const uint32_t lane = threadIdx.x & 31, hl = lane & 15;
-    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= r.total) return;
-    const uint32_t s = seq_of_row(r.cu, a.c.n_seqs, row, lane);
-    if (s >= a.c.n_seqs) return;
-    const uint64_t e = uint64_t(first ? ld_plain(first + s) : 0u) + (row - ld_plain(r.cu + s));
-    const uint32_t page = kv4_page(a.c, s, e, a.err);
-    if (page == ~0u) return;
-    const uint32_t slot = uint32_t(e % kKvPage), units = a.c.num_kv_heads * 2 * G.ng;
-    for (uint32_t u = lane >> 4; u < units; u += 2) {
-        const uint32_t g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
-        const uint8_t* blk = a.c.blocks + (size_t(page) * a.c.num_kv_heads + h) * G.block;
-        const uint32_t code = *reinterpret_cast<const uint16_t*>(blk + G.codes(kv, g) + slot * 32 + hl * 2);
-        const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + G.sb(kv, g) + slot * 4);
-        const float scale = __uint_as_float(sb << 16), bias = __uint_as_float(sb & 0xffff0000u);
-        float v[4];
+    const uint32_t quad = threadIdx.x >> 2, j = threadIdx.x & 3, units = a.c.num_kv_heads * 2 * G.ng, row0 = blockIdx.x * kKwRows;
+    const uint32_t all = min(uint32_t(kKwRows), r.total - row0) * units;
+    constexpr uint32_t STEP = kKwThreads / 4;
+    float x[2][16];
+    auto load = [&](uint32_t i, float* y) {
+        const uint32_t row = row0 + i / units, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
+        kv4_load16<DTYPE, WIDE>(kv ? r.v : r.k, (kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head) + g * 64 + j * 16, y);
+    };
+    auto store = [&](uint32_t i, const float* y) {
+        const uint32_t u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
+        const Kv4RowPlace p = places[i / units];
+        float lo = y[0], hi = y[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(__fmul_rn(float(code >> (4 * i) & 15u), scale), bias);
-        const size_t at = (kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head) + g * 64 + hl * 4;
-        void* dst = kv ? r.v : r.k;
-        if (r.dtype == SMOE_DTYPE_F32)
-            *reinterpret_cast<float4*>(static_cast<float*>(dst) + at) = make_float4(v[0], v[1], v[2], v[3]);
-        else
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + at) =
-                make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        for (int k = 1; k < 16; ++k) {
+            lo = fminf(lo, y[k]);
+            hi = fmaxf(hi, y[k]);
+        }
+        const uint32_t mask = 0xfu << (threadIdx.x & 28);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+        }
+        if (p.page == ~0u) return;
+        const __nv_bfloat16 bb = __float2bfloat16_rn(lo);
+        const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+        const float bias = __bfloat162float(bb), scale = __bfloat162float(sb);
+        uint32_t code[2];
+        kv4_codes16(y, bias, scale, code);
+        uint8_t* blk = a.c.blocks + (size_t(p.page) * a.c.num_kv_heads + h) * G.block;
+        *reinterpret_cast<uint2*>(blk + G.codes(kv, g) + p.slot * 32 + j * 8) = make_uint2(code[0], code[1]);
+        if (j == 0) {
+            *reinterpret_cast<uint32_t*>(blk + G.sb(kv, g) + p.slot * 4) =
+                uint32_t(__bfloat16_as_ushort(sb)) | uint32_t(__bfloat16_as_ushort(bb)) << 16;
+            if (kv == 0 && g == 0) {
+                const size_t at = (size_t(p.page) * a.c.num_kv_heads + h) * kKvPage + p.slot;
+                if (a.c.pos) a.c.pos[at] = p.pos;
+                if (a.c.score) a.c.score[at] = 0.0f;
+            }
+        }
+    };
+    if (quad < all) load(quad, x[0]);
+    if (quad + STEP < all) load(quad + STEP, x[1]);
+    kv4_places(a, r, a.c.len, places);
+#pragma unroll 1
+    for (uint32_t i = quad; i < all; i += STEP) {
+        store(i, x[0]);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[0][k] = x[1][k];
+        if (i + 2 * STEP < all) load(i + 2 * STEP, x[1]);
+    }
+}
+
+template <int DTYPE, bool WIDE>
+__global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32_t* first, SmoeKv4Rows r) {
+    __shared__ Kv4RowPlace places[kKwRows];
+    pdl_release();
+    pdl_acquire();
+    const Kv4Geom G(a.c.head_dim);
+    const uint32_t quad = threadIdx.x >> 2, j = threadIdx.x & 3, units = a.c.num_kv_heads * 2 * G.ng, row0 = blockIdx.x * kKwRows;
+    const uint32_t all = min(uint32_t(kKwRows), r.total - row0) * units;
+    constexpr uint32_t STEP = kKwThreads / 4;
+    kv4_places(a, r, first, places);
+#pragma unroll 1
+    for (uint32_t i0 = quad; i0 < all; i0 += 2 * STEP) {
+        uint2 code[2];
+        uint32_t sb[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t i = i0 + q * STEP, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
+            code[q] = make_uint2(0u, 0u);
+            sb[q] = 0u;
+            if (i >= all) continue;
+            const Kv4RowPlace p = places[i / units];
+            if (p.page == ~0u) continue;
+            const uint8_t* blk = a.c.blocks + (size_t(p.page) * a.c.num_kv_heads + h) * G.block;
+            code[q] = ld_plain(reinterpret_cast<const uint2*>(blk + G.codes(kv, g) + p.slot * 32 + j * 8));
+            sb[q] = ld_plain(reinterpret_cast<const uint32_t*>(blk + G.sb(kv, g) + p.slot * 4));
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t i = i0 + q * STEP, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
+            if (i >= all || places[i / units].page == ~0u) continue;
+            const float scale = __uint_as_float(sb[q] << 16), bias = __uint_as_float(sb[q] & 0xffff0000u);
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                v[k] = __fadd_rn(__fmul_rn(float((k < 8 ? code[q].x : code[q].y) >> (4 * (k % 8)) & 15u), scale), bias);
+            const uint32_t row = row0 + i / units;
+            const size_t at = (kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head) + g * 64 + j * 16;
+            void* dst = kv ? r.v : r.k;
+            if (DTYPE == SMOE_DTYPE_F32) {
+                float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                continue;
+            }
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(v[2 * k], v[2 * k + 1]);
+            if (WIDE) {
+                uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at);
+                d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+                uint2* d = reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = make_uint2(w[2 * k], w[2 * k + 1]);
+            }
+        }
     }
 }
 
@@ -156,10 +285,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Args a, const uint32_t* fir
 // part of (warp, pair) has the number warp + pair: along the line at least
 // one of the two grows from a part to the next, so no two share one.
 constexpr int kKaWarps = 4, kKaStages = 3;
-#ifndef KA_CTAS
-#define KA_CTAS 3
-#endif
-constexpr uint32_t kKaCtas = KA_CTAS, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
+constexpr uint32_t kKaCtas = 3, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
 
 struct Kv4Attn {
     Kv4Args a;
@@ -187,34 +313,39 @@ SMOE_DEVINL uint32_t kv4_valid(const Kv4Attn& p, uint32_t s) {
 SMOE_DEVINL uint32_t kv4_pages(uint32_t n) { return (n + kKvPage - 1) / kKvPage; }
 
 // The line of pages: sequence s starts at heads * (pages of the sequences
-// before it), `heads` pairs of equal length each.
+// before it), `heads` pairs of equal length each. (Below 2^31 pages: the host
+// refuses more.)
 struct Kv4Line {
-    uint64_t total, per;                         // pages, pages of a stretch
-    SMOE_DEVINL uint64_t first(uint32_t w) const { return min(total, uint64_t(w) * per); }
+    uint32_t total, per;                         // pages, pages of a stretch
+    SMOE_DEVINL uint32_t first(uint32_t w) const { return min(uint64_t(total), uint64_t(w) * per); }
 };
 // By a whole warp: the line, and the sequence that holds warp w's first page
 // with the page of the line that it starts at.
-SMOE_DEVINL Kv4Line kv4_line(const Kv4Attn& p, uint32_t heads, uint32_t lane, uint32_t w, uint32_t& seq, uint64_t& start) {
+SMOE_DEVINL Kv4Line kv4_line(const Kv4Attn& p, uint32_t heads, uint32_t lane, uint32_t w, uint32_t& seq, uint32_t& start) {
     const uint32_t ns = p.a.c.n_seqs;
-    uint64_t total = 0, before = 0;
+    uint32_t total = 0, before = 0, n = 0;
+#pragma unroll 1
     for (uint32_t b = 0; b < ns; b += 32) {
-        const uint32_t s = b + lane, n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;
+        const uint32_t s = b + lane;
+        n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;
         total += __reduce_add_sync(0xffffffffu, n);
     }
-    Kv4Line L{total * heads, max(uint64_t(1), (total * heads + p.warps - 1) / p.warps)};
-    const uint64_t want = L.first(w);
+    const Kv4Line L{total * heads, max(1u, (total * heads + p.warps - 1) / p.warps)};
+    const uint32_t want = L.first(w);
     seq = ns;
+    start = 0;
     if (want >= L.total) return L;
+#pragma unroll 1
     for (uint32_t b = 0; b < ns; b += 32) {
-        const uint32_t s = b + lane, n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;
+        const uint32_t s = b + lane;
+        if (ns > 32) n = s < ns ? kv4_pages(kv4_valid(p, s)) : 0u;             // (else they are still at hand)
         uint32_t incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= uint32_t(o)) incl += v;
         }
-        const uint64_t end = (before + incl) * heads;
-        const uint32_t hit = __ballot_sync(0xffffffffu, end > want);
+        const uint32_t hit = __ballot_sync(0xffffffffu, (before + incl) * heads > want);
         if (hit) {
             const int l = __ffs(hit) - 1;
             seq = b + l;
@@ -310,14 +441,14 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
     __syncwarp();
     pdl_acquire();
     uint32_t seq;
-    uint64_t start;
+    uint32_t start;
     const Kv4Line L = kv4_line(p, nheads, lane, me, seq, start);
-    const uint64_t t0 = L.first(me), t1 = L.first(me + 1);
+    const uint32_t t0 = L.first(me), t1 = L.first(me + 1);
     if (t0 >= t1) return;
-    const uint32_t mine = uint32_t(t1 - t0);
+    const uint32_t mine = t1 - t0;
 
     // where the stretch starts, and the next unit to send for (ahead of the one in work)
-    uint32_t n = kv4_valid(p, seq), np = kv4_pages(n), hc = uint32_t((t0 - start) / np), pg = uint32_t((t0 - start) % np);
+    uint32_t n = kv4_valid(p, seq), np = kv4_pages(n), hc = (t0 - start) / np, pg = (t0 - start) % np;
     uint32_t a_seq = seq, a_np = np, a_hc = hc, a_pg = pg, sent = 0;
     uint32_t a_page = 0, good = 0, slot = 0, phase = 0;          // good: bit i % 2, page i can be read; slot, phase: of the unit in work
     auto send = [&](uint32_t st) {               // unit `sent`, into slot st
@@ -372,7 +503,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
         if (fresh) {
             fresh = false;
             if (pg == 0 && lane == 0)            // this warp is the pair's first one
-                p.meta[uint64_t(seq) * nheads + hc] = make_uint2(me, uint32_t((t0 + i + np - 1) / L.per) - me + 1);
+                p.meta[uint64_t(seq) * nheads + hc] = make_uint2(me, (t0 + i + np - 1) / L.per - me + 1);
             const uint32_t kvh = hc / p.chunks, h0 = hc % p.chunks * kKaHeads;
             heads = min(kKaHeads, p.group - h0);
             head0 = kvh * p.group + h0;

@@ -58,6 +58,9 @@ int smem_limit(const CtxView& c, K kern, size_t smem) {
     return SMOE_OK;
 }
 
+// bf16 rows whose groups all start on 16 bytes.
+bool wide_rows(const SmoeKv4Rows* r) { return (r->k_row | r->k_head | r->v_row | r->v_head) % 8 == 0; }
+
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
 EncodeTiled encode_tiled() {
     static const EncodeTiled fn = [] {
@@ -226,7 +229,12 @@ int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const Smoe
     if (rc || (rc = check_rows(rows, "kv4_append: bad rows"))) return rc;
     if (rows->total == 0) return SMOE_OK;
     const CtxView c = smoe::ctx_view(ctx);
-    return launch(c, smoe::k_kv4_append, dim3((rows->total + 7) / 8), dim3(256), 0, smoe::Kv4Args{*cache, c.err}, *rows);
+    using namespace smoe;
+    auto run = [&](auto kern) {
+        return launch(c, kern, dim3((rows->total - 1) / kKwRows + 1), dim3(kKwThreads), 0, Kv4Args{*cache, c.err}, *rows);
+    };
+    if (rows->dtype == SMOE_DTYPE_F32) return run(k_kv4_append<SMOE_DTYPE_F32, true>);
+    return wide_rows(rows) ? run(k_kv4_append<SMOE_DTYPE_BF16, true>) : run(k_kv4_append<SMOE_DTYPE_BF16, false>);
 }
 
 int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32_t* first, const SmoeKv4Rows* rows) {
@@ -235,7 +243,12 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
     if (rc || (rc = check_rows(rows, "kv4_read: bad rows"))) return rc;
     if (rows->total == 0) return SMOE_OK;
     const CtxView c = smoe::ctx_view(ctx);
-    return launch(c, smoe::k_kv4_read, dim3((rows->total + 7) / 8), dim3(256), 0, smoe::Kv4Args{*cache, c.err}, first, *rows);
+    using namespace smoe;
+    auto run = [&](auto kern) {
+        return launch(c, kern, dim3((rows->total - 1) / kKwRows + 1), dim3(kKwThreads), 0, Kv4Args{*cache, c.err}, first, *rows);
+    };
+    if (rows->dtype == SMOE_DTYPE_F32) return run(k_kv4_read<SMOE_DTYPE_F32, true>);
+    return wide_rows(rows) ? run(k_kv4_read<SMOE_DTYPE_BF16, true>) : run(k_kv4_read<SMOE_DTYPE_BF16, false>);
 }
 
 uint64_t smoe_cuda_kv4_attention_workspace(const SmoeKv4Cache* cache, const SmoeKv4AttnArgs* t) {
@@ -254,6 +267,8 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: q and out are fp32 or bf16", t->dtype);
     if (!aligned(t->q, 16) || !aligned(t->out, 16) || (t->q_row | t->out_row) % 4)
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention needs 16-byte aligned q and out and strides that are multiples of 4", 0);
+    if (uint64_t(cache->n_seqs) * t->num_heads * ((uint64_t(t->max_len) + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE) >= (uint64_t(1) << 31))
+        return ctx_fail(SMOE_ERR_UNSUPPORTED, "kv4_attention: more than 2^31 pages to read", long(t->max_len));
     const uint64_t need = smoe_cuda_kv4_attention_workspace(cache, t);
     if (need && (!t->workspace || t->workspace_bytes < need || !aligned(t->workspace, 16)))
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: workspace missing, too small or unaligned; bytes needed", long(need));
