@@ -262,11 +262,12 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 
 // ---------------------------------------------------------------- attention
 // One query token per sequence. With a group's codes c (0..15), scales s and
-// biases b:
-//   q . k = sum_g s_g (q_g . c_g) + b_g sum(q_g)
-//   sum_j p_j v_j = sum_j (p_j s_j) c_j + sum_j p_j b_j          (per group)
-// so the raw codes are the tensor cores' operands (exact in fp16) and scales
-// and biases stay in fp32. q goes in as one (bf16 q) or two fp16 pieces, each
+// biases b, and c' = c - 8, b' = b + 8 s:
+//   q . k = sum_g s_g (q_g . c'_g) + b'_g sum(q_g)
+//   sum_j p_j v_j = sum_j (p_j s_j) c'_j + sum_j p_j b'_j        (per group)
+// so the codes are the tensor cores' operands (exact in fp16) and scales and
+// biases stay in fp32. (c' and not c: the two sums then do not cancel - fp32
+// results were four times as far from 64 bits with c.) q goes in as one (bf16 q) or two fp16 pieces, each
 // head scaled by a power of two so that its largest value is near 2^14; p s
 // as two fp16 pieces (22 bits), times a power of two per group that follows
 // the largest scale seen. (bf16 pieces need no such power, but three more
@@ -357,15 +358,15 @@ SMOE_DEVINL Kv4Line kv4_line(const Kv4Attn& p, uint32_t heads, uint32_t lane, ui
     return L;
 }
 
-// 8 codes as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c are
-// exact, and so is what the subtraction or the multiply-add makes of them.
+// 8 codes less 8 as fp16 pairs (code n, code n + 4): 1024 + c and 1024 + 16 c
+// are exact, and so is what the subtraction or the multiply-add makes of them.
 SMOE_DEVINL void kv4_half_codes(uint32_t w, uint32_t* r) {
     constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u, ONE = 0x64006400u;
     const uint32_t w8 = w >> 8;
-    r[0] = hsub_1024(lop3_and_or(w, M0, ONE));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(lop3_and_or(w, M1, ONE)), "r"(0x2C002C00u), "r"(0xD400D400u));
-    r[2] = hsub_1024(lop3_and_or(w8, M0, ONE));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(lop3_and_or(w8, M1, ONE)), "r"(0x2C002C00u), "r"(0xD400D400u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[0]) : "r"(lop3_and_or(w, M0, ONE)), "r"(0x64086408u));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(lop3_and_or(w, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[2]) : "r"(lop3_and_or(w8, M0, ONE)), "r"(0x64086408u));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(lop3_and_or(w8, M1, ONE)), "r"(0x2C002C00u), "r"(0xD480D480u));
 }
 SMOE_DEVINL void mma_f16f32_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float s0 = lo_f(sa[g]), b0 = hi_f(sa[g]), s1 = lo_f(sb[g]), b1 = hi_f(sb[g]);
+                const float s0 = lo_f(sa[g]), b0 = fmaf(8.0f, s0, hi_f(sa[g])), s1 = lo_f(sb[g]), b1 = fmaf(8.0f, s1, hi_f(sb[g]));
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     x[mt][k] = fmaf(s0, d[g][k], g ? fmaf(b0, qsm[g][k], x[mt][k]) : b0 * qsm[g][k]);
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             for (int g = 0; g < NG; ++g) {
                 const uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + ka * 4);
                 const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + kb * 4);
-                const float s0 = lo_f(sa) * up[g], b0 = hi_f(sa), s1 = lo_f(sb) * up[g], b1 = hi_f(sb);
+                const float b0 = fmaf(8.0f, lo_f(sa), hi_f(sa)), b1 = fmaf(8.0f, lo_f(sb), hi_f(sb)), s0 = lo_f(sa) * up[g], s1 = lo_f(sb) * up[g];
                 // codes of this lane's 8 dimensions (8 gr ..) of the entries 2 cl, 2 cl + 1, 2 cl + 8, 2 cl + 9 of the tile;
                 // lanes cl >= 2 load the pair the other way round (the four entries of a load then lie in different banks)
                 uint32_t w[4];
