@@ -574,7 +574,8 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
  *   heads of p[h][j]     (decay 0 or cache->score NULL: without the first)
  * for the attended entries; others stay. fp32 statistics and accumulators;
  * the codes are exact tensor-core operands, probabilities and an fp32 q go
- * in as sums of bf16 pieces, so results are good to about 2^-16. max_len: an
+ * in as sums of two fp16 pieces, good to about 2^-20 of the largest term.
+ * scale finite and not negative. max_len: an
  * upper limit of len[s] + extra, known to the host (it sizes the grid and
  * the workspace; longer sequences are cut there and raise SMOE_ERR_DEVICE).
  * workspace: smoe_cuda_kv4_attention_workspace bytes, 16-byte aligned, its
@@ -596,10 +597,11 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
 
 /* Cut every sequence with more than `keep` entries to `keep`, per KV head:
  * the entries whose pos + recent >= seen[s] stay, and of the others the best
- * by score (ties: the lowest entry; NaN is the lowest score; more recent ones
- * than keep: the lowest entries of them). Kept entries below `keep` stay
- * where they are; the j-th kept entry past it moves to the j-th free one
- * below it, K, V, pos and score. Entries past `keep` are left as they are.
+ * by score (ties: the lowest entry; NaN is the lowest score; when more than
+ * `keep` are that recent, the lowest `keep` entries of them stay). Kept
+ * entries below `keep` stay where they are; the j-th kept entry past it moves
+ * to the j-th free one below it, K, V, pos and score. Entries past `keep` are
+ * left as they are.
  * pos_out / score_out NULL: pos and score are updated in place; else those of
  * all entries below min(len, keep) are written there (distinct arrays, same
  * layout) and cache->pos / score stay. len stays (smoe_cuda_kv4_advance cuts

@@ -44,7 +44,10 @@ SMOE_DEVINL uint32_t kv4_page(const SmoeKv4Cache& c, uint32_t s, uint64_t e, uin
 // values a lane: the group's 32 bytes of codes are 8 a lane, its minimum and
 // maximum two shuffles. Values are fetched before the entries are known, and
 // two units a lane are in flight. Bound by the chain of look-ups (bounds,
-// length, page table) for a step's rows and by the bytes for a prompt's.
+// length, page table) for a step's rows (256 fp32 rows of 4 heads of 128: 7 us,
+// their read-back 6, both cold) and by the instructions that find the codes
+// for a prompt's (5,800 bf16 rows: 17 us cold, half of the issue slots used).
+// With a division for each code and two lanes a unit those took 10 and 26 us.
 constexpr int kKwRows = 8, kKwThreads = 256;
 
 struct Kv4RowPlace {
@@ -274,17 +277,25 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // instructions for every 16 codes.)
 // The entries are the M rows of both products and 8 of a KV head's query
 // heads the N columns. (16 at a time halve the unpacking of wide groups, but
-// need 255 registers: 8 warps an SM instead of 16, and 1.2 times the time.)
+// need 255 registers: 8 warps an SM instead of 12, and 1.2 times the time.)
 //
 // All pages of all (sequence, KV head) pairs, in one line, are cut into equal
 // stretches, one a warp of a grid that fills the GPU once: ragged lengths do
 // not matter, and no warp waits for another. A warp copies its pages' keys and
-// values, by turns, into a ring of three of its own (216 KB an SM), and for
+// values, by turns, into a ring of three of its own (166 KB an SM), and for
 // each pair that its stretch touches it keeps a running maximum, sums and
 // accumulators. A pair inside one stretch is done (unless weights are
 // wanted); the parts of the others are stored and joined by k_kv4_join. The
 // part of (warp, pair) has the number warp + pair: along the line at least
 // one of the two grows from a part to the next, so no two share one.
+//
+// Bound by issue: 16 entries cost about 400 warp instructions (the codes'
+// unpacking on the integer units, the probabilities' pieces), 53% of the issue
+// slots with 12 warps an SM. Two contexts of 125,000 (head_dim 128, 32 / 4
+// heads, bf16, weights): 58 us of k_kv4_attention cold for 148 MB, 2.6 TB/s
+// (3.9 TB/s once the rings run; the start and the stretches' whole pages cost
+// about 14 us), and 8 us of k_kv4_join. 32 contexts of 512 to 8,192: 33 us
+// with the join; one of 300: 10.6 us, of which most is the two launches.
 constexpr int kKaWarps = 4, kKaStages = 3;
 constexpr uint32_t kKaCtas = 3, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
 
@@ -804,7 +815,9 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
 // sharing the parts of an output (many parts, few outputs: the chain of loads
 // stays short); the others 1024 entries each, 4 a thread. Every CTA first
 // forms the maxima and sums of the heads that it needs from the parts'
-// (contiguous: a thread a head and every 32nd part).
+// (contiguous: a thread a head and every 32nd part). Bound by that chain of
+// loads: 4 us for a short sequence, 8 to 12 us where 260,000 entries get
+// weights (their stored scores pass at 2 to 3 TB/s).
 constexpr int kKjThreads = 256, kKjEntries = 4 * kKjThreads;
 __global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p, uint32_t outs) {
     constexpr uint32_t heads = kKaHeads;
@@ -965,8 +978,11 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     Sources are past `keep` and targets below it: no move reads what
 //     another writes. (Separate outputs have pos and score of all entries
 //     below `keep` from step 1, before the moved ones' overwrite them.)
-// Bound by the chain of steps for short sequences and by the moves' bytes for
-// long ones.
+// Bound by the chain of steps for short sequences (8 of 1,100 entries cut to
+// 1,024, 4 KV heads: 12.7 us) and by the moves for long ones (16 of 6,000 to
+// 32,768 cut to 4,096: 56 us, of which the selection takes 18; the moves'
+// 32-byte sectors pass at about 6 TB/s, as far as memory goes). One launch:
+// with a launch a step the first took 37 us, the second 244.
 constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvDigits = 3;
 constexpr uint32_t kEvBins = 2048;
 __host__ __device__ constexpr uint32_t kv4_evict_smem(uint32_t cached) { return (kEvDigits * kEvBins + cached) * 4; }
