@@ -12,7 +12,10 @@ namespace smoe {
 // keys and values then serve all its query heads from one shared-memory copy,
 // and a short prompt fills a tile with G times fewer tokens. A CTA works on
 // two tiles of 128 rows at a time (the tensor cores work for one while the
-// other's softmax runs) and walks the keys 128 at a time.
+// other's softmax runs) and walks the keys 64 at a time. Each tile has room for
+// the scores of two blocks: the next block's are there when the softmax has
+// done one (with 128 keys and one place it waited for two products every
+// time; 24 prompts of 17 to 2,048 tokens took 1.13 times as long).
 //
 // Small calls run a CTA per tile pair. Otherwise there is one CTA an SM, which
 // goes from pair to pair with the next one's loads in flight:
@@ -25,17 +28,15 @@ namespace smoe {
 //
 // Softmax by the running maximum and sum; probabilities go back to tensor
 // memory as bf16 (over the scores) and are the left operand of the second
-// product. A block of 128 keys takes a tile pair 3,900 cycles: of each tile's
-// chain 3,100 are the softmax (2,300 of them the exponentials, whose unit the
-// two tiles share and which alone would need 2,048) and 850 the two products.
-// 16,384 causal tokens of 32 / 4 heads of 128: 1.87 ms, 1,180 TFLOP/s (2.1 ms
-// when the call repeats for seconds, at the power limit); 24 prompts of 17 to
-// 2,048: 196 us, 760 TFLOP/s; 4 x 200..512 tokens over 6,000 keys, heads of
-// 64: 41 us; 45 tokens: 9.5 us. (Part of the exponentials by polynomial, all
-// 128 scores in registers with a register split between the warps, and
+// product. A block of 64 keys takes a tile pair 1,800 cycles, of which the
+// exponentials' unit needs 1,024 (its two tiles take it by turns, 900 each)
+// and the tensor cores 1,060. 16,384 causal tokens of 32 / 4 heads of 128:
+// 1.77 ms, 1,240 TFLOP/s; 24 prompts of 17 to 2,048: 170 us, 877 TFLOP/s;
+// 4 x 200..512 tokens over 6,000 keys, heads of 64: 36 us; 45 tokens: 8.9 us.
+// (Without turns 1.05 times as long; part of the exponentials by polynomial,
 // chunks of 16 were no faster.)
-constexpr uint32_t kPaRows = 128, kPaKeys = 128;
-constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA, MMA, items and checks, a warp each
+constexpr uint32_t kPaRows = 128, kPaKeys = 64;
+constexpr int kPaThreads = 384;                  // 2 x 4 softmax warps; TMA, MMA of each tile and items, a warp each
 constexpr int kPaItems = 2;                       // items that a CTA has at hand: the one in work and the next
 constexpr uint32_t kPaMaxPairs = 65536;          // tile pairs of a planned call (per KV head)
 
@@ -61,9 +62,10 @@ struct PackedArgs {
 template <int HP>                                // head_dim rounded up to 64 or 128
 struct PackedSmem {
     static constexpr uint32_t TILE = HP / 64 * 16384;            // 128 rows, 64-column halves of 128-byte rows
-    static constexpr int STAGES = HP == 128 ? 4 : 8;             // even: keys in the even ones, values in the odd
-    static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + STAGES * TILE;        // OUT: 4 KB a softmax warp, rows on their way out
-    static constexpr uint32_t BAR = OUT + 8 * 4096, ITEMS = BAR + 384, END = ITEMS + kPaItems * 64;
+    static constexpr uint32_t BLOCK = TILE * kPaKeys / kPaRows;  // 64 rows of keys or values, likewise
+    static constexpr int STAGES = 8;                             // even: keys in the even ones, values in the odd
+    static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + STAGES * BLOCK;        // OUT: 4 KB a softmax warp, rows on their way out
+    static constexpr uint32_t BAR = OUT + 8 * 4096, ITEMS = BAR + 512, END = ITEMS + kPaItems * 64;
     static constexpr uint32_t bytes() { return END + 1024; }     // the base is rounded up to 1024
 };
 
@@ -155,7 +157,7 @@ struct PaWalk {
 };
 
 // One CTA: the places where `ctas` equal shares of the work start. A pair
-// costs its blocks and one more.
+// costs its blocks and two more.
 constexpr int kPlThreads = 1024;
 SMOE_DEVINL uint32_t pl_scan(uint32_t v, uint32_t* sums, uint32_t& all) {      // exclusive sum over the CTA
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -181,8 +183,8 @@ SMOE_DEVINL uint32_t pl_scan(uint32_t v, uint32_t* sums, uint32_t& all) {      /
 // cost: [kPaMaxPairs] scratch, the exclusive sums of the pairs' costs; place:
 // [kPaMaxPairs] (sequence, token) of each pair. (The host has checked that
 // the call cannot have more pairs.) With `list` instead of `plan`: the places
-// sorted by their costs, longest first (those past 1023 blocks, and equal
-// ones, in any order).
+// sorted by their costs, longest first (by 128 keys; those past 1023 such, and
+// equal ones, in any order).
 __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, PaPlace* plan, uint32_t ctas, uint32_t* cost, uint2* place,
                                                             uint2* list) {
     __shared__ uint32_t sums[32], bins[kPlThreads];
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
         for (uint32_t i = tid; i < pairs; i += kPlThreads) {
             const uint2 at = place[i];
             const PackedSeq S = packed_seq(p.a, at.x);
-            const uint32_t n = min(uint32_t(kPlThreads - 1), max(S.blocks(at.y, p.tokens, 0), S.blocks(at.y, p.tokens, 1)));
+            const uint32_t n = min(uint32_t(kPlThreads - 1), max(S.blocks(at.y, p.tokens, 0), S.blocks(at.y, p.tokens, 1)) / 2);
             cost[i] = n;
             atomicAdd(&bins[kPlThreads - 1 - n], 1u);
         }
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
         if (i < pairs) {
             const uint2 at = place[i];
             const PackedSeq S = packed_seq(p.a, at.x);
-            n = max(S.blocks(at.y, p.tokens, 0), S.blocks(at.y, p.tokens, 1)) + 1;
+            n = max(S.blocks(at.y, p.tokens, 0), S.blocks(at.y, p.tokens, 1)) + 2;
         }
         const uint32_t before = total + pl_scan(n, sums, all);
         if (i < pairs) cost[i] = before;
@@ -269,10 +271,10 @@ __global__ void __launch_bounds__(kPlThreads) k_packed_plan(const PackedArgs p, 
                 if (cost[mid] <= y) lo = mid;
                 else hi = mid - 1;
             }
-            const uint32_t n = (lo + 1 < pairs ? cost[lo + 1] : total) - cost[lo] - 1, off = y - cost[lo];
-            uint32_t blk = off > 0 ? off - 1 : 0u;
-            if (blk < 2) blk = 0;                // (no part of a single block)
-            if (n < blk + 2 && blk) {
+            const uint32_t n = (lo + 1 < pairs ? cost[lo + 1] : total) - cost[lo] - 2, off = y - cost[lo];
+            uint32_t blk = off > 1 ? off - 2 : 0u;
+            if (blk < 4) blk = 0;                // (no part of few blocks)
+            if (n < blk + 4 && blk) {
                 blk = 0;
                 if (++lo == pairs) lo = 0, ++kvh;
             }
@@ -426,10 +428,10 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
-    const Bar qf{base + SM::BAR}, qe = qf + 2, sf = qf + 4, pr = qf + 6, pl = qf + 8, of = qf + 10, vc = qf + 12, itf = qf + 16, ite = itf + kPaItems,
-              xb = ite + kPaItems, kvf = xb + 3, kve = kvf + ST;
+    const Bar qf{base + SM::BAR}, qe = qf + 2, sf = qf + 4, pr = qf + 8, of = qf + 12, itf = qf + 16, ite = itf + kPaItems,
+              xb = ite + kPaItems, turn = xb + 3, kvf = turn + 8, kve = kvf + ST;
     const Word fail{(kve + ST).a}, begun = fail + 1, odds = fail + 4;          // begun[t]: the accumulator holds something before block 0's P V
-    uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + SM::BAR + ((kve + ST).a - qf.a)) + 3;  // odds[4]: of the last masked blocks: its values hold an infinity or NaN
+    uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + SM::BAR + ((kve + ST).a - qf.a)) + 3;  // odds: a word of each softmax warp, by turns in two
     PaItem* const items = reinterpret_cast<PaItem*>(smem + SM::ITEMS);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const SmoeCudaPackedAttnArgs& a = p.a;
@@ -439,20 +441,21 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         for (int i = 0; i < 2; ++i) {
             (qf + i).init(1);
             (qe + i).init(1);
+        }
+        for (int i = 0; i < 4; ++i) {            // sf, pr, of: of tile i / 2, for its even and odd blocks
             (sf + i).init(1);
             (pr + i).init(4);
-            (pl + i).init(4);
             (of + i).init(1);
         }
-        for (int i = 0; i < 4; ++i) (vc + i).init(1);
         for (int i = 0; i < kPaItems; ++i) {
             (itf + i).init(1);
-            (ite + i).init(11);              // the TMA lane, the MMA lane, the checking warp, eight softmax warps
+            (ite + i).init(11);              // the TMA lane, the MMA lanes, eight softmax warps
         }
         for (int i = 0; i < 3; ++i) (xb + i).init(i < 2 ? 4 : 8);
+        for (int i = 0; i < 8; ++i) (turn + i).init(1);
         for (int i = 0; i < ST; ++i) {
             (kvf + i).init(1);
-            (kve + i).init(1 + i % 2);       // the MMA lane; of values (odd stages), the checking warp, too
+            (kve + i).init(2);               // the MMA lanes
         }
         fail.set(0u);
         begun.set(0u);
@@ -495,9 +498,9 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     }
                     const uint32_t st = j % ST, round = j / ST;
                     if (round) wait(kve + st, round - 1);
-                    (kvf + st).expect(SM::TILE);
+                    (kvf + st).expect(SM::BLOCK);
                     for (int h = 0; h < NH; ++h)
-                        tma_load3(base + SM::KV + st * SM::TILE + h * 16384, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
+                        tma_load3(base + SM::KV + st * SM::BLOCK + h * 8192, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
                 }
             }
             // nothing may be in flight when the CTA ends (the MMA warp has
@@ -507,76 +510,72 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
             for (int t = 0; t < 2; ++t)
                 if (nq[t]) pa_drain(qf + t, (nq[t] - 1) & 1);
         }
-    } else if (warp == 9) {
-        // ------------------------------------------------------ MMA (one lane)
+    } else if (warp == 9 || warp == 10) {
+        // ------------------------------------- MMA (one lane each for the two
+        // tiles: a wait or a commit costs a lane some 90 cycles, and with one
+        // lane for both the tensor cores stood still for a third of the time)
         if (elect_one()) {
-            constexpr uint32_t IQK = tc_idesc_bf16(128, 128, 0), IPV = tc_idesc_bf16(128, HP, 1);
-            const uint32_t sq = base + SM::Q, skv = base + SM::KV;
-            uint32_t j0 = 0, nq[2] = {0u, 0u}, nb[2] = {0u, 0u}; // units, Q tiles, blocks of each tile so far
-            auto qk = [&](uint32_t t, uint32_t st, bool last) {
-                const uint64_t qd = tc_desc_sw128(sq + t * SM::TILE, 16), kd = tc_desc_sw128(skv + st * SM::TILE, 16);
+            constexpr uint32_t IQK = tc_idesc_bf16(128, kPaKeys, 0), IPV = tc_idesc_bf16(128, HP, 1);
+            const uint32_t t = warp - 9, ts = tmem + t * 128, to = tmem + TMEM_O + t * 128, skv = base + SM::KV;
+            const uint64_t qd = tc_desc_sw128(base + SM::Q + t * SM::TILE, 16);
+            uint32_t j0 = 0, nq = 0, nb = 0;     // units, Q tiles, blocks of the tile so far
+            auto qk = [&](uint32_t st, uint32_t n, bool last) {  // scores of the tile's block n
+                const uint64_t kd = tc_desc_sw128(skv + st * SM::BLOCK, 16);
 #pragma unroll
-                for (int s = 0; s < HP / 16; ++s) {
-                    const uint32_t o = (s / 4 * 16384 + s % 4 * 32) >> 4;
-                    tc_mma_f16(tmem + t * 128, qd + o, kd + o, IQK, s > 0);
-                }
-                (sf + t).commit();
+                for (int s = 0; s < HP / 16; ++s)
+                    tc_mma_f16(ts + n % 2 * 64, qd + ((s / 4 * 16384 + s % 4 * 32) >> 4), kd + ((s / 4 * 8192 + s % 4 * 32) >> 4), IQK, s > 0);
+                (sf + t * 2 + n % 2).commit();
                 if (last) (qe + t).commit();     // the tile's Q has been read
             };
-            auto pv = [&](uint32_t t, uint32_t st, bool more, uint32_t block) {
-                const uint64_t vd = tc_desc_sw128(skv + st * SM::TILE, 16384);
+            auto pv = [&](uint32_t st, uint32_t n, bool more) {
+                const uint64_t vd = tc_desc_sw128(skv + st * SM::BLOCK, 8192);
 #pragma unroll
-                for (int s = 0; s < kPaKeys / 16; ++s) {
-                    if (s == kPaKeys / 16 * 3 / 4) {             // the last quarter of P
-                        wait(pl + t, block);
-                        tc_fence_after();
-                    }
-                    tc_mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + s * 8, vd + ((s * 2048) >> 4), IPV, more || s > 0);
-                }
-                (of + t).commit();
+                for (int s = 0; s < int(kPaKeys) / 16; ++s)
+                    tc_mma_ts(to, ts + n % 2 * 64 + s * 8, vd + ((s * 2048) >> 4), IPV, more || s > 0);
+                (of + t * 2 + n % 2).commit();
             };
 #pragma unroll 1
             for (uint32_t k = 0; !fail.get(); ++k) {
                 const PaItem& it = item(k);
                 if (!it.more) break;
-                const uint32_t c0 = it.cnt[0], c1 = it.cnt[1], m = max(c0, c1);
+                const uint32_t nt = it.cnt[t], m = max(it.cnt[0], it.cnt[1]);
                 item_done(k);
-                if (m) {
-                    wait(kvf + j0 % ST, j0 / ST);
-#pragma unroll
-                    for (uint32_t t = 0; t < 2; ++t)
-                        if (t ? c1 : c0) {
-                            wait(qf + t, nq[t]++);
-                            tc_fence_after();
-                            qk(t, j0 % ST, (t ? c1 : c0) == 1);
-                        }
-                    (kve + j0 % ST).commit();
+#pragma unroll 1
+                for (uint32_t i = 0; i < min(m, 2u); ++i) {      // the first two blocks' scores
+                    const uint32_t jk = j0 + 2 * i;
+                    wait(kvf + jk % ST, jk / ST);    // (all of them in turn: a phase skipped could be taken for another)
+                    if (i < nt) {
+                        if (i == 0) wait(qf + t, nq++);
+                        tc_fence_after();
+                        qk(jk % ST, nb + i, i + 1 == nt);
+                    }
+                    (kve + jk % ST).commit();
                 }
 #pragma unroll 1
                 for (uint32_t i = 0; i < m; ++i) {
-                    const uint32_t jv = j0 + 2 * i + 1, jk = jv + 1, sv = jv % ST, sk = jk % ST;
+                    const uint32_t jv = j0 + 2 * i + 1, jk = jv + 3, sv = jv % ST, sk = jk % ST;
                     wait(kvf + sv, jv / ST);
-                    if (i + 1 < m) wait(kvf + sk, jk / ST);
-#pragma unroll
-                    for (uint32_t t = 0; t < 2; ++t) {
-                        const uint32_t nt = t ? c1 : c0;
-                        if (i < nt) {
-                            // (of an item's first block this also says that the
-                            // softmax warps have read the last item's sums)
-                            wait(pr + t, nb[t]);
-                            tc_fence_after();
-                            pv(t, sv, i > 0 || (begun + t).get(), nb[t]++);
-                        }
-                        if (i + 1 < nt) qk(t, sk, i + 2 == nt);
+                    if (i < nt) {
+                        // (of an item's first block this also says that the
+                        // softmax warps have read the last item's sums)
+                        wait(pr + t * 2 + nb % 2, nb / 2);
+                        tc_fence_after();
+                        pv(sv, nb, i > 0 || (begun + t).get());
                     }
                     (kve + sv).commit();
-                    if (i + 1 < m) (kve + sk).commit();
+                    if (i + 2 < m) wait(kvf + sk, jk / ST);
+                    if (i + 2 < nt) {
+                        tc_fence_after();
+                        qk(sk, nb, i + 3 == nt); // (where the block's probabilities were)
+                    }
+                    if (i + 2 < m) (kve + sk).commit();
+                    nb += i < nt;
                 }
                 j0 += 2 * m;
             }
             if (j0) pa_drain(kve + (j0 - 1) % ST, ((j0 - 1) / ST) & 1);                // all MMAs done: the last commit
         }
-    } else if (warp == 10) {
+    } else if (warp == 11) {
         // ------------------------------------------------------------- items
         PaWalk walk;
         walk.single = !p.plan;
@@ -639,56 +638,9 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 (itf + k % kPaItems).arrive();
             }
         }
-    } else if (warp == 11) {
-        // ------------------------------------------------- checks (one warp)
-        // Values of blocks that not every row may see all of: is there an
-        // infinity or NaN?
-        uint32_t j0 = 0, nm = 0;
-#pragma unroll 1
-        for (uint32_t k = 0;; ++k) {
-            const PaItem& it = item(k);
-            if (__any_sync(0xffffffffu, fail.get() || !it.more)) break;
-            const uint32_t m = max(it.cnt[0], it.cnt[1]);
-#pragma unroll 1
-            for (uint32_t i = 0; i < m; ++i) {
-                const uint32_t jv = j0 + 2 * i + 1;
-                wait(kvf + jv % ST, jv / ST);    // (all of them in turn: a phase skipped could be taken for another)
-                if (!pa_masked(it, i)) {
-                    if (lane == 0) (kve + jv % ST).arrive();
-                    continue;
-                }
-                const uint4* v = reinterpret_cast<const uint4*>(smem + SM::KV + jv % ST * SM::TILE) + lane;
-                __nv_bfloat162 acc[4];
-                const __nv_bfloat162 zero = __float2bfloat162_rn(0.0f);
-                acc[0] = acc[1] = acc[2] = acc[3] = zero;
-#pragma unroll 8
-                for (uint32_t q = 0; q < SM::TILE / 16; q += 32) {               // 0 times one of those is a NaN
-                    const uint4 x = v[q];
-                    acc[0] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.x), zero, acc[0]);
-                    acc[1] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.y), zero, acc[1]);
-                    acc[2] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.z), zero, acc[2]);
-                    acc[3] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x.w), zero, acc[3]);
-                }
-                const __nv_bfloat162 all = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
-                const bool odd = __any_sync(0xffffffffu, __hisnan(all.x) || __hisnan(all.y));
-                if (lane == 0) {
-                    // (At most four V tiles are in the ring, so of the masked block four
-                    // back all products are done: the softmax warps have read its flag.)
-                    (odds + nm % 4).set(odd);
-                    (vc + nm % 4).arrive();
-                    (kve + jv % ST).arrive();
-                }
-                ++nm;
-            }
-            j0 += 2 * m;
-            __syncwarp();
-            if (lane == 0) item_done(k);
-        }
     } else {
         // ----------------------------------------------------------- softmax
-        // One thread a row, which reads its scores twice, 32 at a time with the
-        // next 32 on their way: for the maximum and for the exponentials. (All
-        // 128 at once left the loop without registers.) The reference maximum is only moved when the
+        // One thread a row. The reference maximum is only moved when the
         // running one is more than 8 (in log2) above it, so the
         // accumulator is rarely rescaled; probabilities stay below 2^8.
         const uint32_t t = warp >> 2, r = tid & 127;
@@ -696,7 +648,6 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
         const float sl = p.scale_log2;
         const uint32_t tk = r / p.group, hd = r % p.group;       // the row's token of the tile and head of the group
         uint32_t j0 = 0, nb = 0;                 // units and this tile's blocks so far
-        uint32_t nm = 0;                         // masked blocks so far
         // A meeting of this tile's four warps, or of both tiles' eight. (An
         // mbarrier and not a named one, so that the wait is bounded.)
         uint32_t met[2] = {0u, 0u};
@@ -706,6 +657,16 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
             if (lane == 0) (xb + x).arrive();
             wait(xb + x, turn);
             __syncwarp();
+        };
+        // The exponentials by turns with the warp of the other tile that has the
+        // same scheduler, tile 0 first.
+        const Bar mine_b = turn + warp, yours_b = turn + (warp ^ 4);
+        auto await = [&](uint32_t u) {
+            if (t) wait(mine_b, u);
+            else if (u) wait(mine_b, u - 1);
+        };
+        auto pass = [&] {
+            if (lane == 0) yours_b.arrive();
         };
 #pragma unroll 1
         for (uint32_t k = 0;; ++k) {
@@ -723,31 +684,29 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     const uint32_t key0 = first_key + i * kPaKeys, jv = j0 + 2 * i + 1;
                     const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;   // (pa_masked)
                     const uint32_t ja = lo > key0 ? lo - key0 : 0u, jb = hi > key0 ? hi - key0 : 0u;       // columns [ja, jb)
-                    uint4* const vt = reinterpret_cast<uint4*>(smem + SM::KV + jv % ST * SM::TILE);
-                    float x[2][32];              // 32 scores at hand, the next 32 on their way
-                    auto hide = [&](float* y, int c) {           // those of columns 32 c .. that the row may not see
-                        auto below = [](uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-                        const uint32_t from = ja > c * 32u ? ja - c * 32u : 0u, to_ = jb > c * 32u ? jb - c * 32u : 0u, open = below(to_) & ~below(from);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!(open >> j & 1u)) y[j] = -INFINITY;
-                    };
-                    wait(sf + t, nb + i);
+                    uint4* const vt = reinterpret_cast<uint4*>(smem + SM::KV + jv % ST * SM::BLOCK);
+                    const uint32_t n = nb + i, tp = ts + n % 2 * 64;             // the block's scores, and then its probabilities
+                    float x[kPaKeys];
+                    wait(sf + t * 2 + n % 2, n / 2);
                     tc_fence_after();
-                    tmem_ld32(ts, x[0]);
+                    tmem_ld32(tp, x);
+                    tmem_ld32(tp + 32, x + 32);
                     tmem_ld_wait();
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {            // bits of the 32 columns in [ja, jb)
+                            auto below = [](uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+                            const uint32_t from = ja > c * 32u ? ja - c * 32u : 0u, to_ = jb > c * 32u ? jb - c * 32u : 0u, open = below(to_) & ~below(from);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(open >> j & 1u)) x[c * 32 + j] = -INFINITY;
+                        }
+                    }
                     float mq[8];                 // eight chains: the maximum's latency is the softmax warps' to wait for
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mq[j] = -INFINITY;
+                    for (int j = 0; j < 8; ++j) mq[j] = fmaxf(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float* y = x[c & 1];
-                        tmem_ld32(ts + (c + 1) % 4 * 32, x[(c + 1) & 1]);        // (after the last the first again, for the exponentials)
-                        if (masked) hide(y, c);
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) mq[j / 2 % 8] = fmaxf(fmaxf(mq[j / 2 % 8], y[j]), y[j + 1]);
-                        tmem_ld_wait();
-                    }
+                    for (int j = 16; j < int(kPaKeys); j += 2) mq[j / 2 % 8] = fmaxf(fmaxf(mq[j / 2 % 8], x[j]), x[j + 1]);
 #pragma unroll
                     for (int w = 4; w; w >>= 1)
 #pragma unroll
@@ -759,7 +718,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     if (__any_sync(0xffffffffu, move)) {
                         const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - mx) * sl);
                         if (i) {
-                            wait(of + t, nb + i - 1);
+                            wait(of + t * 2 + (n - 1) % 2, (n - 1) / 2);
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < HP; c += 16) {
@@ -780,37 +739,43 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     // has keys that not every row may see: was there one?
                     bool odd = false;
                     if (masked) {
-                        wait(vc + nm % 4, nm / 4);
-                        odd = __any_sync(0xffffffffu, (odds + nm++ % 4).get());
+                        wait(kvf + jv % ST, jv / ST);            // (its scores are there: the stage's earlier loads are long done)
+                        const __nv_bfloat162 zero = __float2bfloat162_rn(0.0f);
+                        __nv_bfloat162 acc[4] = {zero, zero, zero, zero};
+#pragma unroll 4
+                        for (uint32_t q = r; q < SM::BLOCK / 16; q += 128) {     // 0 times one of those is a NaN
+                            const uint4 v = vt[q];
+                            acc[0] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v.x), zero, acc[0]);
+                            acc[1] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v.y), zero, acc[1]);
+                            acc[2] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v.z), zero, acc[2]);
+                            acc[3] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v.w), zero, acc[3]);
+                        }
+                        const __nv_bfloat162 all = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
+                        const bool mine = __any_sync(0xffffffffu, __hisnan(all.x) || __hisnan(all.y));
+                        const Word w = odds + (met[0] & 1) * 8 + t * 4;
+                        if (lane == 0) (w + (warp & 3)).set(mine);
+                        meet(false);
+                        odd = (w + 0).get() | (w + 1).get() | (w + 2).get() | (w + 3).get();
                     }
                     const float ml = m == -INFINITY ? 0.0f : m * sl;
                     const uint64_t sl2 = pack2(sl, sl), ml2 = pack2(-ml, -ml);
                     uint64_t sums[2] = {0ull, 0ull};
+                    await(j0 / 2 + i);
                     if (i == 0 && r == 0) (begun + t).set(odd);        // the product then adds to what the rows put there
-                    auto give = [&](Bar b) {               // what this warp has put into tensor memory, to the MMA warp
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) b.arrive();
-                    };
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float* y = x[c & 1];
-                        if (c < 3) tmem_ld32(ts + (c + 1) * 32, x[(c + 1) & 1]);
-                        if (masked) hide(y, c);
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
                             float u, v;
-                            unpack2(fma2(pack2(y[2 * k], y[2 * k + 1]), sl2, ml2), u, v);
+                            unpack2(fma2(pack2(x[c * 32 + 2 * k], x[c * 32 + 2 * k + 1]), sl2, ml2), u, v);
                             u = ex2(u);
                             v = ex2(v);
                             sums[k % 2] = add2(sums[k % 2], pack2(u, v));
                             w[k] = cvt_bf16x2(u, v);
                         }
-                        if (c < 3) tmem_ld_wait();
-                        tmem_st16(ts + c * 16, w);               // (over scores that have been read)
-                        if (c == 2 && !odd) give(pr + t);        // three quarters of the block's product can start
+                        if (c == 1) pass();
+                        tmem_st16(tp + c * 16, w);               // (over scores that have been read)
                     }
                     if (odd) {
                         // Rare. Each row adds its own share of the infinities and
@@ -818,7 +783,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         // shared tile, for both tiles' products.
                         tmem_st_wait();
                         if (i) {
-                            wait(of + t, nb + i - 1);
+                            wait(of + t * 2 + (n - 1) % 2, (n - 1) / 2);
                             tc_fence_after();
                         }
 #pragma unroll 1
@@ -832,13 +797,13 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                                 for (int k = 0; k < 16; ++k) o[k] = 0.0f;
                             }
 #pragma unroll 1
-                            for (uint32_t j = 0; j < 128; ++j) {
-                                const uint32_t pp = __float_as_uint(tmem_ld1(ts + j / 2));
+                            for (uint32_t j = 0; j < kPaKeys; ++j) {
+                                const uint32_t pp = __float_as_uint(tmem_ld1(tp + j / 2));
                                 const float x = __uint_as_float(j & 1 ? pp & 0xffff0000u : pp << 16);
                                 if (j < ja || j >= jb) continue;
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {    // 8 columns: one swizzled 16-byte piece of key j's row
-                                    const uint4 v = vt[c / 64 * 1024 + j * 8 + (((c % 64) / 8 + h) ^ (j & 7))];
+                                    const uint4 v = vt[c / 64 * 512 + j * 8 + (((c % 64) / 8 + h) ^ (j & 7))];
                                     const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                                     for (int k = 0; k < 4; ++k) {
@@ -855,7 +820,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         }
                         meet(both);  // all rows of both tiles have read them
 #pragma unroll 1
-                        for (uint32_t k = both ? tid : r; k < SM::TILE / 16; k += both ? 256 : 128) {
+                        for (uint32_t k = both ? tid : r; k < SM::BLOCK / 16; k += both ? 256 : 128) {
                             uint4 x = vt[k];
                             uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -871,12 +836,17 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     float sum_x, sum_y;
                     unpack2(add2(sums[0], sums[1]), sum_x, sum_y);
                     l += sum_x + sum_y;
-                    if (odd) give(pr + t);
-                    give(pl + t);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) (pr + t * 2 + n % 2).arrive();
                 }
                 nb += nt;
             }
-            for (uint32_t i = nt; i < im.cnt[t ^ 1]; ++i) nm += pa_masked(im, i);
+            for (uint32_t i = nt; i < im.cnt[t ^ 1]; ++i) {
+                await(j0 / 2 + i);
+                pass();
+            }
             j0 += 2 * max(im.cnt[0], im.cnt[1]);
             // Rows go out through shared memory, 128 bytes of each at a time:
             // eight lanes a row, four whole lines an instruction (a thread
@@ -899,50 +869,43 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 p.stat[at] = make_float2(m, nt ? l : 0.0f);
             }
             if (nt) {
-                wait(of + t, nb - 1);
+                wait(of + t * 2 + (nb - 1) % 2, (nb - 1) / 2);
                 tc_fence_after();
             }
             const uint32_t row_bytes = whole ? a.head_dim * 2 : HP * 4;
 #pragma unroll 1
             for (uint32_t c = 0; c * 128 < row_bytes; ++c) {     // 64 columns of the result, or 32 of a part
-                uint4 w[8];
-                if (whole) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float o[32];
-                        if (nt) {
-                            tmem_ld32(to + c * 64 + h * 32, o);
-                            tmem_ld_wait();
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            w[h * 4 + k] = keys ? make_uint4(cvt_bf16x2(o[8 * k] * l, o[8 * k + 1] * l), cvt_bf16x2(o[8 * k + 2] * l, o[8 * k + 3] * l),
-                                                             cvt_bf16x2(o[8 * k + 4] * l, o[8 * k + 5] * l), cvt_bf16x2(o[8 * k + 6] * l, o[8 * k + 7] * l))
-                                                : make_uint4(0u, 0u, 0u, 0u);
-                    }
-                } else if (nt) {
-                    float o[32];
-                    tmem_ld32(to + c * 32, o);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        w[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
-                }
                 __syncwarp();                    // (the last round's have been read)
+#pragma unroll 1
+                for (uint32_t h = 0; h < (whole ? 2u : 1u); ++h) {
+                    float o[32];
+                    if (nt) {
+                        tmem_ld32(to + (whole ? c * 64 + h * 32 : c * 32), o);
+                        tmem_ld_wait();
+                    }
+                    if (whole) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) out[lane * 8 + (k ^ (lane & 7))] = w[k];
+                        for (uint32_t k = 0; k < 4; ++k)
+                            out[lane * 8 + ((h * 4 + k) ^ (lane & 7))] =
+                                keys ? make_uint4(cvt_bf16x2(o[8 * k] * l, o[8 * k + 1] * l), cvt_bf16x2(o[8 * k + 2] * l, o[8 * k + 3] * l),
+                                                  cvt_bf16x2(o[8 * k + 4] * l, o[8 * k + 5] * l), cvt_bf16x2(o[8 * k + 6] * l, o[8 * k + 7] * l))
+                                     : make_uint4(0u, 0u, 0u, 0u);
+                    } else if (nt) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k)
+                            out[lane * 8 + (k ^ (lane & 7))] =
+                                make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+                    }
+                }
                 __syncwarp();
-                uint8_t* at[8];
                 const uint32_t byte = c * 128 + piece * 16;
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
+                for (uint32_t g = 0; g < 8; ++g) {
                     const uint32_t from = g * 4 + row;
-                    at[g] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
-                    w[g] = out[from * 8 + (piece ^ (from & 7))];
+                    uint8_t* const at = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
+                    const uint4 w = out[from * 8 + (piece ^ (from & 7))];
+                    if (at && byte < row_bytes) *reinterpret_cast<uint4*>(at + byte) = w;
                 }
-#pragma unroll
-                for (int g = 0; g < 8; ++g)
-                    if (at[g] && byte < row_bytes) *reinterpret_cast<uint4*>(at[g] + byte) = w[g];
             }
             tc_fence_before();                   // (the sums have been read: the next pr says so)
             __syncwarp();
