@@ -53,6 +53,39 @@ constexpr int kKwRows = 8, kKwThreads = 256;
 struct Kv4RowPlace {
     uint32_t page, slot, pos;                    // page ~0: nowhere
 };
+// The units of a CTA's rows that a group of four lanes takes, every
+// kKwThreads / 4th.
+struct Kv4Units {
+    uint32_t units, rows, lg, dr, du;            // per row; rows here; log2 of the groups; a step in rows and units
+    uint32_t row, u;
+    SMOE_DEVINL Kv4Units(const Kv4Geom& G, uint32_t heads, uint32_t total) {
+        constexpr uint32_t step = kKwThreads / 4;
+        units = heads * 2 * G.ng;
+        rows = min(uint32_t(kKwRows), total - blockIdx.x * kKwRows);
+        lg = G.ng >> 1;                          // (1 or 2 groups)
+        dr = step / units;
+        du = step % units;
+        row = (threadIdx.x >> 2) / units;
+        u = (threadIdx.x >> 2) % units;
+    }
+    SMOE_DEVINL bool more() const { return row < rows; }
+    SMOE_DEVINL uint32_t g() const { return u & ((1u << lg) - 1u); }
+    SMOE_DEVINL uint32_t kv() const { return u >> lg & 1u; }
+    SMOE_DEVINL uint32_t h() const { return u >> (lg + 1); }
+    // element of the row's k or v where this lane's 16 values start
+    SMOE_DEVINL size_t at(const SmoeKv4Rows& r) const {
+        const size_t w = blockIdx.x * kKwRows + row;
+        return (kv() ? w * r.v_row + h() * r.v_head : w * r.k_row + h() * r.k_head) + g() * 64 + (threadIdx.x & 3) * 16;
+    }
+    SMOE_DEVINL void next() {
+        row += dr;
+        u += du;
+        if (u >= units) {
+            u -= units;
+            ++row;
+        }
+    }
+};
 // The places of the CTA's rows, a warp a row; entry = base[s] + index in the sequence.
 SMOE_DEVINL void kv4_places(const Kv4Args& a, const SmoeKv4Rows& r, const uint32_t* base, Kv4RowPlace* places) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kKwRows + warp, ns = a.c.n_seqs;
@@ -118,30 +151,49 @@ static __device__ __noinline__ uint32_t kv4_code(float x, float bias, float scal
     const float q = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x, bias), scale)) : 0.0f;
     return uint32_t(fminf(fmaxf(q, 0.0f), 15.0f));
 }
-// Those of 16 values, without dividing: with d = x - bias, the code nearest to
-// d / scale by way of the reciprocal is right or off by one. r scale (4 + 8
-// bits) and u = d - r scale are exact, so 2 |u| against scale says which, ties
+// Those of 16 values, without dividing: with d = x - bias, the whole number r
+// nearest to d / scale by way of the reciprocal is right or off by one. For r
+// of -1 .. 16 (others are cut to 0 or 15) r scale (5 + 8 bits) and
+// u = d - r scale are exact, so |u| against scale / 2 says which, ties
 // included: fl(d / scale) is exactly half-way only where d is (2 r + 1) scale / 2
 // - neighbours of that number in fp32 are further from it than half a unit of
-// the quotient. (bf16 values hit ties often: some in every second warp.)
+// the quotient. (bf16 values hit ties often: some in every second warp.) |u|
+// and scale / 2 are compared as integers, |u| one unit up where r is odd, which
+// moves ties to even. Infinities and NaN: d / scale is infinite or NaN then,
+// which r takes to a value past 15 or (NaN too) to -1.
 SMOE_DEVINL void kv4_codes16(const float* y, float bias, float scale, uint32_t* code) {
     code[0] = code[1] = 0u;
-    if (!(scale >= 1e-37f)) {                    // no finite reciprocal, or no positive scale
+    if (!(scale >= 1e-37f && scale <= 3e38f)) {  // no finite reciprocal, or no positive scale
         if (scale > 0.0f)
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int k = 0; k < 16; ++k) code[k / 8] |= kv4_code(y[k], bias, scale) << (4 * (k % 8));
+                for (int i = 0; i < 8; ++i) code[k] |= kv4_code(k ? y[8 + i] : y[i], bias, scale) << (4 * i);
         return;
     }
     const float inv = 1.0f / scale, magic = 12582912.0f;         // 1.5 x 2^23: adding it rounds to a whole number, in the low bits
+    const uint64_t off = pack2(-bias, -bias), inv2 = pack2(inv, inv), up = pack2(magic, magic), down = pack2(-magic, -magic), step = pack2(-scale, -scale);
+    const int half = __float_as_int(0.5f * scale);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const float d = __fsub_rn(y[k], bias), t = fminf(fmaxf(d * inv, 0.0f), 15.0f) + magic;
-        const float u = fmaf(-(t - magic), scale, d), v = fabsf(u + u);
-        const uint32_t r = __float_as_uint(t) & 15u;
-        const bool off = v > scale || (v == scale && (r & 1u));
-        const int c = int(r) + (off ? (u > 0.0f ? 1 : -1) : 0);
-        code[k / 8] |= uint32_t(max(0, min(15, c))) << (4 * (k % 8));
-    }
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int k = 6; k >= 0; k -= 2) {
+            const uint64_t d = add2(pack2(y[8 * w + k], y[8 * w + k + 1]), off);
+            float t[2], u[2];
+            unpack2(fma2(d, inv2, up), t[0], t[1]);
+            int c[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) t[i] = fmaxf(t[i], magic - 1.0f);
+            unpack2(fma2(add2(pack2(t[0], t[1]), down), step, d), u[0], u[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                c[i] = __float_as_int(t[i]) - __float_as_int(magic);
+                const int v = (__float_as_int(u[i]) & 0x7fffffff) + (c[i] & 1);
+                if (v > half) c[i] += __float_as_int(u[i]) >> 31 | 1;
+            }
+            // (cut to 0 .. 15 and put below the pairs so far)
+            asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %3;" : "=r"(code[w]) : "r"(c[1]), "r"(c[0]), "r"(code[w]));
+        }
 }
 
 template <int DTYPE, bool WIDE>
@@ -150,17 +202,12 @@ __global__ void __launch_bounds__(kKwThreads, 4) k_kv4_append(Kv4Args a, SmoeKv4
     pdl_release();
     pdl_acquire();
     const Kv4Geom G(a.c.head_dim);
-    const uint32_t quad = threadIdx.x >> 2, j = threadIdx.x & 3, units = a.c.num_kv_heads * 2 * G.ng, row0 = blockIdx.x * kKwRows;
-    const uint32_t all = min(uint32_t(kKwRows), r.total - row0) * units;
-    constexpr uint32_t STEP = kKwThreads / 4;
+    const uint32_t j = threadIdx.x & 3;
     float x[2][16];
-    auto load = [&](uint32_t i, float* y) {
-        const uint32_t row = row0 + i / units, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
-        kv4_load16<DTYPE, WIDE>(kv ? r.v : r.k, (kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head) + g * 64 + j * 16, y);
-    };
-    auto store = [&](uint32_t i, const float* y) {
-        const uint32_t u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
-        const Kv4RowPlace p = places[i / units];
+    auto load = [&](const Kv4Units& w, float* y) { kv4_load16<DTYPE, WIDE>(w.kv() ? r.v : r.k, w.at(r), y); };
+    auto store = [&](const Kv4Units& w, const float* y) {
+        const uint32_t g = w.g(), kv = w.kv(), h = w.h();
+        const Kv4RowPlace p = places[w.row];
         float lo = y[0], hi = y[0];
 #pragma unroll
         for (int k = 1; k < 16; ++k) {
@@ -191,15 +238,18 @@ __global__ void __launch_bounds__(kKwThreads, 4) k_kv4_append(Kv4Args a, SmoeKv4
             }
         }
     };
-    if (quad < all) load(quad, x[0]);
-    if (quad + STEP < all) load(quad + STEP, x[1]);
+    Kv4Units w(G, a.c.num_kv_heads, r.total), ahead = w;
+    if (w.more()) load(w, x[0]);
+    ahead.next();
+    if (ahead.more()) load(ahead, x[1]);
     kv4_places(a, r, a.c.len, places);
 #pragma unroll 1
-    for (uint32_t i = quad; i < all; i += STEP) {
-        store(i, x[0]);
+    for (; w.more(); w.next()) {
+        store(w, x[0]);
 #pragma unroll
         for (int k = 0; k < 16; ++k) x[0][k] = x[1][k];
-        if (i + 2 * STEP < all) load(i + 2 * STEP, x[1]);
+        ahead.next();
+        if (ahead.more()) load(ahead, x[1]);
     }
 }
 
@@ -209,21 +259,24 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
     pdl_release();
     pdl_acquire();
     const Kv4Geom G(a.c.head_dim);
-    const uint32_t quad = threadIdx.x >> 2, j = threadIdx.x & 3, units = a.c.num_kv_heads * 2 * G.ng, row0 = blockIdx.x * kKwRows;
-    const uint32_t all = min(uint32_t(kKwRows), r.total - row0) * units;
-    constexpr uint32_t STEP = kKwThreads / 4;
+    const uint32_t j = threadIdx.x & 3;
     kv4_places(a, r, first, places);
+    Kv4Units w(G, a.c.num_kv_heads, r.total);
 #pragma unroll 1
-    for (uint32_t i0 = quad; i0 < all; i0 += 2 * STEP) {
+    while (w.more()) {
+        Kv4Units at[2] = {w, w};
+        at[1].next();
+        w = at[1];
+        w.next();
         uint2 code[2];
         uint32_t sb[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const uint32_t i = i0 + q * STEP, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
+            const uint32_t g = at[q].g(), kv = at[q].kv(), h = at[q].h();
             code[q] = make_uint2(0u, 0u);
             sb[q] = 0u;
-            if (i >= all) continue;
-            const Kv4RowPlace p = places[i / units];
+            if (!at[q].more()) continue;
+            const Kv4RowPlace p = places[at[q].row];
             if (p.page == ~0u) continue;
             const uint8_t* blk = a.c.blocks + (size_t(p.page) * a.c.num_kv_heads + h) * G.block;
             code[q] = ld_plain(reinterpret_cast<const uint2*>(blk + G.codes(kv, g) + p.slot * 32 + j * 8));
@@ -231,18 +284,16 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const uint32_t i = i0 + q * STEP, u = i % units, g = u % G.ng, kv = u / G.ng & 1, h = u / (2 * G.ng);
-            if (i >= all || places[i / units].page == ~0u) continue;
+            if (!at[q].more() || places[at[q].row].page == ~0u) continue;
             const float scale = __uint_as_float(sb[q] << 16), bias = __uint_as_float(sb[q] & 0xffff0000u);
             float v[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k)
                 v[k] = __fadd_rn(__fmul_rn(float((k < 8 ? code[q].x : code[q].y) >> (4 * (k % 8)) & 15u), scale), bias);
-            const uint32_t row = row0 + i / units;
-            const size_t at = (kv ? row * r.v_row + h * r.v_head : row * r.k_row + h * r.k_head) + g * 64 + j * 16;
-            void* dst = kv ? r.v : r.k;
+            const size_t to = at[q].at(r);
+            void* dst = at[q].kv() ? r.v : r.k;
             if (DTYPE == SMOE_DTYPE_F32) {
-                float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + at);
+                float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + to);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) d[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 continue;
@@ -251,11 +302,11 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(v[2 * k], v[2 * k + 1]);
             if (WIDE) {
-                uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at);
+                uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + to);
                 d[0] = make_uint4(w[0], w[1], w[2], w[3]);
                 d[1] = make_uint4(w[4], w[5], w[6], w[7]);
             } else {
-                uint2* d = reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + at);
+                uint2* d = reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + to);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) d[k] = make_uint2(w[2 * k], w[2 * k + 1]);
             }

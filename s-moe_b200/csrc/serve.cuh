@@ -65,4 +65,22 @@ SMOE_DEVINL uint32_t seq_of_row(const uint32_t* cu, uint32_t n, uint32_t row, ui
     return (span == 1 && ld_plain(cu + lo) <= row && row < ld_plain(cu + lo + 1)) ? lo : n;
 }
 
+// Two fp32 operations in one instruction.
+SMOE_DEVINL uint64_t pack2(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+SMOE_DEVINL void unpack2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+SMOE_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+SMOE_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 }  // namespace smoe
