@@ -45,9 +45,11 @@ SMOE_DEVINL uint32_t kv4_page(const SmoeKv4Cache& c, uint32_t s, uint64_t e, uin
 // maximum two shuffles. Values are fetched before the entries are known, and
 // two units a lane are in flight. Bound by the chain of look-ups (bounds,
 // length, page table) for a step's rows (256 fp32 rows of 4 heads of 128: 7 us,
-// their read-back 6, both cold) and by the instructions that find the codes
-// for a prompt's (5,800 bf16 rows: 17 us cold, half of the issue slots used).
-// With a division for each code and two lanes a unit those took 10 and 26 us.
+// their read-back 6, both cold) and by that chain and the instructions that
+// find the codes for a prompt's (5,800 bf16 rows: 14 us cold, 54% of the issue
+// slots used; 14,400 entries read back: 16 us). With a division for each code
+// and two lanes a unit the first took 10 us, the third 26. (16 or 32 rows a
+// CTA, so that all CTAs fit the GPU at once, took 1.1 and 1.3 times as long.)
 constexpr int kKwRows = 8, kKwThreads = 256;
 
 struct Kv4RowPlace {

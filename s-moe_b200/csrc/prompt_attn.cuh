@@ -113,11 +113,6 @@ struct alignas(16) PaItem {
     uint16_t more, pad;                          // 0: there was no further item
 };
 static_assert(sizeof(PaItem) == 64, "an item's place in shared memory");
-// Whether some row of the pair may not see some key of the item's block i.
-SMOE_DEVINL bool pa_masked(const PaItem& it, uint32_t i) {
-    const uint32_t key0 = it.key0 + i * kPaKeys;
-    return key0 + kPaKeys > it.inner_hi || key0 < it.inner_lo;
-}
 struct PaWalk {
     PaPlace at, end;
     bool single;                                 // just the pair at `at`
@@ -413,8 +408,8 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint32_t base = smem_u32(smem);
     const Bar qf{base + SM::BAR}, qe = qf + 2, sf = qf + 4, pr = qf + 8, of = qf + 12, itf = qf + 16, ite = itf + kPaItems,
               xb = ite + kPaItems, turn = xb + 3, kvf = turn + 8, kve = kvf + ST;
-    const Word fail{(kve + ST).a}, begun = fail + 1, odds = fail + 4;          // begun[t]: the accumulator holds something before block 0's P V
-    uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + SM::BAR + ((kve + ST).a - qf.a)) + 3;  // odds: a word of each softmax warp, by turns in two
+    const Word fail{(kve + ST).a}, begun = fail + 1, odds = fail + 4;          // begun[t]: the accumulator holds something before block 0's P V; odds: a word of each softmax warp, by turns in two
+    uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + SM::BAR + ((kve + ST).a - qf.a)) + 3;
     PaItem* const items = reinterpret_cast<PaItem*>(smem + SM::ITEMS);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const SmoeCudaPackedAttnArgs& a = p.a;
@@ -486,7 +481,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                         tma_load3(base + SM::KV + st * SM::BLOCK + h * 8192, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
                 }
             }
-            // nothing may be in flight when the CTA ends (the MMA warp has
+            // nothing may be in flight when the CTA ends (the MMA lanes have
             // waited for all of it unless a wait ran out)
 #pragma unroll 1
             for (uint32_t k = j > ST ? j - ST : 0; k < j; ++k) pa_drain(kvf + k % ST, (k / ST) & 1);
@@ -665,7 +660,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll 1
                 for (uint32_t i = 0; i < nt; ++i) {
                     const uint32_t key0 = first_key + i * kPaKeys, jv = j0 + 2 * i + 1;
-                    const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;   // (pa_masked)
+                    const bool masked = key0 + kPaKeys > inner_hi || key0 < inner_lo, both = i < cnt_o;   // some row of the pair may not see some key of the block
                     const uint32_t ja = lo > key0 ? lo - key0 : 0u, jb = hi > key0 ? hi - key0 : 0u;       // columns [ja, jb)
                     uint4* const vt = reinterpret_cast<uint4*>(smem + SM::KV + jv % ST * SM::BLOCK);
                     const uint32_t n = nb + i, tp = ts + n % 2 * 64;             // the block's scores, and then its probabilities
