@@ -1025,19 +1025,20 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     (a ballot each, lane i keeps the i-th), counts free entries below `keep`
 //     and kept ones past it, and - with what the warps and CTAs before it
 //     counted - lists both, ascending.
-//  4. The j-th kept entry goes to the j-th free one: a warp takes 32 moves,
-//     looks up their pages a lane each, and copies eight at a time, 128 bytes
+//  4. The j-th kept entry goes to the j-th free one: a warp takes up to 32
+//     moves (few moves go to many warps, eight each), looks up their pages a
+//     lane each, and copies eight at a time, 128 bytes
 //     of codes as a word a lane, scales, biases, pos and score another.
 //     Sources are past `keep` and targets below it: no move reads what
 //     another writes. (Separate outputs have pos and score of all entries
 //     below `keep` from step 1, before the moved ones' overwrite them.)
 // Bound by the chain of steps for short sequences (8 of 1,100 entries cut to
-// 1,024, 4 KV heads: 12.7 us) and by the moves for long ones (16 of 6,000 to
-// 32,768 cut to 4,096: 56 us, of which the selection takes 18; the moves'
-// 32-byte sectors pass at about 6 TB/s, as far as memory goes). One launch:
-// with a launch a step the first took 37 us, the second 244.
+// 1,024, 4 KV heads: 10.1 us; 12.7 with 32 moves a warp) and by the moves for
+// long ones (16 of 6,000 to 32,768 cut to 4,096: 56 us, of which the selection
+// takes 18; the moves' 32-byte sectors pass at about 6 TB/s, as far as memory
+// goes). One launch: with a launch a step the first took 37 us, the second 244.
 constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvDigits = 3;
-constexpr uint32_t kEvBins = 2048;
+constexpr uint32_t kEvBins = 2048, kEvCtas = 8;  // of a cluster, at most
 __host__ __device__ constexpr uint32_t kv4_evict_smem(uint32_t cached) { return (kEvDigits * kEvBins + cached) * 4; }
 
 // Exclusive sum over the threads of a CTA of two counts at once; totals in `all`.
@@ -1167,12 +1168,16 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
         uint32_t mine[4] = {0u, 0u, 0u, 0u};
         const uint32_t b = kEvBins - 4 - 4 * tid;
         static_assert(kEvBins == 4 * kEvThreads, "four bins a thread");
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(h, r) + b);
-            mine[0] += v.x;
-            mine[1] += v.y;
-            mine[2] += v.z;
-            mine[3] += v.w;
+        uint4 theirs[kEvCtas];                   // (all of them on their way at once)
+#pragma unroll
+        for (uint32_t r = 0; r < kEvCtas; ++r)
+            theirs[r] = r < ctas ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(h, r) + b) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (uint32_t r = 0; r < kEvCtas; ++r) {
+            mine[0] += theirs[r].x;
+            mine[1] += theirs[r].y;
+            mine[2] += theirs[r].z;
+            mine[3] += theirs[r].w;
         }
         uint2 all;
         uint32_t above = ev_scan(make_uint2(mine[0] + mine[1] + mine[2] + mine[3], 0u), warp_sums, warp, lane, all).x;
@@ -1204,7 +1209,8 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
         eq0 = __shfl_sync(0xffffffffu, ev_scan(make_uint2(lane == 0 ? equal : 0u, 0u), warp_sums, warp, lane, all).x, 0);
         if (tid == 0) counts[0] = all;
         cluster.sync();
-        for (uint32_t r = 0; r < rank; ++r) eq0 += cluster.map_shared_rank(counts, r)[0].x;
+#pragma unroll
+        for (uint32_t r = 0; r < kEvCtas; ++r) eq0 += r < rank ? cluster.map_shared_rank(counts, r)[0].x : 0u;
     }
     // masks of the words wb, wb + 1, .. that stay: lane i's of word wb + i
     uint32_t eq = eq0;
@@ -1243,8 +1249,9 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
     if (tid == 0) counts[1] = all;
     cluster.sync();
     uint32_t moves = 0;
-    for (uint32_t r = 0; r < ctas; ++r) {
-        const uint2 v = cluster.map_shared_rank(counts, r)[1];
+#pragma unroll
+    for (uint32_t r = 0; r < kEvCtas; ++r) {
+        const uint2 v = r < ctas ? cluster.map_shared_rank(counts, r)[1] : make_uint2(0u, 0u);
         if (r < rank) first.x += v.x, first.y += v.y;
         moves += v.y;
     }
@@ -1294,9 +1301,10 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
     uint8_t* rest_to = x < G.ng * 2 ? c.blocks + G.sb(0, 0) + x * kKvPage * 4
                        : x == G.ng * 2 ? reinterpret_cast<uint8_t*>(p.pos_out ? p.pos_out : c.pos)
                                        : reinterpret_cast<uint8_t*>(p.score_out ? p.score_out : c.score);
-    for (uint32_t m0 = (rank * kEvWarps + warp) * 32; m0 < moves; m0 += ctas * kEvWarps * 32) {
+    const uint32_t warps = ctas * kEvWarps, some_moves = min(32u, ((moves + warps - 1) / warps + 7) / 8 * 8);     // a warp's at a time
+    for (uint32_t m0 = (rank * kEvWarps + warp) * some_moves; m0 < moves; m0 += warps * some_moves) {
         uint32_t te = 0, fe = 0, tb = 0, fb = 0;
-        bool ok = m0 + lane < moves;
+        bool ok = lane < some_moves && m0 + lane < moves;
         if (ok) {
             te = to_list[m0 + lane];
             fe = from_list[m0 + lane];

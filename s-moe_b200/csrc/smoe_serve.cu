@@ -333,7 +333,7 @@ int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t ke
     const CtxView c = smoe::ctx_view(ctx);
     // CTAs of a pair: 8192 entries each, 8 at most; past what their shared memory holds keys are read again each time
     uint32_t ctas = 1;
-    while (ctas < 8 && uint64_t(ctas) * 8192 < max_len) ctas *= 2;
+    while (ctas < smoe::kEvCtas && uint64_t(ctas) * 8192 < max_len) ctas *= 2;
     const uint32_t cached = std::min<uint32_t>(49152, (max_len / ctas + 64 + 31) / 32 * 32);
     if (uint64_t(cache->num_kv_heads) * ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_ARG, "kv4_evict: too many KV heads", cache->num_kv_heads);
     if ((rc = smem_limit(c, smoe::k_kv4_evict, smoe::kv4_evict_smem(49152)))) return rc;
