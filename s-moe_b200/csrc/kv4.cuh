@@ -342,13 +342,14 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // part of (warp, pair) has the number warp + pair: along the line at least
 // one of the two grows from a part to the next, so no two share one.
 //
-// Bound by issue: 16 entries cost about 400 warp instructions (the codes'
-// unpacking on the integer units, the probabilities' pieces), 53% of the issue
-// slots with 12 warps an SM. Two contexts of 125,000 (head_dim 128, 32 / 4
-// heads, bf16, weights): 58 us of k_kv4_attention cold for 148 MB, 2.6 TB/s
-// (3.9 TB/s once the rings run; the start and the stretches' whole pages cost
-// about 14 us), and 8 us of k_kv4_join. 32 contexts of 512 to 8,192: 33 us
-// with the join; one of 300: 10.6 us, of which most is the two launches.
+// Bound by each warp's chain: 16 entries cost about 400 warp instructions (the
+// codes' unpacking on the integer units, the probabilities' pieces), a page
+// takes a warp 5 us, and the 12 warps an SM that their registers allow use 53%
+// of the issue slots. Two contexts of 125,000 (head_dim 128, 32 / 4 heads,
+// bf16, weights): 65 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
+// rings run; the first pages come in after 7 us, warps end between 37 and 56).
+// 32 contexts of 512 to 8,192: 33 us with the join; one of 300: 10.8 us, of
+// which most is the two launches.
 constexpr int kKaWarps = 4, kKaStages = 3;
 constexpr uint32_t kKaCtas = 3, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
 

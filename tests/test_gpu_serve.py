@@ -356,6 +356,28 @@ def test_kv4_append_nonfinite(ctx):
     assert not torch.isfinite(vo[bad_v]).any()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_kv4_append_magnitudes(ctx, dtype):
+    """Groups from subnormal to 1e37, groups far from zero, constant ones, whole numbers that end half-way between two codes."""
+    n = 200
+    c = Cache(2, 128, [n], 1, 10)
+    k = torch.randn(n, 2, 128, generator=c.g, device="cuda")
+    v = k * 10.0 ** torch.linspace(-44, 37, n, device="cuda")[:, None, None]
+    k[:40] = 1000 + k[:40] * 1e-3
+    k[40:80] = -7e5 + k[40:80] * 2
+    k[80:120] = torch.arange(128, device="cuda") % 31 - 4.0         # (scale 2: every other value is half-way)
+    k[120:130] = 3.25
+    k, v = k.to(dtype), v.to(dtype)
+    ctx.kv4_append(c.desc(), S.kv4_rows(k, v, starts([n])))
+    ko, vo = torch.zeros(n, 2, 128, device="cuda"), torch.zeros(n, 2, 128, device="cuda")
+    c.len += n
+    ctx.kv4_read(c.desc(), None, S.kv4_rows(ko, vo, starts([n])))
+    ctx.synchronize()
+    for x, o in ((k, ko), (v, vo)):
+        code, scale, bias = quantised(x)
+        assert torch.equal(o, (code * scale + bias).flatten(-2))
+
+
 def test_kv4_bad_pages_are_skipped(ctx):
     c = Cache(2, 64, [64, 64], 70, 9)
     c.fill(ctx)
@@ -452,6 +474,22 @@ def test_kv4_attention(ctx, dtype, case):
     assert torch.equal(out2, again) and torch.equal(so, so2)
     attn_run(ctx, c, q, max(lens), extra, score=True, decay=0.5, in_place=True)
     assert torch.equal(c.score[~rest], so[~rest]) and torch.equal(c.score[rest], old[rest])
+
+
+@pytest.mark.parametrize("lens", [[14300, 0, 14250, 3], [56900], [28500, 28400]])
+def test_kv4_attention_long_stretches(ctx, lens):
+    """Enough pages that every warp has eight or more: stretches of two lengths, which cut pairs at any page."""
+    Hkv = 32 if sum(lens) < 40000 else 16
+    c = Cache(Hkv, 64, lens, 1, 55)
+    c.fill(ctx)
+    assert sum((n + 63) // 64 for n in lens) * Hkv > 8 * 1776
+    q = torch.randn(len(lens), Hkv, 64, generator=c.g, device="cuda") * 2
+    c.score.copy_(torch.rand(c.score.shape, generator=c.g, device="cuda"))
+    old = c.score.clone()
+    out, so = attn_run(ctx, c, q, max(lens), score=True, decay=0.5)
+    attn_check(c, q, lens, out, so, old, 0.5)
+    again, so2 = attn_run(ctx, c, q, max(lens), score=True, decay=0.5)
+    assert torch.equal(out, again) and torch.equal(so, so2)
 
 
 @pytest.mark.parametrize("std", [0.0, 40.0])
