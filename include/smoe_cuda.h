@@ -557,7 +557,8 @@ typedef struct SmoeKv4Rows {
 } SmoeKv4Rows;
 /* Quantise the rows into the entries len[s], len[s] + 1, .. of each sequence:
  * bias = bf16(min), scale = bf16((max - min) * (1/15)), code =
- * clamp(round((x - bias) / scale), 0, 15) (0 when scale is not positive).
+ * clamp(round((x - bias) / scale), 0, 15) (0 when scale is not positive). A
+ * group with a NaN among its values is NaN as a whole.
  * pos (if given) gets seen[s], seen[s] + 1, ..; score (if given) 0. len and
  * seen stay. */
 int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4Rows* rows);

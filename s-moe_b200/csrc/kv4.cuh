@@ -148,6 +148,18 @@ SMOE_DEVINL void kv4_load16(const void* p, size_t at, float* x) {
     }
 }
 
+// Minimum and maximum that a NaN passes through (fminf and fmaxf drop it): a
+// group with a NaN has a NaN as its scale and bias, and reads back as NaN.
+SMOE_DEVINL float kv4_min(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+SMOE_DEVINL float kv4_max(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // The code of one value by the definition.
 static __device__ __noinline__ uint32_t kv4_code(float x, float bias, float scale) {
     const float q = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x, bias), scale)) : 0.0f;
@@ -213,14 +225,14 @@ __global__ void __launch_bounds__(kKwThreads, 4) k_kv4_append(Kv4Args a, SmoeKv4
         float lo = y[0], hi = y[0];
 #pragma unroll
         for (int k = 1; k < 16; ++k) {
-            lo = fminf(lo, y[k]);
-            hi = fmaxf(hi, y[k]);
+            lo = kv4_min(lo, y[k]);
+            hi = kv4_max(hi, y[k]);
         }
         const uint32_t mask = 0xfu << (threadIdx.x & 28);
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+            lo = kv4_min(lo, __shfl_xor_sync(mask, lo, o));
+            hi = kv4_max(hi, __shfl_xor_sync(mask, hi, o));
         }
         if (p.page == ~0u) return;
         const __nv_bfloat16 bb = __float2bfloat16_rn(lo);

@@ -1,0 +1,50 @@
+"""GPU tests of the long-context serving operators at their edges: strides,
+NaN in cache rows, scales of 0, row ranges outside their buffers, outliers
+among the cache's groups. Bars as in test_gpu_serve.py unless derived here."""
+import math
+
+import pytest
+import torch
+
+import smoe_cuda as S
+import test_gpu_serve as T
+from test_gpu_serve import BF16, F32, attn_run, ints, quantised, starts
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------- NaN in cache rows
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("other", [0.0, math.inf, -math.inf])
+def test_kv4_append_carries_nan(ctx, dtype, other):
+    """One NaN makes its whole group NaN (bias = min of the group), wherever it is and whatever else is there, and no other group."""
+    n = 64
+    c = T.Cache(2, 128, [n], 1, 500)
+    k, v = ((torch.randn(n, 2, 128, generator=c.g, device="cuda")).to(dtype) for _ in range(2))
+    for i in range(n):                   # each place of a group, both groups, heads and sides
+        k[i, i % 2, 64 + i] = math.nan
+        v[i, 1 - i % 2, i] = -math.nan
+        if other:
+            k[i, i % 2, 64 + (i + 17) % 64] = other
+    ctx.kv4_append(c.desc(), S.kv4_rows(k, v, starts([n])))
+    ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+    ctx.kv4_read(c.desc(), None, S.kv4_rows(ko, vo, starts([n])))
+    ctx.synchronize()
+    for x, o in ((k, ko), (v, vo)):
+        bad = x.isnan().unflatten(-1, (2, 64)).any(-1, keepdim=True).expand(-1, -1, -1, 64).flatten(-2)
+        assert bad.sum() == 64 * n and o[bad].isnan().all()
+        code, scale, bias = quantised(x)
+        assert torch.equal(o[~bad], (code * scale + bias).flatten(-2).to(dtype)[~bad])
+
+
+def test_kv4_attention_over_a_nan(ctx):
+    """A NaN among the keys makes its KV head's results NaN, among the values those of its group; nothing else."""
+    c = T.Cache(2, 128, [300], 1, 501)
+    k, v = (torch.randn(300, 2, 128, generator=c.g, device="cuda") for _ in range(2))
+    k[200, 0, 5] = math.nan
+    v[100, 1, 70] = math.nan
+    ctx.kv4_append(c.desc(), S.kv4_rows(k, v, starts([300])))
+    c.len += 300
+    q = torch.randn(1, 8, 128, generator=c.g, device="cuda")
+    out, _ = attn_run(ctx, c, q, 300)
+    assert out[0, :4].isnan().all() and out[0, 4:, 64:].isnan().all() and torch.isfinite(out[0, 4:, :64]).all()
