@@ -377,6 +377,7 @@ struct Kv4Attn {
     float* logits;                               // [n_seqs][num_heads][rows] log2-scaled scores, with weights
     uint32_t rows;                               // max_len rounded up to a page
     float scale_log2;                            // positive
+    int most_e;                                  // largest power of two that q may go in with
 };
 
 // Entries of sequence s that the token attends to.
@@ -612,8 +613,9 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // 2^e with mx 2^e in [2^14, 2^15), kept within what fp32 can invert (an infinity or NaN in q stays one)
-            const int e = max(-100, min(100, 14 - (int(__float_as_uint(mx) >> 23) - 127)));
+            // 2^e with mx 2^e in [2^14, 2^15), kept within what fp32 can invert (an infinity or NaN in q stays one) and
+            // low enough for scale_log2 / 2^e to be a normal number: at 0 it would make NaN of the masked scores
+            const int e = max(-100, min(p.most_e, 14 - (int(__float_as_uint(mx) >> 23) - 127)));
             const float by = __uint_as_float(uint32_t(127 + e) << 23), inv = p.scale_log2 * __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {

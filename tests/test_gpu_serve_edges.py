@@ -48,3 +48,33 @@ def test_kv4_attention_over_a_nan(ctx):
     q = torch.randn(1, 8, 128, generator=c.g, device="cuda")
     out, _ = attn_run(ctx, c, q, 300)
     assert out[0, :4].isnan().all() and out[0, 4:, 64:].isnan().all() and torch.isfinite(out[0, 4:, :64]).all()
+
+
+# ------------------------------------------------------------------ scales of 0
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, 1e-37, 1e-20, 0.05])
+def test_kv4_attention_small_scales(ctx, dtype, scale):
+    """Equal probabilities at a scale of 0, for zero, tiny and ordinary queries, with lengths that end inside a page, and their weights."""
+    lens = [1, 63, 65, 200, 1000]
+    c = T.Cache(2, 64, lens, 1, 510)
+    c.fill(ctx)
+    q = torch.randn(len(lens), 16, 64, generator=c.g, device="cuda")
+    q[:, 0] = 0
+    q[:, 1] *= 1e-12
+    q[:, 2] *= 1e-30
+    q[:, 3] *= 1e-42
+    q = q.to(dtype)
+    out, so = torch.full_like(q, math.nan), torch.full_like(c.score, -1.0)
+    args = S.kv4_attn_args(q, out, max(lens), scale=scale, score_out=so, decay=0.0)
+    ws = torch.full((S.kv4_attention_workspace(c.desc(), args),), 255, dtype=torch.uint8, device="cuda")
+    ctx.kv4_attention(c.desc(), S.kv4_attn_set_workspace(args, ws))
+    ctx.synchronize()
+    assert torch.isfinite(out).all()
+    for b, n in enumerate(lens):
+        k, v = c.values(b, n)
+        p = torch.softmax(torch.einsum("kgd,nkd->kgn", q[b].double().view(2, -1, 64), k) * scale, -1)
+        want, mag = (torch.einsum("kgn,nkd->kgd", p, x).reshape(16, 64) for x in (v, v.abs()))
+        assert ((out[b].double() - want).abs() <= 2 ** -14 * mag + (2 ** -8 * want.abs() if dtype == BF16 else 0)).all()
+        page, slot = c.at(b, n)
+        w = p.sum(1).t()
+        assert ((so[page, :, slot].double() - w).abs() <= 2e-5 * (w + p.sum(1).max())).all()
