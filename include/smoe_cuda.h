@@ -544,7 +544,9 @@ typedef struct SmoeKv4Cache {
 /* Bytes of one page of one KV head; 0 for an unsupported head_dim. */
 uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim);
 
-/* Packed K and V rows: sequence s has the rows [cu[s], cu[s+1]). Row r of KV
+/* Packed K and V rows: sequence s has the rows [cu[s], cu[s+1]), cu ascending;
+ * a sequence whose range is not within `total` rows is skipped as a whole, and
+ * rows past the last sequence's are left alone. Row r of KV
  * head h of k starts at element r * k_row + h * k_head; strides multiples of
  * 4, bases 16-byte aligned, head_dim contiguous. */
 typedef struct SmoeKv4Rows {
@@ -615,7 +617,8 @@ int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t ke
 
 /* End of a step, once for all layers: len[s] = min(len[s] + n, keep) (keep 0:
  * no limit) and seen[s] += n (seen optional), n = cu[s+1] - cu[s], or
- * n_each when cu is NULL. */
+ * n_each when cu is NULL. It knows no buffers: after a call that skipped rows
+ * or entries (SMOE_ERR_DEVICE) the lengths count them all the same. */
 int smoe_cuda_kv4_advance(SmoeCudaCtx* ctx, uint32_t* len, uint32_t* seen, uint32_t n_seqs,
                           const uint32_t* cu, uint32_t n_each, uint32_t keep);
 

@@ -88,17 +88,34 @@ struct Kv4Units {
         }
     }
 };
+// Sequence of a row where seq_of_row finds none: past the last one's rows, or
+// starts that do not ascend, of which it may miss the row's. By one warp.
+static __device__ __noinline__ uint32_t kv4_seq_by_scan(const uint32_t* cu, uint32_t n, uint32_t row, uint32_t lane) {
+    for (uint32_t b = 0; b < n; b += 32) {
+        const uint32_t s = b + lane;
+        const uint32_t hit = __ballot_sync(0xffffffffu, s < n && ld_plain(cu + s) <= row && row < ld_plain(cu + s + 1));
+        if (hit) return b + __ffs(hit) - 1;
+    }
+    return n;
+}
 // The places of the CTA's rows, a warp a row; entry = base[s] + index in the sequence.
 SMOE_DEVINL void kv4_places(const Kv4Args& a, const SmoeKv4Rows& r, const uint32_t* base, Kv4RowPlace* places) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * kKwRows + warp, ns = a.c.n_seqs;
     Kv4RowPlace p{~0u, 0u, 0u};
+    // Each CTA reports on some of the sequences' ranges (one that is bad may have no row here): fetched first, looked at last
+    const uint32_t mine = blockIdx.x * kKwThreads + threadIdx.x;
+    const uint32_t from = mine < ns ? ld_plain(r.cu + mine) : 0u, to = mine < ns ? ld_plain(r.cu + mine + 1) : 0u;
     if (row < r.total) {
         // (a decode step has a row a sequence: look there first)
-        uint32_t s = ns;
-        if (row < ns && ld_plain(r.cu + row) <= row && row < ld_plain(r.cu + row + 1)) s = row;
-        else s = seq_of_row(r.cu, ns, row, lane);
-        if (s < ns) {                            // (else: a row past the last sequence)
-            const uint32_t t = row - ld_plain(r.cu + s);
+        uint32_t s = row, lo = row < ns ? ld_plain(r.cu + row) : ~0u, hi = row < ns ? ld_plain(r.cu + row + 1) : 0u;
+        if (lo > row || row >= hi) {
+            s = seq_of_row(r.cu, ns, row, lane);
+            if (s >= ns) s = kv4_seq_by_scan(r.cu, ns, row, lane);
+            lo = s < ns ? ld_plain(r.cu + s) : 0u;
+            hi = s < ns ? ld_plain(r.cu + s + 1) : 0u;
+        }
+        if (s < ns && hi <= r.total) {           // (no sequence: a row past the last one's)
+            const uint32_t t = row - lo;
             const uint64_t e = uint64_t(base ? ld_plain(base + s) : 0u) + t;
             if (a.c.pos) p.pos = ld_plain((a.c.seen ? a.c.seen : a.c.len) + s) + t;
             p.page = kv4_page(a.c, s, e, a.err);
@@ -106,6 +123,11 @@ SMOE_DEVINL void kv4_places(const Kv4Args& a, const SmoeKv4Rows& r, const uint32
         }
     }
     if (lane == 0) places[warp] = p;
+    bool bad = from > to || to > r.total;
+#pragma unroll 1
+    for (uint32_t s = mine + gridDim.x * kKwThreads; s < ns; s += gridDim.x * kKwThreads)
+        bad |= ld_plain(r.cu + s) > ld_plain(r.cu + s + 1) || ld_plain(r.cu + s + 1) > r.total;
+    if (bad) serve_err(a.err, SMOE_DEVERR_BAD_RANGE);
     __syncthreads();
 }
 
@@ -1368,12 +1390,18 @@ __global__ void __launch_bounds__(kEvThreads) k_kv4_evict(const Kv4Evict p) {
 }
 
 __global__ void __launch_bounds__(256) k_kv4_advance(uint32_t* len, uint32_t* seen, uint32_t n_seqs, const uint32_t* cu,
-                                                     uint32_t n_each, uint32_t keep) {
+                                                     uint32_t n_each, uint32_t keep, uint32_t* err) {
     pdl_release();
     pdl_acquire();
     const uint32_t s = blockIdx.x * 256 + threadIdx.x;
     if (s >= n_seqs) return;
-    const uint32_t n = cu ? cu[s + 1] - cu[s] : n_each, l = len[s] + n;
+    uint32_t n = n_each;
+    if (cu) {
+        const uint32_t from = cu[s], to = cu[s + 1];
+        if (from > to) serve_err(err, SMOE_DEVERR_BAD_RANGE);
+        n = from > to ? 0u : to - from;
+    }
+    const uint32_t l = len[s] + n;
     len[s] = keep && l > keep ? keep : l;
     if (seen) seen[s] += n;
 }

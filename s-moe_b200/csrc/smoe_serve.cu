@@ -347,8 +347,8 @@ int smoe_cuda_kv4_evict(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, uint32_t ke
 int smoe_cuda_kv4_advance(SmoeCudaCtx* ctx, uint32_t* len, uint32_t* seen, uint32_t n_seqs, const uint32_t* cu,
                           uint32_t n_each, uint32_t keep) {
     if (!ctx || !len || n_seqs == 0) return ctx_fail(SMOE_ERR_ARG, "bad kv4_advance arguments", n_seqs);
-    return launch(smoe::ctx_view(ctx), smoe::k_kv4_advance, dim3((n_seqs + 255) / 256), dim3(256), 0, len, seen, n_seqs, cu,
-                  n_each, keep);
+    const CtxView c = smoe::ctx_view(ctx);
+    return launch(c, smoe::k_kv4_advance, dim3((n_seqs - 1) / 256 + 1), dim3(256), 0, len, seen, n_seqs, cu, n_each, keep, c.err);
 }
 
 }  // extern "C"

@@ -78,3 +78,62 @@ def test_kv4_attention_small_scales(ctx, dtype, scale):
         page, slot = c.at(b, n)
         w = p.sum(1).t()
         assert ((so[page, :, slot].double() - w).abs() <= 2e-5 * (w + p.sum(1).max())).all()
+
+
+# ------------------------------------------------------------------- row ranges
+RANGES = [
+    # starts, rows, sequences that must be skipped
+    ([0, 5, 9, 9], 7, [1]),              # the second one ends past the rows
+    ([0, 7, 12, 12], 7, [1]),            # .. and starts there
+    ([0, 4, 4, 200], 9, [2]),
+    ([0, 3, 6, 2 ** 31 + 5], 9, [2]),
+    ([0, 6, 2, 2], 8, [1]),              # one that ends before it starts
+]
+
+
+@pytest.mark.parametrize("case", range(len(RANGES)))
+@pytest.mark.parametrize("what", ["append", "read"])
+def test_kv4_rows_outside_their_buffer(ctx, case, what):
+    """A sequence whose rows are not all there is skipped as a whole and reported; the others are served."""
+    cu, total, bad = RANGES[case]
+    c = T.Cache(2, 64, [70, 10, 64], 300, 520)
+    c.fill(ctx)
+    before = c.blocks.clone()
+    k, v = (torch.randn(total, 2, 64, generator=c.g, device="cuda") for _ in range(2))
+    cu_t = torch.tensor([x - (x >> 31 << 32) for x in cu], dtype=torch.int32, device="cuda")
+    ko, vo = torch.full_like(k, -9), torch.full_like(v, -9)
+    if what == "append":
+        ctx.kv4_append(c.desc(), S.kv4_rows(k, v, cu_t))
+    else:
+        ctx.kv4_read(c.desc(), None, S.kv4_rows(ko, vo, cu_t))
+    with pytest.raises(S.SmoeCudaError, match="ERR_DEVICE"):
+        ctx.synchronize()
+    ctx.synchronize()                    # reported once
+    lens = [70, 10, 64]
+    for s in range(3):
+        n = cu[s + 1] - cu[s]
+        if s in bad or n == 0 or any(cu[b + 1] < cu[b] for b in bad) and s > 0:
+            continue
+        if what == "append":
+            page, slot = c.at(s, n, lens[s])
+            assert (c.pos[page, :, slot] == torch.arange(lens[s], lens[s] + n, device="cuda")[:, None]).all()
+            got = T.Cache.values(c, s, lens[s] + n)[0][lens[s]:]
+            code, scale, bias = quantised(k[cu[s]: cu[s + 1]])
+            assert ((got - (code * scale + bias).flatten(-2).double()).abs() <= 1e-5).all()
+        else:
+            want = c.values(s, n)[0]
+            assert ((ko[cu[s]: cu[s + 1]].double() - want).abs() <= 1e-5).all()
+    for s in bad:
+        if what == "append":             # nothing was written for it
+            page, slot = c.at(s, 64, lens[s])
+            assert torch.equal(c.blocks[page], before[page]) and (c.pos[page, :, slot] == 0).all()
+        elif cu[s] < min(cu[s + 1], total):
+            assert (ko[cu[s]: cu[s + 1]] == -9).all() and (vo[cu[s]: cu[s + 1]] == -9).all()
+
+
+def test_kv4_advance_reports_a_range_that_runs_backwards(ctx):
+    lens, seen = ints([10, 20, 30]), ints([11, 21, 31])
+    ctx.kv4_advance(lens, seen, 3, cu=ints([0, 4, 1, 8]))
+    with pytest.raises(S.SmoeCudaError, match="ERR_DEVICE"):
+        ctx.synchronize()
+    assert lens.tolist() == [14, 20, 37] and seen.tolist() == [15, 21, 38]
