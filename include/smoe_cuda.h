@@ -498,10 +498,12 @@ int smoe_cuda_decode_advance_batch(SmoeCudaCtx* ctx, SmoeSamplerRow* rows, uint3
  * bf16 operands and result, fp32 scores, statistics and accumulators; the
  * probabilities are rounded to bf16 for the tensor cores.
  * Strides in elements: row r of head h of q starts at q + r * q_row + h *
- * q_head; strides are multiples of 8 and bases 16-byte aligned; head_dim
- * contiguous, a multiple of 8, <= 128; <= 128 query heads per KV head; scale
- * finite and not negative. The
- * rows of a call with equal arguments give equal bits. */
+ * q_head; strides are multiples of 8 and bases 16-byte aligned. k_head and
+ * v_head may be 0 (KV heads that share their rows); no other stride may be
+ * where its dimension has more than one element, and rows and heads of out do
+ * not overlap (SMOE_ERR_ARG). head_dim contiguous, a multiple of 8, <= 128;
+ * <= 128 query heads per KV head; scale finite and not negative. The rows of
+ * a call with equal arguments give equal bits. */
 typedef struct SmoeCudaPackedAttnArgs {
     const uint16_t* q;            /* bf16 [total_q][num_heads][head_dim]     */
     const uint16_t* k;            /* bf16 [total_k][num_kv_heads][head_dim]  */

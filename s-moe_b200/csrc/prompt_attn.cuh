@@ -49,6 +49,7 @@ struct PaPlace {
 struct PackedArgs {
     SmoeCudaPackedAttnArgs a;
     uint32_t group, tokens;                      // query heads per KV head, tokens per tile (128 / group)
+    uint32_t k_step, v_step;                     // 1, or 0 where all KV heads have the same keys / values
     float scale_log2;                            // scale * log2(e), positive
     uint32_t* err;
     const PaPlace* plan;                         // [CTAs + 1] where each CTA's share starts, or null
@@ -463,7 +464,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                 const PaItem& it = item(k);
                 if (!it.more) break;
                 const uint32_t m = max(it.cnt[0], it.cnt[1]), kvh = it.kvh, row_q = it.S.q0 + it.tok, row_k = it.S.k0 + it.key0;
-                const uint32_t cnt[2] = {it.cnt[0], it.cnt[1]};
+                const uint32_t cnt[2] = {it.cnt[0], it.cnt[1]}, head_k = kvh * p.k_step, head_v = kvh * p.v_step;
                 item_done(k);
 #pragma unroll 1
                 for (uint32_t i = 0; i < 2 * m; ++i, ++j) {      // K0 V0 K1 V1 .., the Q tiles around K0
@@ -478,7 +479,7 @@ k_attention_packed(const __grid_constant__ CUtensorMap mq, const __grid_constant
                     if (round) wait(kve + st, round - 1);
                     (kvf + st).expect(SM::BLOCK);
                     for (int h = 0; h < NH; ++h)
-                        tma_load3(base + SM::KV + st * SM::BLOCK + h * 8192, i & 1 ? &mv : &mk, h * 64, kvh, row_k + i / 2 * kPaKeys, kvf + st);
+                        tma_load3(base + SM::KV + st * SM::BLOCK + h * 8192, i & 1 ? &mv : &mk, h * 64, i & 1 ? head_v : head_k, row_k + i / 2 * kPaKeys, kvf + st);
                 }
             }
             // nothing may be in flight when the CTA ends (the MMA lanes have

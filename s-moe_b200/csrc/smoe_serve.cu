@@ -58,6 +58,15 @@ int smem_limit(const CtxView& c, K kern, size_t smem) {
     return SMOE_OK;
 }
 
+// No two rows or heads of an output share an element: either all heads of a
+// row lie before the next row starts, or all rows of a head before the next head.
+bool apart(uint64_t row, uint64_t head, uint64_t rows, uint64_t heads, uint64_t head_dim) {
+    const auto span = [](uint64_t stride, uint64_t n, uint64_t inner) { return static_cast<unsigned __int128>(stride) * (n - 1) + inner; };
+    const bool heads_inside = (heads <= 1 || head >= head_dim) && (rows <= 1 || row >= span(head, heads, head_dim));
+    const bool rows_inside = (rows <= 1 || row >= head_dim) && (heads <= 1 || head >= span(row, rows, head_dim));
+    return heads_inside || rows_inside;
+}
+
 // bf16 rows whose groups all start on 16 bytes.
 bool wide_rows(const SmoeKv4Rows* r) { return (r->k_row | r->k_head | r->v_row | r->v_head) % 8 == 0; }
 
@@ -74,14 +83,15 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// bf16 [rows][heads][head_dim] with the given strides (elements), read in
-// boxes of 64 columns x box_heads x box_rows, 128-byte swizzle, zeros outside.
+// bf16 [rows][heads][head_dim] with the given strides (elements; of a dimension
+// of one element any, of another not 0), read in boxes of 64 columns x
+// box_heads x box_rows, 128-byte swizzle, zeros outside.
 int map_rows(CUtensorMap* m, const void* base, uint32_t head_dim, uint32_t heads, uint32_t rows, uint64_t row, uint64_t head,
              uint32_t box_heads, uint32_t box_rows) {
     const EncodeTiled enc = encode_tiled();
     if (!enc) return ctx_fail(SMOE_ERR_CUDA, "cuTensorMapEncodeTiled is missing", 0);
     const cuuint64_t dims[3] = {head_dim, heads, rows};
-    const cuuint64_t strides[2] = {std::max<uint64_t>(head, 8) * 2, std::max<uint64_t>(row, 8) * 2};
+    const cuuint64_t strides[2] = {heads > 1 ? head * 2 : 16, rows > 1 ? row * 2 : 16};
     const cuuint32_t box[3] = {64, box_heads, box_rows}, one[3] = {1, 1, 1};
     const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, one,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -163,9 +173,19 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
         return ctx_fail(SMOE_ERR_UNSUPPORTED, "packed attention takes head_dim <= 128, a multiple of 8", a->head_dim);
     if (a->num_heads / a->num_kv_heads > 128)
         return ctx_fail(SMOE_ERR_UNSUPPORTED, "at most 128 query heads per KV head", a->num_heads / a->num_kv_heads);
-    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) ||
-        (a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head | a->out_row | a->out_head) % 8)
+    // (a dimension of one element has no stride)
+    const uint64_t rows[] = {a->q_row, a->out_row, a->k_row, a->v_row}, heads[] = {a->q_head, a->out_head, a->k_head, a->v_head};
+    uint64_t all_strides = 0;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t n = i < 2 ? a->total_q : a->total_k, h = i < 2 ? a->num_heads : a->num_kv_heads;
+        all_strides |= (n > 1 ? rows[i] : 0) | (h > 1 ? heads[i] : 0);
+        if ((n > 1 && rows[i] == 0) || (h > 1 && heads[i] == 0 && i < 2))
+            return ctx_fail(SMOE_ERR_ARG, "packed attention: a stride of 0 is taken for the heads of k and v only", i);
+    }
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || all_strides % 8)
         return ctx_fail(SMOE_ERR_ARG, "packed attention needs 16-byte aligned bases and strides that are multiples of 8", 0);
+    if (!apart(a->out_row, a->out_head, a->total_q, a->num_heads, a->head_dim))
+        return ctx_fail(SMOE_ERR_ARG, "packed attention: rows or heads of out overlap", long(a->out_row));
     if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return ctx_fail(SMOE_ERR_ARG, "packed attention needs a finite scale >= 0", 0);
     const CtxView c = smoe::ctx_view(ctx);
     smoe::PackedArgs p{};
@@ -178,9 +198,12 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
     CUtensorMap mq, mk, mv;
     int rc = map_rows(&mq, a->q, a->head_dim, a->num_heads, a->total_q, a->q_row, a->q_head, p.group, p.tokens);
     if (rc) return rc;
+    // (KV heads that share their rows are one head of the map)
+    p.k_step = a->k_head != 0;
+    p.v_step = a->v_head != 0;
     if (a->total_k) {
-        if ((rc = map_rows(&mk, a->k, a->head_dim, a->num_kv_heads, a->total_k, a->k_row, a->k_head, 1, smoe::kPaKeys)) ||
-            (rc = map_rows(&mv, a->v, a->head_dim, a->num_kv_heads, a->total_k, a->v_row, a->v_head, 1, smoe::kPaKeys)))
+        if ((rc = map_rows(&mk, a->k, a->head_dim, p.k_step ? a->num_kv_heads : 1, a->total_k, a->k_row, a->k_head, 1, smoe::kPaKeys)) ||
+            (rc = map_rows(&mv, a->v, a->head_dim, p.v_step ? a->num_kv_heads : 1, a->total_k, a->v_row, a->v_head, 1, smoe::kPaKeys)))
             return rc;
     } else {
         mk = mv = mq;                            // no row has a key: never read

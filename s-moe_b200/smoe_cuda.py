@@ -514,8 +514,9 @@ def _ints(t, name, n=None):
 
 def packed_attn_args(q, k, v, out, cu_q, cu_k=None, scale=None, causal=True, window=0, lse=None) -> PackedAttnArgs:
     """Arguments of Context.attention_packed from torch tensors: q, out
-    [total_q, heads, head_dim], k, v [total_k, kv_heads, head_dim] (bf16, any
-    row and head strides), cu_q / cu_k [n_seqs + 1] int32, lse [total_q,
+    [total_q, heads, head_dim], k, v [total_k, kv_heads, head_dim] (bf16, row
+    and head strides that are multiples of 8; k and v may be expanded over
+    their heads, nothing else may be expanded), cu_q / cu_k [n_seqs + 1] int32, lse [total_q,
     heads] fp32. scale: 1 / sqrt(head_dim) by default. The tensors must stay
     alive while the structure is used."""
     import torch

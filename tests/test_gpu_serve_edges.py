@@ -13,6 +13,61 @@ from test_gpu_serve import BF16, F32, attn_run, ints, quantised, starts
 pytestmark = pytest.mark.gpu
 
 
+# ---------------------------------------------------------------------- strides
+@pytest.mark.parametrize("lens,H,Hkv,hd", [([(45, 45), (3, 200)], 32, 4, 128),                # a CTA per pair
+                                           ([(150, 900), (40, 1300), (77, 777)], 16, 2, 64),   # equal shares
+                                           ([(940, 1300), (1500, 1500), (333, 333)], 32, 8, 128)])     # the list
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+def test_packed_attention_shared_kv_heads(ctx, lens, H, Hkv, hd, which):
+    """K and V expanded over their heads (stride 0) give the bits of copies."""
+    q, k, v = T.packed_inputs(lens, H, Hkv, hd, 600)
+    a, b = (x[:, :1].contiguous().expand(-1, Hkv, -1) if n in which else x for n, x in (("k", k), ("v", v)))
+    assert (a.stride(1) == 0) == ("k" in which)
+    out, lse = T.packed_run(ctx, q, a, b, lens)
+    want, want_lse = T.packed_run(ctx, q, a.contiguous(), b.contiguous(), lens)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    T.packed_check(out, lse, T.packed_ref(q, a, b, lens, True, 0, 1 / math.sqrt(hd)))
+
+
+def test_packed_attention_stride_refusals(ctx):
+    """Strides of 0 and outputs that overlap are refused; a dimension of one element may have any stride."""
+    lens = [(20, 20)]
+    q, k, v = T.packed_inputs(lens, 8, 2, 64, 601)
+    out = torch.zeros_like(q)
+
+    def refused(q=q, k=k, v=v, out=out, **kw):
+        a = S.packed_attn_args(q, k, v, out, starts([20]))
+        for n, x in kw.items():
+            setattr(a, n, x)
+        with pytest.raises(S.SmoeCudaError, match="ERR_ARG"):
+            ctx.attention_packed(a)
+    refused(q=q[:, :1].expand(-1, 8, -1))
+    refused(q=q[:1].expand(20, -1, -1))
+    refused(k=k[:1].expand(20, -1, -1))
+    refused(v=v[:1].expand(20, -1, -1))
+    refused(out=out[:, :1].expand(-1, 8, -1))
+    refused(out=out[:1].expand(20, -1, -1))
+    refused(out_row=64 * 7)              # rows that end in the next one
+    refused(out_head=56)
+    refused(out_row=8 * 64 * 10, out_head=8 * 64 * 10)
+    ctx.synchronize()
+    assert (out == 0).all()
+    # one row, one query head per call: their strides are nobody's
+    want, want_lse = T.packed_run(ctx, q[:1], k[:1], v[:1], [(1, 1)])
+    a = S.packed_attn_args(q[:1], k[:1], v[:1], out[:1], starts([1]))
+    a.q_row, a.k_row, a.v_row, a.out_row = 0, 3, 5, 0
+    ctx.attention_packed(a)
+    q1, k1, v1 = q[:, :1].contiguous(), k[:, :1].contiguous(), v[:, :1].contiguous()
+    one = torch.zeros_like(q1)
+    b = S.packed_attn_args(q1, k1, v1, one, starts([20]))
+    b.q_head, b.k_head, b.v_head, b.out_head = 1, 0, 7, 0
+    ctx.attention_packed(b)
+    ctx.synchronize()
+    assert torch.equal(out[:1], want)
+    want, _ = T.packed_run(ctx, q1, k1, v1, lens)
+    assert torch.equal(one, want)
+
+
 # ------------------------------------------------------------- NaN in cache rows
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("other", [0.0, math.inf, -math.inf])
