@@ -78,6 +78,7 @@ class AttnLayerArgs(C.Structure):
 
 class PackedAttnArgs(C.Structure):
     """SmoeCudaPackedAttnArgs (packed_attn_args makes one from torch tensors)."""
+    made_of = None                         # what the builder knows of the tensors; the calls compare it
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "cu_q", "cu_k")] + \
               [(n, C.c_uint64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
                                          "out_head")] + \
@@ -87,12 +88,14 @@ class PackedAttnArgs(C.Structure):
 
 class Kv4Cache(C.Structure):
     """SmoeKv4Cache (kv4_cache makes one from torch tensors)."""
+    made_of = None                         # what the builder knows of the tensors; the calls compare it
     _fields_ = [(n, C.c_void_p) for n in ("blocks", "table", "len", "seen", "pos", "score")] + \
               [(n, C.c_uint32) for n in ("n_pages", "n_seqs", "table_stride", "num_kv_heads", "head_dim")]
 
 
 class Kv4Rows(C.Structure):
     """SmoeKv4Rows (kv4_rows makes one from torch tensors)."""
+    made_of = None                         # what the builder knows of the tensors; the calls compare it
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "cu")] + \
               [(n, C.c_uint64) for n in ("k_row", "k_head", "v_row", "v_head")] + \
               [("total", C.c_uint32), ("dtype", C.c_int)]
@@ -100,6 +103,7 @@ class Kv4Rows(C.Structure):
 
 class Kv4AttnArgs(C.Structure):
     """SmoeKv4AttnArgs (kv4_attn_args makes one from torch tensors)."""
+    made_of = None                         # what the builder knows of the tensors; the calls compare it
     _fields_ = [(n, C.c_void_p) for n in ("q", "out", "score_out", "workspace")] + \
               [(n, C.c_uint64) for n in ("workspace_bytes", "q_row", "out_row")] + \
               [(n, C.c_uint32) for n in ("num_heads", "extra", "max_len")] + \
@@ -460,24 +464,35 @@ class Context:
 
     # ---- long-context serving
     def attention_packed(self, args: PackedAttnArgs):
+        _on_gpu(args)
         check(self.L.smoe_cuda_attention_packed(self.h, C.byref(args)), "attention_packed")
 
     def kv4_append(self, cache: Kv4Cache, rows: Kv4Rows):
+        _rows_fit(cache, rows)
         check(self.L.smoe_cuda_kv4_append(self.h, C.byref(cache), C.byref(rows)), "kv4_append")
 
     def kv4_read(self, cache: Kv4Cache, first, rows: Kv4Rows):
-        check(self.L.smoe_cuda_kv4_read(self.h, C.byref(cache), ptr(first), C.byref(rows)), "kv4_read")
+        _rows_fit(cache, rows)
+        check(self.L.smoe_cuda_kv4_read(self.h, C.byref(cache), _gpu_ints(first, "first", cache.n_seqs), C.byref(rows)),
+              "kv4_read")
 
     def kv4_attention(self, cache: Kv4Cache, args: Kv4AttnArgs):
+        _attn_fits(cache, args)
         check(self.L.smoe_cuda_kv4_attention(self.h, C.byref(cache), C.byref(args)), "kv4_attention")
 
     def kv4_evict(self, cache: Kv4Cache, keep, recent, max_len, workspace, pos_out=None, score_out=None):
-        """workspace: a torch tensor of at least kv4_evict_workspace(cache, max_len) bytes."""
-        check(self.L.smoe_cuda_kv4_evict(self.h, C.byref(cache), keep, recent, max_len, ptr(pos_out), ptr(score_out),
-                                         ptr(workspace), _nbytes(workspace)), "kv4_evict")
+        """workspace: a torch tensor of at least kv4_evict_workspace(cache, max_len) bytes; pos_out, score_out: like the
+        cache's pos and score."""
+        _on_gpu(cache)
+        n = cache.n_pages * cache.num_kv_heads * KV4_PAGE
+        pos_p, score_p = _gpu_ints(pos_out, "pos_out", n), _gpu_floats(score_out, "score_out", n)
+        check(self.L.smoe_cuda_kv4_evict(self.h, C.byref(cache), _u32(keep, "keep"), _u32(recent, "recent"),
+                                         _u32(max_len, "max_len"), pos_p, score_p, *_workspace(workspace)), "kv4_evict")
 
     def kv4_advance(self, lens, seen, n_seqs, cu=None, n_each=1, keep=0):
-        check(self.L.smoe_cuda_kv4_advance(self.h, ptr(lens), ptr(seen), n_seqs, ptr(cu), n_each, keep),
+        n = _u32(n_seqs, "n_seqs")
+        check(self.L.smoe_cuda_kv4_advance(self.h, _gpu_ints(lens, "lens", n), _gpu_ints(seen, "seen", n), n,
+                                           _gpu_ints(cu, "cu", n + 1), _u32(n_each, "n_each"), _u32(keep, "keep")),
               "kv4_advance")
 
     def sample(self, logits, vocab, batch, rows, history, history_stride, tokens):
@@ -485,8 +500,60 @@ class Context:
                                       history_stride, ptr(tokens)), "sample")
 
 
-def _nbytes(t) -> int:
-    return 0 if t is None else t.numel() * t.element_size()
+def _u32(x, name) -> int:
+    if not 0 <= x < 1 << 32:
+        raise ValueError(f"{name}: {x} is not in the range of 32 bits")
+    return int(x)
+
+
+def _need_gpu(t, name):
+    if not t.is_cuda:
+        raise ValueError(f"{name}: a tensor on the GPU is taken")
+
+
+def _on_gpu(args):
+    """Refuses a structure that its builder made of a tensor in host memory."""
+    if args.made_of is not None and args.made_of["host"]:
+        raise ValueError(f"{args.made_of['host']}: a tensor on the GPU is taken")
+
+
+def _host(**tensors):
+    """The name of one of the tensors that is not on the GPU, or None."""
+    return next((n for n, t in tensors.items() if t is not None and not t.is_cuda), None)
+
+
+def _rows_fit(cache, rows):
+    """Rows against the cache they go to or come from (structures that were filled in by hand are taken as they are)."""
+    c, r = cache.made_of, rows.made_of
+    if c is not None and r is not None:
+        if (r["heads"], r["head_dim"]) != (c["kv_heads"], c["head_dim"]):
+            raise ValueError(f"k and v: {c['kv_heads']} KV heads of {c['head_dim']} are taken by this cache, not "
+                             f"{r['heads']} of {r['head_dim']}")
+        if r["starts"] < c["n_seqs"] + 1:
+            raise ValueError(f"cu: {c['n_seqs'] + 1} values are taken by this cache")
+    _on_gpu(cache)
+    _on_gpu(rows)
+
+
+def _attn_fits(cache, args):
+    c, a = cache.made_of, args.made_of
+    if c is not None and a is not None:
+        if (a["n_seqs"], a["head_dim"]) != (c["n_seqs"], c["head_dim"]):
+            raise ValueError(f"q and out: [{c['n_seqs']}, heads, {c['head_dim']}] is taken by this cache")
+        if a["scores"] is not None and a["scores"] < c["entries"]:
+            raise ValueError(f"score_out: {c['entries']} values are taken by this cache")
+    _on_gpu(cache)
+    _on_gpu(args)
+
+
+def _workspace(t):
+    """Pointer and bytes of a workspace tensor."""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor is taken")
+    _need_gpu(t, "workspace")
+    return ptr(t), t.numel() * t.element_size()
 
 
 def _dtype_of(t) -> int:
@@ -512,6 +579,30 @@ def _ints(t, name, n=None):
     return ptr(t)
 
 
+def _floats(t, name, n):
+    import torch
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{name}: a contiguous float32 tensor of {n} values is taken")
+    return ptr(t)
+
+
+def _gpu_ints(t, name, n):
+    """The address of n 32-bit integers: of a tensor on the GPU, or an address as it is (None: none)."""
+    if t is None or isinstance(t, int):
+        return t
+    p = _ints(t, name, n)
+    _need_gpu(t, name)
+    return p
+
+
+def _gpu_floats(t, name, n):
+    if t is None or isinstance(t, int):
+        return t
+    p = _floats(t, name, n)
+    _need_gpu(t, name)
+    return p
+
+
 def packed_attn_args(q, k, v, out, cu_q, cu_k=None, scale=None, causal=True, window=0, lse=None) -> PackedAttnArgs:
     """Arguments of Context.attention_packed from torch tensors: q, out
     [total_q, heads, head_dim], k, v [total_k, kv_heads, head_dim] (bf16, row
@@ -534,13 +625,14 @@ def packed_attn_args(q, k, v, out, cu_q, cu_k=None, scale=None, causal=True, win
         if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2]:
             raise ValueError("lse: a contiguous float32 [total_q, heads] tensor is taken")
         a.lse = ptr(lse)
+    a.cu_q = _ints(cu_q, "cu_q", 1)
     a.n_seqs = cu_q.numel() - 1
-    a.cu_q = _ints(cu_q, "cu_q")
     a.cu_k = None if cu_k is None else _ints(cu_k, "cu_k", a.n_seqs + 1)
     a.total_q, a.total_k = q.shape[0], k.shape[0]
     a.num_heads, a.num_kv_heads, a.head_dim = q.shape[1], k.shape[1], q.shape[2]
-    a.causal, a.window = int(causal), window
+    a.causal, a.window = int(bool(causal)), _u32(window, "window")
     a.scale = 1.0 / q.shape[2] ** 0.5 if scale is None else scale
+    a.made_of = {"host": _host(q=q, k=k, v=v, out=out, cu_q=cu_q, cu_k=cu_k, lse=lse)}
     return a
 
 
@@ -563,10 +655,9 @@ def kv4_cache(blocks, table, lens, head_dim, seen=None, pos=None, score=None) ->
     c.seen = None if seen is None else _ints(seen, "seen", c.n_seqs)
     n = c.n_pages * c.num_kv_heads * KV4_PAGE
     c.pos = None if pos is None else _ints(pos, "pos", n)
-    if score is not None:
-        if score.dtype != torch.float32 or not score.is_contiguous() or score.numel() < n:
-            raise ValueError("score: a contiguous float32 [n_pages, kv_heads, 64] tensor is taken")
-        c.score = ptr(score)
+    c.score = None if score is None else _floats(score, "score", n)
+    c.made_of = {"n_seqs": c.n_seqs, "kv_heads": c.num_kv_heads, "head_dim": head_dim, "entries": n,
+                 "host": _host(blocks=blocks, table=table, lens=lens, seen=seen, pos=pos, score=score)}
     return c
 
 
@@ -584,9 +675,10 @@ def kv4_rows(k, v, cu) -> Kv4Rows:
     if k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v have the same shape and type")
     r = Kv4Rows()
-    r.k, r.v, r.cu = ptr(k), ptr(v), _ints(cu, "cu")
+    r.k, r.v, r.cu = ptr(k), ptr(v), _ints(cu, "cu", 1)
     (r.k_row, r.k_head), (r.v_row, r.v_head) = _rows3(k, "k"), _rows3(v, "v")
     r.total, r.dtype = k.shape[0], _dtype_of(k)
+    r.made_of = {"heads": k.shape[1], "head_dim": k.shape[2], "starts": cu.numel(), "host": _host(k=k, v=v, cu=cu)}
     return r
 
 
@@ -595,15 +687,18 @@ def kv4_attn_args(q, out, max_len, extra=0, scale=None, score_out=None, decay=1.
     (float32 or bfloat16, heads contiguous); score_out: paged like the
     cache's score array, which it may be."""
     for name, t in (("q", q), ("out", out)):
-        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+        if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
             raise ValueError(f"{name}: [n_seqs, heads, head_dim] with contiguous heads is taken")
     if q.shape != out.shape or q.dtype != out.dtype:
         raise ValueError("q and out have the same shape and type")
     a = Kv4AttnArgs()
     a.q, a.out, a.q_row, a.out_row = ptr(q), ptr(out), q.stride(0), out.stride(0)
-    a.num_heads, a.extra, a.max_len, a.dtype = q.shape[1], extra, max_len, _dtype_of(q)
+    a.num_heads, a.extra, a.max_len, a.dtype = q.shape[1], _u32(extra, "extra"), _u32(max_len, "max_len"), _dtype_of(q)
     a.scale = 1.0 / q.shape[2] ** 0.5 if scale is None else scale
-    a.decay, a.score_out = decay, ptr(score_out)
+    scores = None if score_out is None or isinstance(score_out, int) else score_out
+    a.decay, a.score_out = decay, score_out if scores is None else _floats(scores, "score_out", 0)
+    a.made_of = {"n_seqs": q.shape[0], "head_dim": q.shape[2], "scores": None if scores is None else scores.numel(),
+                 "host": _host(q=q, out=out, score_out=scores)}
     return a
 
 
@@ -612,12 +707,12 @@ def kv4_attention_workspace(cache: Kv4Cache, args: Kv4AttnArgs) -> int:
 
 
 def kv4_attn_set_workspace(args: Kv4AttnArgs, workspace) -> Kv4AttnArgs:
-    args.workspace, args.workspace_bytes = ptr(workspace) if workspace is not None else None, _nbytes(workspace)
+    args.workspace, args.workspace_bytes = _workspace(workspace)
     return args
 
 
 def kv4_evict_workspace(cache: Kv4Cache, max_len: int) -> int:
-    return int(lib().smoe_cuda_kv4_evict_workspace(C.byref(cache), max_len))
+    return int(lib().smoe_cuda_kv4_evict_workspace(C.byref(cache), _u32(max_len, "max_len")))
 
 
 def _vault_bytes(vault):
