@@ -550,7 +550,8 @@ uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim);
  * a sequence whose range is not within `total` rows is skipped as a whole, and
  * rows past the last sequence's are left alone. Row r of KV
  * head h of k starts at element r * k_row + h * k_head; strides multiples of
- * 4, bases 16-byte aligned, head_dim contiguous. */
+ * 4, bases 16-byte aligned, head_dim contiguous. Rows that are read may
+ * overlap (strides of 0), rows that are written may not (SMOE_ERR_ARG). */
 typedef struct SmoeKv4Rows {
     void*           k;            /* dtype [total][num_kv_heads][head_dim]   */
     void*           v;
@@ -591,7 +592,7 @@ typedef struct SmoeKv4AttnArgs {
     float*       score_out;
     void*        workspace;
     uint64_t     workspace_bytes;
-    uint64_t     q_row, out_row;  /* elements between sequences, multiples of 4 */
+    uint64_t     q_row, out_row;  /* elements between sequences, multiples of 4; rows of out do not overlap */
     uint32_t     num_heads, extra, max_len;
     int          dtype;           /* SMOE_DTYPE_F32 or SMOE_DTYPE_BF16       */
     float        scale, decay;

@@ -113,8 +113,11 @@ int check_cache(const SmoeKv4Cache* c, const char* what) {
     return SMOE_OK;
 }
 
-int check_rows(const SmoeKv4Rows* r, const char* what) {
+int check_rows(const SmoeKv4Rows* r, const SmoeKv4Cache* c, bool written, const char* what) {
     if (!r || !r->k || !r->v || !r->cu) return ctx_fail(SMOE_ERR_ARG, what, 0);
+    if (written && (!apart(r->k_row, r->k_head, r->total, c->num_kv_heads, c->head_dim) ||
+                    !apart(r->v_row, r->v_head, r->total, c->num_kv_heads, c->head_dim)))
+        return ctx_fail(SMOE_ERR_ARG, "rows or heads of the rows to write overlap", long(r->k_row));
     if (r->dtype != SMOE_DTYPE_F32 && r->dtype != SMOE_DTYPE_BF16)
         return ctx_fail(SMOE_ERR_ARG, "rows are fp32 or bf16", r->dtype);
     if (!aligned(r->k, 16) || !aligned(r->v, 16) || (r->k_row | r->k_head | r->v_row | r->v_head) % 4)
@@ -249,7 +252,7 @@ uint64_t smoe_cuda_kv4_block_bytes(uint32_t head_dim) {
 int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const SmoeKv4Rows* rows) {
     if (!ctx) return ctx_fail(SMOE_ERR_ARG, "null context", 0);
     int rc = check_cache(cache, "kv4_append: bad cache");
-    if (rc || (rc = check_rows(rows, "kv4_append: bad rows"))) return rc;
+    if (rc || (rc = check_rows(rows, cache, false, "kv4_append: bad rows"))) return rc;
     if (rows->total == 0) return SMOE_OK;
     const CtxView c = smoe::ctx_view(ctx);
     using namespace smoe;
@@ -263,7 +266,7 @@ int smoe_cuda_kv4_append(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const Smoe
 int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32_t* first, const SmoeKv4Rows* rows) {
     if (!ctx) return ctx_fail(SMOE_ERR_ARG, "null context", 0);
     int rc = check_cache(cache, "kv4_read: bad cache");
-    if (rc || (rc = check_rows(rows, "kv4_read: bad rows"))) return rc;
+    if (rc || (rc = check_rows(rows, cache, true, "kv4_read: bad rows"))) return rc;
     if (rows->total == 0) return SMOE_OK;
     const CtxView c = smoe::ctx_view(ctx);
     using namespace smoe;
@@ -290,6 +293,8 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: q and out are fp32 or bf16", t->dtype);
     if (!aligned(t->q, 16) || !aligned(t->out, 16) || (t->q_row | t->out_row) % 4)
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention needs 16-byte aligned q and out and strides that are multiples of 4", 0);
+    if (cache->n_seqs > 1 && t->out_row < uint64_t(t->num_heads) * cache->head_dim)
+        return ctx_fail(SMOE_ERR_ARG, "kv4_attention: rows of out overlap", long(t->out_row));
     if (uint64_t(cache->n_seqs) * t->num_heads * ((uint64_t(t->max_len) + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE) >= (uint64_t(1) << 31))
         return ctx_fail(SMOE_ERR_UNSUPPORTED, "kv4_attention: more than 2^31 pages to read", long(t->max_len));
     const uint64_t need = smoe_cuda_kv4_attention_workspace(cache, t);

@@ -68,6 +68,79 @@ def test_packed_attention_stride_refusals(ctx):
     assert torch.equal(one, want)
 
 
+def test_kv4_outputs_that_overlap_are_refused(ctx):
+    c = T.Cache(2, 64, [20, 30], 1, 610)
+    k, v = c.fill(ctx)
+    x = torch.zeros(50, 2, 64, device="cuda")
+    cu = starts([20, 30])
+
+    def refused(k, v, **kw):
+        r = S.kv4_rows(k, v, cu)
+        for n, y in kw.items():
+            setattr(r, n, y)
+        with pytest.raises(S.SmoeCudaError, match="ERR_ARG"):
+            ctx.kv4_read(c.desc(), None, r)
+    refused(x[:, :1].expand(-1, 2, -1), x)
+    refused(x, x[:1].expand(50, -1, -1))
+    refused(x, x.clone(), k_row=64)
+    refused(x, x.clone(), v_head=60)
+    q = torch.randn(2, 4, 64, device="cuda")
+    out = torch.zeros_like(q)
+    args = S.kv4_attn_args(q, out, 40)
+    ws = torch.zeros(S.kv4_attention_workspace(c.desc(), args), dtype=torch.uint8, device="cuda")
+    S.kv4_attn_set_workspace(args, ws)
+    for row in (0, 64, 4 * 64 - 4):
+        args.out_row = row
+        with pytest.raises(S.SmoeCudaError, match="ERR_ARG"):
+            ctx.kv4_attention(c.desc(), args)
+    ctx.synchronize()
+    assert (x == 0).all() and (out == 0).all()
+    # rows that are read may be expanded, and the outputs' heads lie outside their rows
+    ctx.kv4_append(c.desc(), S.kv4_rows(k[:1, :1].expand(3, 2, -1), v[:1].expand(3, -1, -1), starts([0, 3])))
+    ko, vo = (torch.zeros(2, 3, 64, dtype=BF16, device="cuda").transpose(0, 1) for _ in range(2))
+    ctx.kv4_read(c.desc(), ints([0, 30]), S.kv4_rows(ko, vo, starts([0, 3])))
+    ctx.synchronize()
+    for got, x in ((ko, k[:1, :1].expand(3, 2, -1)), (vo, v[:1].expand(3, -1, -1))):
+        code, scale, bias = quantised(x)
+        assert torch.equal(got, (code * scale + bias).flatten(-2).to(BF16))
+
+
+def odd(n, heads, hd, dtype, g):
+    """Rows [n, heads, hd] whose strides are multiples of 4 elements and not of 8, heads outermost."""
+    x = torch.randn(heads, n, hd + 4, generator=g, device="cuda").to(dtype)
+    return x[:, :, :hd].transpose(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Hkv,hd", [(3, 128), (2, 64)])
+def test_kv4_strides_of_four(ctx, dtype, Hkv, hd):
+    """bf16 rows that start on 8 bytes and not on 16: append, read, and attention's q and out."""
+    lens = [130, 1, 70]
+    c = T.Cache(Hkv, hd, lens, 1, 611)
+    n = sum(lens)
+    k, v = odd(n, Hkv, hd, dtype, c.g), odd(n, Hkv, hd, dtype, c.g)
+    assert k.stride(0) % 8 == 4
+    ctx.kv4_append(c.desc(), S.kv4_rows(k, v, starts(lens)))
+    ctx.kv4_advance(c.len, c.seen, 3, cu=starts(lens))
+    ko, vo = odd(n, Hkv, hd, dtype, c.g), odd(n, Hkv, hd, dtype, c.g)
+    ctx.kv4_read(c.desc(), None, S.kv4_rows(ko, vo, starts(lens)))
+    ctx.synchronize()
+    for x, o in ((k, ko), (v, vo)):
+        code, scale, bias = quantised(x)
+        assert torch.equal(o, (code * scale + bias).flatten(-2).to(dtype))
+    H = 4 * Hkv
+    wide = torch.randn(3, H * hd + 12, generator=c.g, device="cuda").to(dtype)
+    q = wide[:, : H * hd].view(3, H, hd)
+    res = torch.full((3, H * hd + 4), -5.0, dtype=dtype, device="cuda")
+    out = res[:, : H * hd].view(3, H, hd)
+    args = S.kv4_attn_args(q, out, 130)
+    ws = torch.zeros(S.kv4_attention_workspace(c.desc(), args), dtype=torch.uint8, device="cuda")
+    ctx.kv4_attention(c.desc(), S.kv4_attn_set_workspace(args, ws))
+    ctx.synchronize()
+    T.attn_check(c, q, lens, out)
+    assert (res[:, H * hd:] == -5).all()
+
+
 # ------------------------------------------------------------- NaN in cache rows
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("other", [0.0, math.inf, -math.inf])
