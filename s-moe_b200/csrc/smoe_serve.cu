@@ -114,7 +114,7 @@ int check_cache(const SmoeKv4Cache* c, const char* what) {
 }
 
 int check_rows(const SmoeKv4Rows* r, const SmoeKv4Cache* c, bool written, const char* what) {
-    if (!r || !r->k || !r->v || !r->cu) return ctx_fail(SMOE_ERR_ARG, what, 0);
+    if (!r || !r->cu || (r->total && (!r->k || !r->v))) return ctx_fail(SMOE_ERR_ARG, what, 0);
     if (written && (!apart(r->k_row, r->k_head, r->total, c->num_kv_heads, c->head_dim) ||
                     !apart(r->v_row, r->v_head, r->total, c->num_kv_heads, c->head_dim)))
         return ctx_fail(SMOE_ERR_ARG, "rows or heads of the rows to write overlap", long(r->k_row));

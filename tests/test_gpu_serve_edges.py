@@ -141,6 +141,31 @@ def test_kv4_strides_of_four(ctx, dtype, Hkv, hd):
     assert (res[:, H * hd:] == -5).all()
 
 
+# -------------------------------------------------------------- nothing to do
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_kv4_no_rows(ctx, dtype):
+    """A step in which no sequence has a row: tensors without elements have no address, and nothing changes."""
+    c = T.Cache(2, 64, [20, 30], 1, 620)
+    c.fill(ctx)
+    before, pos = c.blocks.clone(), c.pos.clone()
+    none = torch.zeros(0, 2, 64, dtype=dtype, device="cuda")
+    cu = ints([0, 0, 0])
+    ctx.kv4_append(c.desc(), S.kv4_rows(none, none, cu))
+    ctx.kv4_read(c.desc(), None, S.kv4_rows(none, none.clone(), cu))
+    ctx.kv4_advance(c.len, c.seen, 2, cu=cu)
+    ctx.synchronize()
+    assert torch.equal(c.blocks, before) and torch.equal(c.pos, pos) and c.len.tolist() == [20, 30]
+
+
+def test_packed_attention_no_keys_at_all(ctx):
+    """Rows, but not one key in the call: zeros and -inf."""
+    q = torch.randn(40, 8, 64, device="cuda").to(BF16)
+    none = torch.zeros(0, 2, 64, dtype=BF16, device="cuda")
+    for causal in (True, False):
+        out, lse = T.packed_run(ctx, q, none, none.clone(), [(30, 0), (10, 0)], causal)
+        assert (out == 0).all() and (lse == -math.inf).all()
+
+
 # ------------------------------------------------------------- NaN in cache rows
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("other", [0.0, math.inf, -math.inf])
