@@ -581,9 +581,10 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
  * for the attended entries; others stay. fp32 statistics and accumulators;
  * the codes are exact tensor-core operands, probabilities and an fp32 q go
  * in as sums of two fp16 pieces, good to about 2^-20 of the largest term.
- * scale finite and not negative. max_len: an
- * upper limit of len[s] + extra, known to the host (it sizes the grid and
- * the workspace; longer sequences are cut there and raise SMOE_ERR_DEVICE).
+ * scale finite and not negative, at most 6144 query heads per KV head.
+ * max_len: an upper limit of len[s] + extra, known to the host (it sizes the
+ * grid and the workspace; longer sequences are cut there and raise
+ * SMOE_ERR_DEVICE).
  * workspace: smoe_cuda_kv4_attention_workspace bytes, 16-byte aligned, its
  * contents free between calls. */
 typedef struct SmoeKv4AttnArgs {

@@ -213,6 +213,7 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
     }
     // at most one partial tile pair a sequence; the kernels count them
     const uint64_t pairs = uint64_t(a->total_q) / (2 * p.tokens) + std::min(a->n_seqs, a->total_q), ctas = pairs * a->num_kv_heads;
+    if (ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_UNSUPPORTED, "packed attention: more than 2^31 tile pairs", long(ctas));
     const uint64_t most = pairs * (uint64_t(a->total_k) / smoe::kPaKeys + 3);
     // A CTA per pair when all of them fit the GPU at once and none is long: the plan and the joining of cut pairs cost
     // some 6 us. (Above 65,536 pairs, or 2^31 blocks, too.)
@@ -297,6 +298,8 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: rows of out overlap", long(t->out_row));
     if (uint64_t(cache->n_seqs) * t->num_heads * ((uint64_t(t->max_len) + SMOE_KV4_PAGE - 1) / SMOE_KV4_PAGE) >= (uint64_t(1) << 31))
         return ctx_fail(SMOE_ERR_UNSUPPORTED, "kv4_attention: more than 2^31 pages to read", long(t->max_len));
+    if (t->num_heads / cache->num_kv_heads > 6144)                // (the joining kernel takes 8 bytes of shared memory for each)
+        return ctx_fail(SMOE_ERR_UNSUPPORTED, "kv4_attention: at most 6144 query heads per KV head", t->num_heads);
     const uint64_t need = smoe_cuda_kv4_attention_workspace(cache, t);
     if (need && (!t->workspace || t->workspace_bytes < need || !aligned(t->workspace, 16)))
         return ctx_fail(SMOE_ERR_ARG, "kv4_attention: workspace missing, too small or unaligned; bytes needed", long(need));
@@ -334,6 +337,8 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     while (p.lanes < 64 && p.lanes * 4 < usual) p.lanes *= 2;
     const uint32_t per = 4 * kKjThreads / p.lanes, outs = (p.group * cache->head_dim + per - 1) / per;
     const uint32_t entries = p.logits ? (t->max_len + kKjEntries - 1) / kKjEntries : 0u;
+    // (past 5,000 heads more than a launch has without asking, with the kernel's own arrays)
+    if (p.group > 5000 && (rc = smem_limit(c, k_kv4_join, 6144 * 8))) return rc;
     return launch(c, k_kv4_join, dim3(outs + entries, cache->num_kv_heads, cache->n_seqs), dim3(kKjThreads),
                   size_t(plan.chunks) * kKaHeads * 8, p, outs);
 }

@@ -166,6 +166,35 @@ def test_packed_attention_no_keys_at_all(ctx):
         assert (out == 0).all() and (lse == -math.inf).all()
 
 
+# --------------------------------------------------------------------- limits
+def test_limits(ctx):
+    """Shapes past what a launch takes are refused before anything runs; 6,144 query heads on one KV head are served."""
+    c = T.Cache(1, 64, [70], 1, 630)
+    c.fill(ctx)
+    for heads in (6144, 6145):
+        q = torch.randn(1, heads, 64, generator=c.g, device="cuda")
+        out, so = torch.zeros_like(q), torch.zeros_like(c.score)
+        args = S.kv4_attn_args(q, out, 70, score_out=so, decay=0.0)
+        ws = torch.zeros(S.kv4_attention_workspace(c.desc(), args), dtype=torch.uint8, device="cuda")
+        S.kv4_attn_set_workspace(args, ws)
+        if heads == 6144:
+            ctx.kv4_attention(c.desc(), args)
+            ctx.synchronize()
+            T.attn_check(c, q, [70], out, so, decay=0.0)
+        else:
+            before = ctx.dispatches()
+            with pytest.raises(S.SmoeCudaError, match="ERR_UNSUPPORTED"):
+                ctx.kv4_attention(c.desc(), args)
+            assert ctx.dispatches() == before
+    q, k, v = T.packed_inputs([(20, 20)], 8, 2, 64, 631)
+    a = S.packed_attn_args(q, k, v, torch.zeros_like(q), starts([20]))
+    a.n_seqs = a.total_q = 0xffffffff
+    before = ctx.dispatches()
+    with pytest.raises(S.SmoeCudaError, match="ERR_UNSUPPORTED"):
+        ctx.attention_packed(a)
+    assert ctx.dispatches() == before
+
+
 # ------------------------------------------------------------- NaN in cache rows
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("other", [0.0, math.inf, -math.inf])
