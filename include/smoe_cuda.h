@@ -579,8 +579,10 @@ int smoe_cuda_kv4_read(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const uint32
  *   score_out[j] = decay * cache->score[j] + sum over the KV head's query
  *   heads of p[h][j]     (decay 0 or cache->score NULL: without the first)
  * for the attended entries; others stay. fp32 statistics and accumulators;
- * the codes are exact tensor-core operands, probabilities and an fp32 q go
- * in as sums of two fp16 pieces, good to about 2^-20 of the largest term.
+ * the codes are exact tensor-core operands, probabilities (times the scales)
+ * and an fp32 q go in as sums of two fp16 pieces: good to 2^-22 of each, or,
+ * of small ones, of the head's largest product of the 64 values, and to 2^-38
+ * of the head's largest |q|.
  * scale finite and not negative, at most 6144 query heads per KV head.
  * max_len: an upper limit of len[s] + extra, known to the host (it sizes the
  * grid and the workspace; longer sequences are cut there and raise

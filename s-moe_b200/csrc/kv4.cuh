@@ -359,9 +359,9 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // biases stay in fp32. (c' and not c: the two sums then do not cancel - fp32
 // results were four times as far from 64 bits with c.) q goes in as one (bf16 q) or two fp16 pieces, each
 // head scaled by a power of two so that its largest value is near 2^14; p s
-// as two fp16 pieces (22 bits), times a power of two per group that follows
-// the largest scale seen. (bf16 pieces need no such power, but three more
-// instructions for every 16 codes.)
+// as two fp16 pieces (22 bits), times a power of two per group and head that
+// follows the largest products. (bf16 pieces need no such power, but three
+// more instructions for every 16 codes.)
 // The entries are the M rows of both products and 8 of a KV head's query
 // heads the N columns. (16 at a time halve the unpacking of wide groups, but
 // need 255 registers: 8 warps an SM instead of 12, and 1.2 times the time.)
@@ -383,7 +383,9 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // bf16, weights): 65 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
 // rings run; the first pages come in after 7 us, warps end between 37 and 56).
 // 32 contexts of 512 to 8,192: 33 us with the join; one of 300: 10.8 us, of
-// which most is the two launches.
+// which most is the two launches. (A power of two per group alone, by the
+// largest scale whatever its weight, is 1 to 2% faster, and wrong in the first
+// digit where a value 2^30 times the others has no weight.)
 constexpr int kKaWarps = 4, kKaStages = 3;
 constexpr uint32_t kKaCtas = 3, kKaGrid = 148 * kKaCtas, kKaHeads = 8;
 
@@ -535,6 +537,46 @@ SMOE_DEVINL void kv4_load_q(const void* q, size_t at, int dtype, float* x) {
     }
 }
 
+// New powers of two of a group's sums o (heads 2 cl, 2 cl + 1 of this lane),
+// where the page's scales do not fit the old ones: the larger of its largest
+// p s and an eighth of the largest sum so far goes near 2^8. (What is lost
+// stays below 2^-32 of the larger one; sums in fp32 have room above.) Bounded
+// so that no scale of the page, the largest being `big`, and no factor of the
+// sums passes fp32.
+SMOE_DEVINL void kv4_new_up(const uint8_t* scales, uint32_t big, uint32_t gr, const float (&x)[4][4], float (&o)[4][4], float (&up)[2]) {
+    float y[2] = {0.0f, 0.0f}, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        const float s0 = fabsf(lo_f(*reinterpret_cast<const uint32_t*>(scales + (mt * 16 + gr) * 4)));
+        const float s1 = fabsf(lo_f(*reinterpret_cast<const uint32_t*>(scales + (mt * 16 + 8 + gr) * 4)));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            y[k] = fmaxf(y[k], fmaxf(x[mt][k] * s0, x[mt][2 + k] * s1));
+            sum[k] = fmaxf(sum[k], fmaxf(fabsf(o[mt][k]), fabsf(o[mt][2 + k])));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            y[k] = fmaxf(y[k], __shfl_xor_sync(0xffffffffu, y[k], d));
+            sum[k] = fmaxf(sum[k], __shfl_xor_sync(0xffffffffu, sum[k], d));
+        }
+        const int was = int(__float_as_uint(up[k]) >> 23);       // biased exponents; 0: none yet
+        const float top = fmaxf(y[k], was ? sum[k] * 0.125f / up[k] : 0.0f);
+        int now = min(262 - int(__float_as_uint(top) >> 23), 373 - int(big >> 7));
+        if (was) now = min(now, was + 100);
+        now = max(1, min(227, now));
+        const float next = __uint_as_float(uint32_t(now) << 23), r = was ? next / up[k] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j][k] *= r;
+            o[j][2 + k] *= r;
+        }
+        up[k] = next;
+    }
+}
+
 template <int NG>
 constexpr uint32_t kv4_attn_smem() { return kKaWarps * kKaStages * (NG * 2304 + 8); }
 
@@ -595,7 +637,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
 
     uint32_t qf[NG][4][QP][2];                   // fragments of q: head gr, dimensions in the order kv4_half_codes gives the codes
     float qsm[NG][2], sc[2];                     // of the heads 2 cl, 2 cl + 1: the groups' sums; scale_log2 over the head's power of two
-    float m[2], l[2], bacc[NG][2], o[NG][4][4], up[NG];          // up: the group's power of two in o
+    float m[2], l[2], bacc[NG][2], o[NG][4][4], up[NG][2];       // up: the power of two of the group's sums in o, for each head
     bool failed = false, fresh = true;           // fresh: the pair starts with this page
     uint32_t heads = 0, head0 = 0;               // of the pair: query heads and the first of them
     float* lrow = nullptr;
@@ -659,7 +701,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
                     }
                 sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
                 sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-                up[g] = 0.0f;
+                up[g][0] = up[g][1] = 0.0f;
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -794,20 +836,25 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             __syncwarp();
             fence_proxy_async();                 // (the slot goes to a bulk copy next)
         }
-        // the power of two of a group's p s: its largest scale near 2^3, and below
-        // 2^7 as pages follow, so that with p <= 2^8 nothing passes fp16's range
+        // The power of two of a group's p s for a head. While the page's scales
+        // times it lie in [2^-2, 2^7] nothing passes fp16's range (p <= 2^8), and
+        // what the pieces lose, 2^-25, is below 2^-22 of the entry with p = 1. A
+        // pair's first page puts its largest scale near 2^3; where scales differ
+        // more, kv4_new_up goes by the products themselves, for a large scale may
+        // have no weight.
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const uint2 w = *reinterpret_cast<const uint2*>(blk + SB + g * 256 + lane * 8);
-            const uint32_t big = __reduce_max_sync(0xffffffffu, max(w.x & 0x7fffu, w.y & 0x7fffu));
-            if (__uint_as_float(big << 16) * up[g] > 128.0f || up[g] == 0.0f) {
-                const float now = __uint_as_float(uint32_t(max(27, min(227, 257 - int(big >> 7)))) << 23);
-                const float r = up[g] == 0.0f ? 0.0f : now / up[g];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[g][j][k] *= r;
-                up[g] = now;
+            const uint32_t s0 = w.x & 0x7fffu, s1 = w.y & 0x7fffu, big = __reduce_max_sync(0xffffffffu, max(s0, s1));
+            const uint32_t low = __reduce_min_sync(0xffffffffu, min(s0 - 1, s1 - 1)) + 1;        // (of those that are not 0)
+            const float hi = __uint_as_float(big << 16), lo = __uint_as_float(min(big, low) << 16);
+            const bool fits = hi * fmaxf(up[g][0], up[g][1]) <= 128.0f && lo * fminf(up[g][0], up[g][1]) >= 0.25f;
+            if (!__all_sync(0xffffffffu, fits || big == 0)) {
+                if (up[g][0] == 0.0f && hi <= 32.0f * lo) {      // (a pair's first page: no head has one yet)
+                    up[g][0] = up[g][1] = __uint_as_float(uint32_t(max(1, min(227, 257 - int(big >> 7)))) << 23);
+                } else {
+                    kv4_new_up(blk + SB + g * 256, big, gr, x, o[g], up[g]);
+                }
             }
         }
 #pragma unroll
@@ -817,7 +864,8 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             for (int g = 0; g < NG; ++g) {
                 const uint32_t sa = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + ka * 4);
                 const uint32_t sb = *reinterpret_cast<const uint32_t*>(blk + SB + g * 256 + kb * 4);
-                const float b0 = fmaf(8.0f, lo_f(sa), hi_f(sa)), b1 = fmaf(8.0f, lo_f(sb), hi_f(sb)), s0 = lo_f(sa) * up[g], s1 = lo_f(sb) * up[g];
+                const float b0 = fmaf(8.0f, lo_f(sa), hi_f(sa)), b1 = fmaf(8.0f, lo_f(sb), hi_f(sb));
+                const float s0[2] = {lo_f(sa) * up[g][0], lo_f(sa) * up[g][1]}, s1[2] = {lo_f(sb) * up[g][0], lo_f(sb) * up[g][1]};
                 // codes of this lane's 8 dimensions (8 gr ..) of the entries 2 cl, 2 cl + 1, 2 cl + 8, 2 cl + 9 of the tile;
                 // lanes cl >= 2 load the pair the other way round (the four entries of a load then lie in different banks)
                 uint32_t w[4];
@@ -833,7 +881,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
                 kv4_half_codes(__byte_perm(w[2], w[3], p_hi), c1 + 4);
                 bacc[g][0] = fmaf(x[mt][0], b0, fmaf(x[mt][2], b1, bacc[g][0]));
                 bacc[g][1] = fmaf(x[mt][1], b0, fmaf(x[mt][3], b1, bacc[g][1]));
-                const float y0 = x[mt][0] * s0, y1 = x[mt][1] * s0, y2 = x[mt][2] * s1, y3 = x[mt][3] * s1;
+                const float y0 = x[mt][0] * s0[0], y1 = x[mt][1] * s0[1], y2 = x[mt][2] * s1[0], y3 = x[mt][3] * s1[1];
                 const uint32_t u0 = cvt_f16x2(y0, y1), u1 = cvt_f16x2(y2, y3);
                 const uint32_t v0 = movm_trans(cvt_f16x2(y0 - half_lo(u0), y1 - half_hi(u0)));
                 const uint32_t v1 = movm_trans(cvt_f16x2(y2 - half_lo(u1), y3 - half_hi(u1)));
@@ -870,7 +918,7 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
                 const float inv = 1.0f / l[k];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const float down = up[g] == 0.0f ? 0.0f : 1.0f / up[g];      // (exact: a power of two)
+                    const float down = up[g][k] == 0.0f ? 0.0f : 1.0f / up[g][k];                // (exact: a power of two)
                     float v[8];                  // dimensions 8 gr .. of the group
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {

@@ -319,3 +319,61 @@ def test_kv4_advance_reports_a_range_that_runs_backwards(ctx):
     with pytest.raises(S.SmoeCudaError, match="ERR_DEVICE"):
         ctx.synchronize()
     assert lens.tolist() == [14, 20, 37] and seen.tolist() == [15, 21, 38]
+
+
+# ----------------------------------------------------------- accuracy of decode
+def test_kv4_attention_accuracy(ctx):
+    """fp32 results over ordinary rows: norm of the error within 2^-19 of the result's. (Scores of magnitude up to 8 in
+    units of log2 take some six roundings of 2^-24 of that: 7e-7 rms of a probability, likewise of the result; products
+    of codes that are not centred would be at 2.8e-6.)"""
+    lens = [1000, 300, 64, 777]
+    c = T.Cache(4, 128, lens, 1, 530)
+    c.fill(ctx)
+    q = torch.randn(4, 32, 128, generator=c.g, device="cuda") * 2
+    out, _ = attn_run(ctx, c, q, 1000)
+    want = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        k, v = c.values(b, n)
+        p = torch.softmax(torch.einsum("kgd,nkd->kgn", q[b].double().view(4, -1, 128), k) / math.sqrt(128), -1)
+        want[b] = torch.einsum("kgn,nkd->kgd", p, v).reshape(32, 128)
+    assert float((out.double() - want).norm() / want.norm()) <= 2 ** -19
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd,n", [(128, 700), (64, 30000), (128, 30000)])      # a page a warp; three
+@pytest.mark.parametrize("kind", ["no weight", "some weight", "own head", "later maximum"])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 30, 2.0 ** 100])
+def test_kv4_attention_outliers(ctx, dtype, hd, n, kind, size):
+    """Values that are much larger than all others but have (almost) no weight leave the result as exact as without them.
+    A score in fp32 is off by some 4 x 2^-24 of its products' magnitudes, and a probability by that in units of log2. They
+    add up to 16 where outliers have no weight (2^-18 of the magnitude); to 100 where outliers of some weight decide the
+    result (2^-15); to 900 where a score of 212 or 300 does (2^-12)."""
+    Hkv, H = 8, 24
+    c = T.Cache(Hkv, hd, [n], 1, 540)
+    g = c.g
+    k, v = (torch.randn(n, Hkv, hd, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(1, H, hd, generator=g, device="cuda")
+    q[..., 0] = 6.0                      # dimension 0 sets the scores: 6 k[0] / sqrt(hd)
+    page = torch.arange(0, n - 63, 64, device="cuda")
+    slot = torch.randint(0, 64, page.shape, generator=g, device="cuda")
+    at = (page + slot)[::5]              # every fifth page has an outlier
+    unit = math.sqrt(hd) / 6
+    if kind == "later maximum":          # every third page has a key that is 300 above, the outliers' pages come before it
+        at = (page + slot)[::3]
+        k[(page + slot)[2::3], :, 0] = 300 * unit
+    else:
+        k[at, :, 0] = (-14 if kind == "some weight" else -212) * unit
+    if kind == "own head":
+        at = at[len(at) // 2:][:1]
+        q[0, 5, 0] = q[0, 13, 0] = -6.0  # this one decides
+    v[at] *= size
+    ctx.kv4_append(c.desc(), S.kv4_rows(k, v, starts([n])))
+    c.len += n
+    q = q.to(dtype)
+    out, _ = attn_run(ctx, c, q, n)
+    kk, vv = c.values(0, n)
+    p = torch.softmax(torch.einsum("kgd,nkd->kgn", q[0].double().view(Hkv, -1, hd), kk) / math.sqrt(hd), -1)
+    want, mag = (torch.einsum("kgn,nkd->kgd", p, x).reshape(H, hd) for x in (vv, vv.abs()))
+    assert torch.isfinite(out).all()
+    bar = 2 ** (-18 if kind == "no weight" else -15 if kind == "some weight" else -12)
+    assert ((out[0].double() - want).abs() <= bar * mag + (2 ** -8 * want.abs() if dtype == BF16 else 0)).all()
