@@ -481,9 +481,12 @@ int smoe_cuda_decode_advance_batch(SmoeCudaCtx* ctx, SmoeSamplerRow* rows, uint3
  * counterpart in the reference, which keeps one fp32 ring per sequence
  * (decode.hpp:34) and prefills one sequence at a time (prefill.cpp:82-465).
  * All pointers are device pointers; calls are asynchronous on the context
- * stream and allocate nothing, so they can be captured in a CUDA graph. Row
- * ranges, lengths and page numbers are read on the device: one outside its
- * buffer is skipped and raises SMOE_ERR_DEVICE at the next synchronize. */
+ * stream and allocate nothing, so they can be captured in a CUDA graph. The
+ * cache's calls work in the caller's workspace; packed attention works in 41 MB
+ * of the context's, so the calls of one context, replayed graphs among them,
+ * must not run at the same time. Row ranges, lengths and page numbers are read
+ * on the device: one outside its buffer is skipped and raises SMOE_ERR_DEVICE
+ * at the next synchronize. */
 
 /* Attention of packed prompts. Sequence s has the q / out rows
  * [cu_q[s], cu_q[s+1]) and the k / v rows [cu_k[s], cu_k[s+1]); query head h
@@ -610,7 +613,10 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
  * `keep` are that recent, the lowest `keep` entries of them stay). Kept
  * entries below `keep` stay where they are; the j-th kept entry past it moves
  * to the j-th free one below it, K, V, pos and score. Entries past `keep` are
- * left as they are.
+ * left as they are. (Entries are then not in the order of their positions: a
+ * window over rows read back counts entries. Scores that no attention has
+ * added to yet are 0 and tie: of a fresh prompt the last `recent` and the
+ * oldest stay.)
  * pos_out / score_out NULL: pos and score are updated in place; else those of
  * all entries below min(len, keep) are written there (distinct arrays, same
  * layout) and cache->pos / score stay. len stays (smoe_cuda_kv4_advance cuts

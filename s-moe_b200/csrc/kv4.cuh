@@ -380,9 +380,9 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // codes' unpacking on the integer units, the probabilities' pieces), a page
 // takes a warp 5 us, and the 12 warps an SM that their registers allow use 53%
 // of the issue slots. Two contexts of 125,000 (head_dim 128, 32 / 4 heads,
-// bf16, weights): 65 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
+// bf16, weights): 66 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
 // rings run; the first pages come in after 7 us, warps end between 37 and 56).
-// 32 contexts of 512 to 8,192: 33 us with the join; one of 300: 10.8 us, of
+// 32 contexts of 512 to 8,192: 33 us with the join; one of 300: 11 us, of
 // which most is the two launches. (A power of two per group alone, by the
 // largest scale whatever its weight, is 1 to 2% faster, and wrong in the first
 // digit where a value 2^30 times the others has no weight.)
@@ -418,10 +418,13 @@ SMOE_DEVINL uint32_t kv4_pages(uint32_t n) { return (n + kKvPage - 1) / kKvPage;
 // The line of pages: sequence s starts at heads * (pages of the sequences
 // before it), `heads` pairs of equal length each. (Below 2^31 pages: the host
 // refuses more.)
-// Stretches are equal up to a page. Short ones are all rounded up instead,
-// which leaves some warps without: they cut fewer pairs (32 contexts of 512 to
-// 8,192, 4.9 pages a warp: 33.1 us, and 34.4 without rounding; two of 125,000,
-// 8.8 pages a warp: 68.8 and 65.5).
+// Stretches are equal up to a page. Short ones, below 8 pages, are all rounded
+// up instead, which leaves some warps without: they cut fewer pairs. 2, 32 and
+// 100 contexts with weights, head_dim 128, call after call: rounding takes 3 to
+// 13% less at 1.5 to 3.5 pages a warp, 1 to 7% at 4.5 to 6.5, 0 to 8% at 7.5,
+// the same at 8.8, and 2 to 3% more at 10.5 and 14.5. (Without weights it stays ahead
+// there for 32 and 100 contexts. One call by itself over cold caches: ahead at
+// 1.5, the same at 3, 2 to 4% behind from 4.5 on.)
 struct Kv4Line {
     uint32_t total, each, more;                  // pages; pages of a stretch, the first `more` of them have one more
     SMOE_DEVINL Kv4Line(uint32_t pages, uint32_t warps) : total(pages), each(pages / warps), more(pages % warps) {
@@ -512,7 +515,7 @@ SMOE_DEVINL float half_hi(uint32_t x) { return __half2float(__ushort_as_half(uin
 SMOE_DEVINL float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 SMOE_DEVINL float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// 16 consecutive values of a head's group, times `up`.
+// 16 consecutive values of a head's group.
 SMOE_DEVINL void kv4_load_q(const void* q, size_t at, int dtype, float* x) {
     if (dtype == SMOE_DTYPE_F32) {
         const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
@@ -1132,9 +1135,9 @@ constexpr uint32_t kKvLate = 0xffffffffu;        // key of an entry that stays f
 //     another writes. (Separate outputs have pos and score of all entries
 //     below `keep` from step 1, before the moved ones' overwrite them.)
 // Bound by the chain of steps for short sequences (8 of 1,100 entries cut to
-// 1,024, 4 KV heads: 10.1 us; 12.7 with 32 moves a warp) and by the moves for
+// 1,024, 4 KV heads: 10.3 us; 12.7 with 32 moves a warp) and by the moves for
 // long ones (16 of 6,000 to 32,768 cut to 4,096: 56 us, of which the selection
-// takes 18; the moves' 32-byte sectors pass at about 6 TB/s, as far as memory
+// takes 15; the moves' 32-byte sectors pass at about 6 TB/s, as far as memory
 // goes). One launch: with a launch a step the first took 37 us, the second 244.
 constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32, kEvDigits = 3;
 constexpr uint32_t kEvBins = 2048, kEvCtas = 8;  // of a cluster, at most

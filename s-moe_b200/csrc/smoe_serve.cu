@@ -215,8 +215,9 @@ int smoe_cuda_attention_packed(SmoeCudaCtx* ctx, const SmoeCudaPackedAttnArgs* a
     const uint64_t pairs = uint64_t(a->total_q) / (2 * p.tokens) + std::min(a->n_seqs, a->total_q), ctas = pairs * a->num_kv_heads;
     if (ctas > 0x7fffffffu) return ctx_fail(SMOE_ERR_UNSUPPORTED, "packed attention: more than 2^31 tile pairs", long(ctas));
     const uint64_t most = pairs * (uint64_t(a->total_k) / smoe::kPaKeys + 3);
-    // A CTA per pair when all of them fit the GPU at once and none is long: the plan and the joining of cut pairs cost
-    // some 6 us. (Above 65,536 pairs, or 2^31 blocks, too.)
+    // A CTA per pair when all of them fit the GPU at once and the keys of the whole call are few - the sequences' own lengths
+    // are on the device - so that no pair can be long: the plan and the joining of cut pairs cost some 6 us. (Above 65,536
+    // pairs, or 2^31 blocks, too.)
     const bool direct = (ctas <= uint64_t(c.num_sms) && a->total_k <= 16 * smoe::kPaKeys) || pairs > smoe::kPaMaxPairs || most >= (uint64_t(1) << 31);
     const bool sorted = !direct && ctas >= uint64_t(4) * c.num_sms;
     const PackedScratch sc(c.num_sms);
