@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kKwThreads) k_kv4_read(Kv4Args a, const uint32
 // codes' unpacking on the integer units, the probabilities' pieces), a page
 // takes a warp 5 us, and the 12 warps an SM that their registers allow use 53%
 // of the issue slots. Two contexts of 125,000 (head_dim 128, 32 / 4 heads,
-// bf16, weights): 66 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
+// bf16, weights): 64 us with the join for 156 MB, 2.4 TB/s (3.9 TB/s once the
 // rings run; the first pages come in after 7 us, warps end between 37 and 56).
 // 32 contexts of 512 to 8,192: 33 us with the join; one of 300: 11 us, of
 // which most is the two launches. (A power of two per group alone, by the
@@ -418,17 +418,15 @@ SMOE_DEVINL uint32_t kv4_pages(uint32_t n) { return (n + kKvPage - 1) / kKvPage;
 // The line of pages: sequence s starts at heads * (pages of the sequences
 // before it), `heads` pairs of equal length each. (Below 2^31 pages: the host
 // refuses more.)
-// Stretches are equal up to a page. Short ones, below 8 pages, are all rounded
-// up instead, which leaves some warps without: they cut fewer pairs. 2, 32 and
-// 100 contexts with weights, head_dim 128, call after call: rounding takes 3 to
-// 13% less at 1.5 to 3.5 pages a warp, 1 to 7% at 4.5 to 6.5, 0 to 8% at 7.5,
-// the same at 8.8, and 2 to 3% more at 10.5 and 14.5. (Without weights it stays ahead
-// there for 32 and 100 contexts. One call by itself over cold caches: ahead at
-// 1.5, the same at 3, 2 to 4% behind from 4.5 on.)
+// Stretches are equal up to a page. Those below 3 pages are all rounded up
+// instead, which leaves some warps without: they cut fewer pairs. 2, 32 and 100
+// contexts, head_dim 128, call after call: rounding takes 2 to 8% less at 1.5
+// pages a warp, from 1.5% less to 4% more at 3.5 and 4.9, and 2 to 5% more at
+// 6.5 to 14.5.
 struct Kv4Line {
     uint32_t total, each, more;                  // pages; pages of a stretch, the first `more` of them have one more
     SMOE_DEVINL Kv4Line(uint32_t pages, uint32_t warps) : total(pages), each(pages / warps), more(pages % warps) {
-        if (each < 8) {
+        if (each < 3) {
             each = max(1u, each + (more != 0));
             more = 0;
         }
@@ -593,7 +591,6 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
     const uint32_t me = blockIdx.x * kKaWarps + warp, nheads = c.num_kv_heads * p.chunks;        // pairs of a sequence
     uint8_t* ring = kv4_smem + warp * kKaStages * UNIT;
     uint64_t* bars = reinterpret_cast<uint64_t*>(kv4_smem + kKaWarps * kKaStages * UNIT) + warp * kKaStages;
-    pdl_release();
     if (lane == 0) {
         for (int i = 0; i < kKaStages; ++i) mbar_init(bars + i, 1);
         fence_mbar_init();
@@ -959,6 +956,11 @@ __global__ void __launch_bounds__(kKaWarps * 32, kKaCtas) k_kv4_attention(const 
             }
         }
     }
+    // Released here, and by k_kv4_join not before its end: CTAs of the next call
+    // that are resident beside those of this one or of the join end up two and
+    // not three on some SMs, and the rest run after all others (32 contexts, 14
+    // pages a warp, no weights: 112 us a call instead of 80).
+    pdl_release();
     if (failed)                                  // no copy may be in flight when the CTA ends
         for (uint32_t u = 2 * mine > uint32_t(kKaStages) ? 2 * mine - kKaStages : 0u; u < 2 * mine; ++u)
             mbar_wait_bounded(bars + u % kKaStages, (u / kKaStages) & 1);
@@ -979,7 +981,6 @@ __global__ void __launch_bounds__(kKjThreads) k_kv4_join(const Kv4Attn p, uint32
     extern __shared__ float2 kv4_stat[];         // [chunks][heads] maximum; 1 / sum (outputs) or log2 of the sum (weights)
     __shared__ float2 red[kKjThreads];
     __shared__ float4 part_v[kKjThreads];
-    pdl_release();
     pdl_acquire();
     const SmoeKv4Cache& c = p.a.c;
     const uint32_t kvh = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, HD = c.head_dim;

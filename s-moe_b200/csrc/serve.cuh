@@ -24,7 +24,8 @@ int ctx_fail(int code, const char* msg, long v);         // sets the message of 
 
 // Programmatic dependent launch: the next kernel of the stream may start its
 // set-up while this one runs; it waits for this one's end before it touches
-// memory. Every kernel of these entries calls both.
+// memory. Every kernel of these entries waits, and all release their dependents
+// at once but the cache attention (at its end) and its join (by its end).
 SMOE_DEVINL void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 SMOE_DEVINL void pdl_acquire() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
