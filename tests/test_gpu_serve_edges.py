@@ -166,6 +166,28 @@ def test_packed_attention_no_keys_at_all(ctx):
         assert (out == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("rows,H,Hkv", [(100, 8, 2), (700, 16, 2), (6000, 32, 4)])     # each of the call's paths
+def test_packed_attention_sequences_without_rows(ctx, rows, H, Hkv):
+    """Rows and keys that belong to no sequence: nothing is written."""
+    q, k, v = T.packed_inputs([(rows, rows + 1000)], H, Hkv, 64, 640)
+    out = torch.full_like(q, 7.0)
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    ctx.attention_packed(S.packed_attn_args(q, k, v, out, ints([0, 0, 0]), lse=lse))
+    ctx.attention_packed(S.packed_attn_args(q, k, v, out, ints([rows] * 4), ints([0, 9, 9, rows]), lse=lse))
+    ctx.synchronize()
+    assert (out == 7).all() and (lse == 7).all()
+
+
+@pytest.mark.parametrize("score", [False, True])
+def test_kv4_attention_empty_sequences(ctx, score):
+    """No sequence has an entry: zeros, and no weight is written."""
+    c = T.Cache(2, 128, [0, 0, 0], 1, 641)
+    q = torch.randn(3, 8, 128, device="cuda")
+    for max_len in (0, 5000):
+        out, so = attn_run(ctx, c, q, max_len, score=score)
+        assert (out == 0).all() and (so is None or (so == -1).all())
+
+
 # --------------------------------------------------------------------- limits
 def test_limits(ctx):
     """Shapes past what a launch takes are refused before anything runs; 6,144 query heads on one KV head are served."""
