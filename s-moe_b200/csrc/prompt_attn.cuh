@@ -30,12 +30,13 @@ namespace smoe {
 // memory as bf16 (over the scores) and are the left operand of the second
 // product, which takes both operands of one type, the values'. Their sum and
 // the lse are taken before that rounding. (Results are 1.8e-3 to 2.2e-3 from
-// 64 bits, with fp32 probabilities 1.6e-3 to 1.7e-3.) A block of 64 keys takes a tile pair 1,800 cycles, of which the
-// exponentials' unit needs 1,024 (its two tiles take it by turns, 900 each)
-// and the tensor cores 1,060. 16,384 causal tokens of 32 / 4 heads of 128:
-// 1.75 ms, 1,260 TFLOP/s in short runs, 1.97 ms, 1,117 for seconds on end (the
-// power limit); 24 prompts of 17 to 2,048: 180 us, 826 TFLOP/s, and 190, 782;
-// 4 x 200..512 tokens over 6,000 keys, heads of 64: 36 us; 45 tokens: 8.4 us.
+// 64 bits, with fp32 probabilities 1.6e-3 to 1.7e-3.) A block of 64 keys
+// takes a tile pair 1,800 cycles, of which the exponentials' unit needs 1,024
+// (its two tiles take it by turns, 900 each) and the tensor cores 1,060.
+// 16,384 causal tokens of 32 / 4 heads of 128: 1.75 ms, 1,260 TFLOP/s in
+// short runs, 1.97 ms, 1,117 for seconds on end (the power limit); 24 prompts
+// of 17 to 2,048: 180 us, 826 TFLOP/s, and 190, 782; 4 x 200..512 tokens over
+// 6,000 keys, heads of 64: 36 us; 45 tokens: 8.4 us.
 // (Without turns 1.05 times as long; part of the exponentials by polynomial,
 // chunks of 16 were no faster.)
 constexpr uint32_t kPaRows = 128, kPaKeys = 64;

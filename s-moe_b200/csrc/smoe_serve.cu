@@ -320,7 +320,7 @@ int smoe_cuda_kv4_attention(SmoeCudaCtx* ctx, const SmoeKv4Cache* cache, const S
     p.rows = plan.rows;
     // (a scale of 0 must still keep the masked scores' -inf: 1e-35 times any finite score is 0 to the exponential)
     p.scale_log2 = std::max(t->scale * 1.4426950408889634f, 1e-35f);
-    p.most_e = std::min(100, std::ilogb(p.scale_log2) + 126);
+    p.most_e = std::min(100, std::ilogb(std::min(p.scale_log2, 1e30f)) + 126);
     auto run = [&](auto kern, uint32_t smem) -> int {
         const int r = smem_limit(c, kern, smem);
         return r ? r : launch(c, kern, dim3(smoe::kKaGrid), dim3(smoe::kKaWarps * 32), smem, p);

@@ -9,6 +9,7 @@ libsmoe_cuda.so is missing or no GPU is present, calls raise.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -501,9 +502,10 @@ class Context:
 
 
 def _u32(x, name) -> int:
-    if not 0 <= x < 1 << 32:
+    n = operator.index(x)
+    if not 0 <= n < 1 << 32:
         raise ValueError(f"{name}: {x} is not in the range of 32 bits")
-    return int(x)
+    return n
 
 
 def _need_gpu(t, name):
@@ -607,9 +609,9 @@ def packed_attn_args(q, k, v, out, cu_q, cu_k=None, scale=None, causal=True, win
     """Arguments of Context.attention_packed from torch tensors: q, out
     [total_q, heads, head_dim], k, v [total_k, kv_heads, head_dim] (bf16, row
     and head strides that are multiples of 8; k and v may be expanded over
-    their heads, nothing else may be expanded), cu_q / cu_k [n_seqs + 1] int32, lse [total_q,
-    heads] fp32. scale: 1 / sqrt(head_dim) by default. The tensors must stay
-    alive while the structure is used."""
+    their heads, nothing else may be expanded), cu_q / cu_k [n_seqs + 1]
+    int32, lse [total_q, heads] fp32. scale: 1 / sqrt(head_dim) by default.
+    The tensors must stay alive while the structure is used."""
     import torch
     a = PackedAttnArgs()
     for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
